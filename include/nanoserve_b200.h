@@ -329,6 +329,68 @@ int b2_rope_kv_store_tp(void* qkv, const void* bias, const void* inv_freq, const
  * (a norm, a sampler): kernels after it on the stream see the gathered rows complete. */
 int b2_tp_wait(const void* wait_sig, const void* epoch, unsigned wait_per_epoch, void* stream);
 
+/*
+ * Serving several sequences: a paged key/value cache, attention over it, and sampling.  No counterpart in the reference library
+ * (it serves one sequence from a contiguous cache, greedily).
+ *
+ * b2_paged_cache: pages of `page_size` tokens (a power of two, 16 to 1024) in two arrays that share one layout: the row of head h
+ * at token s of page p is the head_dim values from p * page_stride + h * head_stride + s * token_stride on (elements, multiples of
+ * 8; k and v 16-byte aligned), so pages may be [head, token, dim] or [token, head, dim], or parts of larger tensors.  Token j of
+ * sequence b is in page block_table[b * table_stride + j / page_size], at j % page_size.  An entry outside 0 .. n_pages - 1, or
+ * beyond table_width, stands for a page that is not there: its keys take no part, and nothing is stored for it.
+ * seq_lens [n_seqs] (int32): the tokens of each sequence, the call's new ones included.
+ *
+ * The rows of a call, T in all, are the new tokens of sequence 0, then of sequence 1, ...; cu_tokens [n_seqs + 1] (int32, not
+ * falling) holds the first row of each sequence and the end of the last one; NULL: one row per sequence (T == n_seqs).  A
+ * sequence's n rows have the positions seq_lens[b] - n .. seq_lens[b] - 1; it may have none.  Rows behind the last sequence, and
+ * rows in front of the first, are left as they are.  Table, lengths and cu_tokens are read on the device: a captured graph may be
+ * replayed with others in the same places.
+ *
+ *   b2_paged_kv_append: qkv [T, (Hq + 2 Hk) D] (rows qkv_stride apart): + bias (may be NULL), rotate-half RoPE on q and k at the
+ *     row's position (the angle in 64 bits), one rounding to bf16; q to q_out [T, Hq D] (rows q_stride apart), k and v to the cache.
+ *     qkv is not modified.  A row whose position is negative is left out.  head_dim % 16 == 0, at most 256.
+ *   b2_paged_attention: out [T, Hq D] = softmax(scale q K^T) V; the row at position i sees the keys j <= i of its sequence and, with
+ *     window > 0, of those only j > i - window and the first `sinks`.  A row that sees no key is zero.  head_dim 64 or 128,
+ *     Hq % Hk == 0.  max_tokens: no sequence has more rows than that (rows beyond it are left as they are).
+ *   b2_shared_prefix_attention: one row per sequence, which sees the first *prefix_len (int32, on the device) tokens of the pages
+ *     prefix_table [prefix_width], and all seq_lens[b] tokens (which may be none) of its own pages.  The prefix's keys and values
+ *     are read once for all sequences.
+ *   Both take device scratch of the caller's, 16-byte aligned, of at least the bytes that the two size calls give, contents
+ *   undefined before and after; calls that may overlap in time need scratch of their own.
+ *
+ *   b2_sample: tokens [rows] (int64) from logits [rows, V] (bf16, or fp32 with fp32 != 0; rows logits_stride elements apart), one
+ *     random number u [rows] (fp32, in [0, 1)) per row.  With w_i = exp((l_i - max l) / temperature): of the logits with w_i >=
+ *     min_p the top_k largest (equal ones: the lowest index first; top_k <= 0: all), of these, in falling order, the fewest whose
+ *     weights reach top_p of theirs (at least one; top_p >= 1: all); drawn is the first of them in the order of the vocabulary at
+ *     which their weights, added up, exceed u times their sum.  Weights are held to 2^-44 of the largest.  temperature <= 0: the
+ *     largest logit, lowest index.  NaN counts as no logit; -1 where a row has no logit above minus infinity.  Each parameter is
+ *     an array [rows] on the device (top_k int32, the others fp32) or, where that is NULL, the value behind the arrays.
+ *     V <= 262144.
+ */
+typedef struct b2_paged_cache {
+  void* k;
+  void* v;
+  long long page_stride, head_stride, token_stride;
+  int n_pages, page_size, n_kv_heads, head_dim;
+  const void* block_table;
+  long long table_stride;
+  int table_width, n_seqs;
+  const void* seq_lens;
+} b2_paged_cache;
+int b2_paged_kv_append(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq, void* q_out,
+                       long long q_stride, const b2_paged_cache* cache, const void* cu_tokens, int T, int Hq, void* stream);
+size_t b2_paged_attention_workspace_bytes(int T, int n_seqs, int max_tokens, int Hq, int Hk, int D);
+int b2_paged_attention(const void* q, long long q_stride, const b2_paged_cache* cache, const void* cu_tokens, int T,
+                       int max_tokens, int Hq, int window, int sinks, float scale, void* out, long long out_stride,
+                       void* workspace, size_t workspace_bytes, void* stream);
+size_t b2_shared_prefix_workspace_bytes(int n_seqs, int Hq, int Hk, int D);
+int b2_shared_prefix_attention(const void* q, long long q_stride, const b2_paged_cache* cache, const void* prefix_table,
+                               int prefix_width, const void* prefix_len, int Hq, float scale, void* out, long long out_stride,
+                               void* workspace, size_t workspace_bytes, void* stream);
+int b2_sample(const void* logits, long long logits_stride, int fp32, int rows, int V, const void* u, const void* temperature,
+              const void* top_k, const void* top_p, const void* min_p, float temperature_all, int top_k_all, float top_p_all,
+              float min_p_all, void* tokens, void* stream);
+
 /* Library identification: "nanoserve-b200 <version> sm_100a". */
 const char* b2_version(void);
 

@@ -8,6 +8,7 @@
 
 #include "../../include/nanoserve_b200.h"
 #include "fused_ops.h"
+#include "paged.h"
 #include "w4_internal.h"
 
 namespace {
@@ -138,6 +139,58 @@ int to_gemv_tp(const b2_tp_desc* tp, b2::GemvTp* out) {
     t.announce_peer[r] = static_cast<unsigned*>(tp->announce_peer[r]);
   }
   *out = t;
+  return 0;
+}
+
+}  // namespace
+
+namespace {
+
+// The SM count alone, for calls that need nothing else of the device's state.
+int sm_count_of_device(int* rc) {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = -1, n = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) { *rc = b2::kErrTooLarge; return 0; }
+  if (e == cudaSuccess && (n = known[dev].load(std::memory_order_relaxed)) == 0) {
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) known[dev].store(n, std::memory_order_relaxed);
+  }
+  *rc = (int)e;
+  return e == cudaSuccess ? n : 0;
+}
+
+// The public description of a paged cache, checked.
+int to_paged(const b2_paged_cache* c, b2::PagedCache* out) {
+  if (!c) return b2::kErrBadPointer;
+  if (c->n_pages < 1 || c->n_kv_heads < 1 || c->n_seqs < 1 || c->table_width < 1 || c->head_dim < 16 || c->head_dim > 256 ||
+      c->head_dim % 16 || c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+    return b2::kErrBadShape;
+  // (a stride of 0 or below would lay rows over one another; where there is one page, its stride says nothing)
+  if (c->page_stride % 8 || c->head_stride % 8 || c->token_stride % 8 || c->page_stride < 0 || c->head_stride < c->head_dim ||
+      c->token_stride < c->head_dim || c->table_stride < (c->n_seqs > 1 ? c->table_width : 0))
+    return b2::kErrBadShape;
+  if ((long long)c->table_width * c->page_size > (1LL << 30)) return b2::kErrTooLarge;  // positions are 32-bit
+  auto off = [](const void* p, uintptr_t to) { return !p || (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; };
+  if (off(c->k, 16) || off(c->v, 16) || off(c->block_table, 4) || off(c->seq_lens, 4)) return b2::kErrBadPointer;
+  b2::PagedCache r;
+  r.k = static_cast<__nv_bfloat16*>(c->k);
+  r.v = static_cast<__nv_bfloat16*>(c->v);
+  r.page_stride = c->page_stride;
+  r.head_stride = c->head_stride;
+  r.token_stride = c->token_stride;
+  r.table = static_cast<const int*>(c->block_table);
+  r.table_stride = c->table_stride;
+  r.lens = static_cast<const int*>(c->seq_lens);
+  r.n_pages = c->n_pages;
+  r.page = c->page_size;
+  r.page_shift = 0;
+  while ((1 << r.page_shift) < r.page) ++r.page_shift;
+  r.Hk = c->n_kv_heads;
+  r.D = c->head_dim;
+  r.width = c->table_width;
+  r.B = c->n_seqs;
+  *out = r;
   return 0;
 }
 
@@ -344,6 +397,73 @@ size_t b2_w4_gemv_scratch_bytes(int M, int N, int K, int G, int flags) {
   if (!st) return 0;
   if (M > 0 && plain_route(*st, nullptr, nullptr, nullptr, nullptr, M, N, K, G, flags) != kRouteGemv) return 0;
   return b2::gemv_scratch_bytes(M, N, K, G, flags, st->sm_count, st->ws.partial_bytes);
+}
+
+int b2_paged_kv_append(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq, void* q_out,
+                       long long q_stride, const b2_paged_cache* cache, const void* cu_tokens, int T, int Hq, void* stream) {
+  b2::PagedCache c;
+  if (const int bad = to_paged(cache, &c)) return bad;
+  return b2::paged_append_launch(qkv, qkv_stride, bias, inv_freq, q_out, q_stride, c, static_cast<const int*>(cu_tokens), T,
+                                 Hq, static_cast<cudaStream_t>(stream));
+}
+
+size_t b2_paged_attention_workspace_bytes(int T, int n_seqs, int max_tokens, int Hq, int Hk, int D) {
+  int rc = 0;
+  const int sms = sm_count_of_device(&rc);
+  if (rc || T < 1 || n_seqs < 1 || max_tokens < 1 || Hq < 1 || Hk < 1 || Hq % Hk || D < 1) return 0;
+  return b2::paged_attention_workspace(T, n_seqs, max_tokens, Hq, Hk, D, sms);
+}
+
+int b2_paged_attention(const void* q, long long q_stride, const b2_paged_cache* cache, const void* cu_tokens, int T,
+                       int max_tokens, int Hq, int window, int sinks, float scale, void* out, long long out_stride,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  b2::PagedCache c;
+  if (const int bad = to_paged(cache, &c)) return bad;
+  int rc = 0;
+  const int sms = sm_count_of_device(&rc);  // (what is wrong with the arguments comes before what is wrong with the device)
+  return b2::paged_attention_launch(q, q_stride, c, static_cast<const int*>(cu_tokens), T, max_tokens, Hq, window, sinks,
+                                    scale, out, out_stride, workspace, workspace_bytes, rc ? -rc : sms, static_cast<cudaStream_t>(stream));
+}
+
+size_t b2_shared_prefix_workspace_bytes(int n_seqs, int Hq, int Hk, int D) {
+  int rc = 0;
+  const int sms = sm_count_of_device(&rc);
+  if (rc || n_seqs < 1 || Hq < 1 || Hk < 1 || Hq % Hk || D < 1) return 0;
+  return b2::shared_prefix_workspace(n_seqs, Hq, Hk, D, sms);
+}
+
+int b2_shared_prefix_attention(const void* q, long long q_stride, const b2_paged_cache* cache, const void* prefix_table,
+                               int prefix_width, const void* prefix_len, int Hq, float scale, void* out, long long out_stride,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  b2::PagedCache c;
+  if (const int bad = to_paged(cache, &c)) return bad;
+  int rc = 0;
+  const int sms = sm_count_of_device(&rc);
+  return b2::shared_prefix_launch(q, q_stride, c, static_cast<const int*>(prefix_table), prefix_width,
+                                  static_cast<const int*>(prefix_len), Hq, scale, out, out_stride, workspace, workspace_bytes,
+                                  rc ? -rc : sms, static_cast<cudaStream_t>(stream));
+}
+
+int b2_sample(const void* logits, long long logits_stride, int fp32, int rows, int V, const void* u, const void* temperature,
+              const void* top_k, const void* top_p, const void* min_p, float temperature_all, int top_k_all, float top_p_all,
+              float min_p_all, void* tokens, void* stream) {
+  b2::Sampling p;
+  p.logits = logits;
+  p.stride = logits_stride;
+  p.fp32 = fp32;
+  p.rows = rows;
+  p.V = V;
+  p.u = static_cast<const float*>(u);
+  p.temperature = static_cast<const float*>(temperature);
+  p.top_k = static_cast<const int*>(top_k);
+  p.top_p = static_cast<const float*>(top_p);
+  p.min_p = static_cast<const float*>(min_p);
+  p.temperature_all = temperature_all;
+  p.top_k_all = top_k_all;
+  p.top_p_all = top_p_all;
+  p.min_p_all = min_p_all;
+  p.tokens = static_cast<long long*>(tokens);
+  return b2::sample_launch(p, static_cast<cudaStream_t>(stream));
 }
 
 const char* b2_version(void) { return "nanoserve-b200 0.1 sm_100a"; }

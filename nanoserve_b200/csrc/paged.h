@@ -1,0 +1,48 @@
+// Host-side declarations of the operators of batched serving: the paged cache's append, attention over it, and sampling.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+namespace b2 {
+
+// b2_paged_cache as the kernels take it (checked by paged_cache_check).
+struct PagedCache {
+  __nv_bfloat16* k;
+  __nv_bfloat16* v;
+  long long page_stride, head_stride, token_stride;  // elements
+  const int* table;
+  long long table_stride;  // entries
+  const int* lens;
+  int n_pages, page, page_shift, Hk, D, width, B;
+};
+
+struct Sampling {
+  const void* logits;
+  long long stride;  // elements between rows
+  int fp32, rows, V;
+  const float* u;
+  const float* temperature;  // null: the value beside it for every row
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all, top_p_all, min_p_all;
+  int top_k_all;
+  long long* tokens;
+};
+
+int paged_append_launch(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq, void* q_out,
+                        long long q_stride, const PagedCache& c, const int* cu_tokens, int T, int Hq, cudaStream_t s);
+// sm_count below 1: minus the error that the device gave, returned once the arguments are found right.
+int paged_attention_launch(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int T,
+                           int max_tokens, int Hq, int window, int sinks, float scale, void* out, long long out_stride,
+                           void* workspace, size_t workspace_bytes, int sm_count, cudaStream_t s);
+size_t paged_attention_workspace(int T, int B, int max_tokens, int Hq, int Hk, int D, int sm_count);
+int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c, const int* prefix_table,
+                         int prefix_width, const int* prefix_len, int Hq, float scale, void* out, long long out_stride,
+                         void* workspace, size_t workspace_bytes, int sm_count, cudaStream_t s);
+size_t shared_prefix_workspace(int B, int Hq, int Hk, int D, int sm_count);
+int sample_launch(const Sampling& p, cudaStream_t s);
+
+}  // namespace b2

@@ -86,6 +86,13 @@ SIGNATURES = {
     "b2_decode_attention_fused_workspace_bytes": ([_i32, _i32, _i32], ctypes.c_size_t),
     "b2_rope_kv_store_tp": ([_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, ctypes.c_uint, _vp], _i32),
     "b2_tp_wait": ([_vp, _vp, ctypes.c_uint, _vp], _i32),
+    "b2_paged_kv_append": ([_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp], _i32),
+    "b2_paged_attention_workspace_bytes": ([_i32] * 6, ctypes.c_size_t),
+    "b2_paged_attention": ([_vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _vp, ctypes.c_size_t, _vp],
+                           _i32),
+    "b2_shared_prefix_workspace_bytes": ([_i32] * 4, ctypes.c_size_t),
+    "b2_shared_prefix_attention": ([_vp, _i64, _vp, _vp, _i32, _vp, _i32, _f32, _vp, _i64, _vp, ctypes.c_size_t, _vp], _i32),
+    "b2_sample": ([_vp, _i64, _i32, _i32, _i32] + [_vp] * 5 + [_f32, _i32, _f32, _f32, _vp, _vp], _i32),
     "b2_version": ([], ctypes.c_char_p),
 }
 
@@ -96,6 +103,13 @@ class TpDesc(ctypes.Structure):
                 ("seg_dst", _i32 * 3), ("y_local", _vp), ("wait_sig", _vp), ("epoch", _vp),
                 ("wait_per_epoch", ctypes.c_uint), ("defer_signal", _i32), ("announce_world", _i32),
                 ("announce_peer", _vp * 8)]
+
+
+class PagedCache(ctypes.Structure):
+    """struct b2_paged_cache of include/nanoserve_b200.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("head_stride", _i64), ("token_stride", _i64),
+                ("n_pages", _i32), ("page_size", _i32), ("n_kv_heads", _i32), ("head_dim", _i32), ("block_table", _vp),
+                ("table_stride", _i64), ("table_width", _i32), ("n_seqs", _i32), ("seq_lens", _vp)]
 
 
 def staged_x_bytes(K: int) -> int:
@@ -377,6 +391,148 @@ class Kernels:
                                  p(wn), eps, None, p(part_max), p(part_idx), idx_offset, self._stream())
         self._check(rc, "b2_lm_head")
         return logits
+
+    # ---- several sequences: a paged cache, attention over it, sampling
+    def _need(self, what, *conditions):
+        if not all(conditions):
+            raise ValueError(f"{what}: see include/nanoserve_b200.h for the shapes, types and strides it takes")
+
+    def _here(self, *tensors):
+        self._cuda(*tensors)
+        dev = torch.cuda.current_device()
+        for t in tensors:
+            if t is not None and t.device.index != dev:
+                raise RuntimeError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
+
+    def _paged(self, what, cache_k, cache_v, block_table, seq_lens, n_kv_heads, head_dim) -> PagedCache:
+        self._here(cache_k, cache_v, block_table, seq_lens)
+        n_seqs = seq_lens.numel()
+        self._need(what, cache_k.dim() == cache_v.dim() == 4, cache_k.dtype == cache_v.dtype == torch.bfloat16,
+                   cache_k.shape == cache_v.shape, cache_k.stride() == cache_v.stride(),
+                   block_table.dtype == seq_lens.dtype == torch.int32, block_table.dim() == 2, seq_lens.dim() == 1)
+        n_pages, heads, page, dim = cache_k.shape
+        sp, sh, st, sd = cache_k.stride()
+        self._need(what, heads == n_kv_heads, dim == head_dim, sd == 1 and seq_lens.is_contiguous(),
+                   block_table.shape[0] == n_seqs, block_table.stride(1) == 1 or block_table.shape[1] == 1)
+        return PagedCache(cache_k.data_ptr(), cache_v.data_ptr(), sp, sh, st, n_pages, page, heads, dim, block_table.data_ptr(),
+                          block_table.stride(0), block_table.shape[1], n_seqs, seq_lens.data_ptr())
+
+    def _rows(self, what, t, width, cu_tokens, n_seqs, rows=None):
+        """Checks rows [T, width] (unit stride within a row) and cu_tokens; returns cu_tokens' address."""
+        self._here(t, cu_tokens)
+        self._need(what, t.dim() == 2, t.dtype == torch.bfloat16, t.shape[1] == width, t.stride(1) == 1,
+                   rows is None or t.shape[0] == rows)
+        if cu_tokens is None:
+            self._need(what, t.shape[0] == n_seqs)
+            return None
+        self._need(what, cu_tokens.dtype == torch.int32, cu_tokens.is_contiguous(), cu_tokens.numel() == n_seqs + 1)
+        return cu_tokens.data_ptr()
+
+    def paged_kv_append(self, qkv, bias, inv_freq, cache_k, cache_v, block_table, seq_lens, n_heads, n_kv_heads, head_dim,
+                        cu_tokens=None, q_out=None):
+        """qkv [T, (Hq + 2 Hk) D], the new tokens of several sequences: bias, RoPE at each row's position, k and v into the
+        sequences' pages (caches [n_pages, Hk, page, D], block_table [B, width] and seq_lens [B] int32, the new tokens
+        counted).  cu_tokens [B + 1] (int32): the first row of every sequence and the end of the last; None: one row each.
+        Returns the rotated q, [T, Hq D]."""
+        what = "paged_kv_append"
+        c = self._paged(what, cache_k, cache_v, block_table, seq_lens, n_kv_heads, head_dim)
+        width = (n_heads + 2 * n_kv_heads) * head_dim
+        cu = self._rows(what, qkv, width, cu_tokens, c.n_seqs)
+        self._here(bias, inv_freq, q_out)
+        self._need(what, inv_freq.dtype == torch.float32, inv_freq.is_contiguous(), inv_freq.numel() == head_dim // 2,
+                   bias is None or bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == width)
+        T = qkv.shape[0]
+        if q_out is None:
+            q_out = torch.empty((T, n_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+        else:
+            self._rows(what, q_out, n_heads * head_dim, cu_tokens, c.n_seqs, T)
+        if T:
+            rc = self.lib.b2_paged_kv_append(qkv.data_ptr(), qkv.stride(0), None if bias is None else bias.data_ptr(),
+                                             inv_freq.data_ptr(), q_out.data_ptr(), q_out.stride(0), ctypes.byref(c), cu, T,
+                                             n_heads, self._stream())
+            self._check(rc, "b2_paged_kv_append")
+        return q_out
+
+    def paged_attention(self, q, cache_k, cache_v, block_table, seq_lens, n_heads, n_kv_heads, head_dim, cu_tokens=None,
+                        max_tokens=None, window=0, sinks=0, scale=None, out=None):
+        """q [T, Hq D], new tokens whose keys and values are in the cache already (see paged_kv_append for the arguments the
+        two share): causal attention, each row over its sequence up to itself, with `window` > 0 over the last `window` keys
+        and the first `sinks`.  max_tokens: no sequence has more rows (None: T, or 1 without cu_tokens; a close bound lets
+        short calls run the kernel for few rows).  scale: head_dim ** -0.5 unless given.  Returns [T, Hq D]."""
+        what = "paged_attention"
+        c = self._paged(what, cache_k, cache_v, block_table, seq_lens, n_kv_heads, head_dim)
+        cu = self._rows(what, q, n_heads * head_dim, cu_tokens, c.n_seqs)
+        T = q.shape[0]
+        if max_tokens is None:
+            max_tokens = 1 if cu is None else T
+        if out is None:
+            out = torch.empty((T, n_heads * head_dim), dtype=q.dtype, device=q.device)
+        else:
+            self._rows(what, out, n_heads * head_dim, cu_tokens, c.n_seqs, T)
+        if T:
+            n = self.lib.b2_paged_attention_workspace_bytes(T, c.n_seqs, max_tokens, n_heads, n_kv_heads, head_dim)
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            rc = self.lib.b2_paged_attention(q.data_ptr(), q.stride(0), ctypes.byref(c), cu, T, max_tokens, n_heads, window,
+                                             sinks, head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
+                                             out.stride(0), ws.data_ptr(), n, self._stream())
+            self._check(rc, "b2_paged_attention")
+        return out
+
+    def shared_prefix_attention(self, q, cache_k, cache_v, prefix_table, prefix_len, block_table, seq_lens, n_heads,
+                                n_kv_heads, head_dim, scale=None, out=None):
+        """q [B, Hq D], one new token per sequence: attention over the first prefix_len (int32 [1], on the device) tokens of
+        the pages prefix_table [width], which all sequences share, and over each sequence's own seq_lens[b] tokens (its new
+        one among them).  The prefix is read once for all.  Returns [B, Hq D]."""
+        what = "shared_prefix_attention"
+        c = self._paged(what, cache_k, cache_v, block_table, seq_lens, n_kv_heads, head_dim)
+        self._rows(what, q, n_heads * head_dim, None, c.n_seqs)
+        self._here(prefix_table, prefix_len)
+        self._need(what, prefix_table.dtype == prefix_len.dtype == torch.int32, prefix_table.dim() == 1,
+                   prefix_table.is_contiguous(), prefix_len.numel() == 1)
+        if out is None:
+            out = torch.empty((q.shape[0], n_heads * head_dim), dtype=q.dtype, device=q.device)
+        else:
+            self._rows(what, out, n_heads * head_dim, None, c.n_seqs)
+        n = self.lib.b2_shared_prefix_workspace_bytes(c.n_seqs, n_heads, n_kv_heads, head_dim)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        rc = self.lib.b2_shared_prefix_attention(q.data_ptr(), q.stride(0), ctypes.byref(c), prefix_table.data_ptr(),
+                                                 prefix_table.numel(), prefix_len.data_ptr(), n_heads,
+                                                 head_dim ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0),
+                                                 ws.data_ptr(), n, self._stream())
+        self._check(rc, "b2_shared_prefix_attention")
+        return out
+
+    def sample(self, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+        """One token per row of logits [B, V] (bf16 or fp32), drawn with the random numbers u [B] (fp32, in [0, 1)): of the
+        logits whose probability is at least min_p of the largest's, the top_k largest, of these the fewest that hold top_p
+        of their probability.  Each parameter is a number or a tensor [B] on the device (top_k int32, the others fp32);
+        temperature 0 picks the largest logit, top_k 0, top_p 1 and min_p 0 leave all.  Returns int64 [B]; -1 where a row
+        has no logit above minus infinity."""
+        self._here(logits, u, out)
+        self._need("sample", logits.dim() == 2, logits.dtype in (torch.bfloat16, torch.float32),
+                   logits.stride(1) == 1 or logits.shape[1] == 1)
+        B, V = logits.shape
+        row = lambda t, dtype: t.dtype == dtype and t.shape == (B,) and t.is_contiguous()
+        self._need("sample", row(u, torch.float32))
+        arrays, values = [], []
+        for t, dtype, off in ((temperature, torch.float32, 1.0), (top_k, torch.int32, 0), (top_p, torch.float32, 1.0),
+                              (min_p, torch.float32, 0.0)):
+            if isinstance(t, torch.Tensor):
+                self._here(t)
+                self._need("sample", row(t, dtype))
+                arrays.append(t.data_ptr())
+                values.append(off)
+            else:
+                arrays.append(None)
+                values.append(t)
+        if out is None:
+            out = torch.empty(B, dtype=torch.int64, device=logits.device)
+        self._need("sample", row(out, torch.int64))
+        if B:
+            rc = self.lib.b2_sample(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), B, V, u.data_ptr(),
+                                    *arrays, *values, out.data_ptr(), self._stream())
+            self._check(rc, "b2_sample")
+        return out
 
     def lm_head_blocks(self, V) -> int:
         return int(self.lib.b2_lm_head_blocks(V))
