@@ -47,6 +47,13 @@ __device__ __forceinline__ int sequence_of(const int* cu_tokens, int B, int t, i
   return t < *first ? -1 : before;
 }
 
+// The page that holds token `col` * page of a table's sequence, -1 where there is none.
+__device__ __forceinline__ int page_at(const PagedCache& c, const int* table, int width, int col) {
+  if (col >= width) return -1;
+  const int page = __ldcg(table + col);
+  return page >= 0 && page < c.n_pages ? page : -1;
+}
+
 // sin and cos of position * f, the product and its reduction by whole turns in 64 bits.
 __device__ __forceinline__ void rotation(int position, float f, float* sn, float* cs) {
   constexpr double kTurn = 6.283185307179586476925286766559;       // 2 pi to 64 bits,

@@ -3,16 +3,463 @@
 //
 //   o = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m},   s_j = scale * q . k_j,   over the keys j that the row sees,
 //
-// in one pass over the keys with the running maximum m, sum and weighted rows in 32 bits.  A row that sees nothing is zero.
+// in one pass over the keys with the running maximum m, sum and weighted rows in 32 bits; weights are rounded to bf16 for the
+// second product, as tensor cores take them (the denominator adds up the unrounded ones).  A row that sees nothing is zero.
+//
+// Here: the kernel for few rows, whose time is that of reading the keys and values once, and what joins the parts of rows
+// whose keys several CTAs shared.  paged_attention_tc.cu: the kernel for many rows.
+//
+// Few rows: the up to sixteen (token, query head) rows of a sequence that share a KV head are the M side of m16n8k16 products.
+// Work is counted in blocks of 64 keys over all sequences and KV heads, and every CTA takes an equal run of them, wherever
+// sequences begin and end: a batch of ragged lengths leaves no SM waiting for its longest member.  The lengths are on the
+// device, so every CTA adds them up for itself.  One warp keeps TMA loads of the pages' rows in flight (a ring of up to
+// 192 KB per SM); each of four warps takes sixteen keys of a block, with a maximum, sum and 16 x D of its own, joined at the
+// end of a run.
+#include <algorithm>
 #include <cfloat>
 
-#include "paged.h"
-#include "paged.cuh"
+#include "paged_attention.cuh"
+#include "paged_rows.cuh"
+#include "ptx.cuh"
+#include "tensor_map.h"
 #include "w4_internal.h"
 
 namespace b2 {
 namespace {
 
+constexpr int kKeys = 64;       // keys per block
+constexpr int kRows = 16;       // rows of a tile
+constexpr int kWarps = 4;       // each takes sixteen keys of a block
+constexpr int kThreads = 32 * (kWarps + 1);
+
+template <int D>
+struct Geo {
+  static constexpr int kTile = kKeys * D * 2;                 // K (or V) of a block
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kStages = D == 128 ? 6 : 12;
+  static constexpr int kJoin = kStages * kStage;              // the warps' 16 x D sums, joined here
+  static constexpr int kBar = kJoin + kWarps * kRows * D * 4;
+  static constexpr int kSmem = kBar + 1024 + 1024;            // barriers, statistics; room to align to 1024
+};
+
+// The run of blocks of CTA c, of n CTAs, out of `total`.
+__device__ __forceinline__ long long run_start(long long total, int n, int c) { return total * c / n; }
+// The CTA whose run block u is in.
+__device__ __forceinline__ int run_owner(long long total, int n, long long u) { return (int)(((u + 1) * n - 1) / total); }
+
+// A sequence's rows and what they see; at least one block, so that somebody writes the rows that see nothing.
+__device__ __forceinline__ Visible sequence_rows(const FewRows& p, int b) {
+  Visible v;
+  v.first = p.mask.flat ? 0 : p.cu_tokens ? __ldcg(p.cu_tokens + b) : b;
+  v.rows = p.mask.flat ? p.mask.flat : p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - v.first : 1;
+  v.set<kKeys>(p.mask, __ldcg(p.c.lens + b), p.c.width << p.c.page_shift);
+  v.rows = max(0, min(v.rows, kRows / p.rep));  // (more than the caller's bound says: left out)
+  v.count = v.rows == 0 ? 0 : max(1, v.count);
+  return v;
+}
+// Blocks of sequences 0 .. b - 1 of one KV head, for the sequences of a warp's lanes in turn; the whole warp asks.
+// With `stop` >= 0 ends at the sequence that holds block `stop` of them (counted over all KV heads) and returns it.
+__device__ __forceinline__ int add_up(const FewRows& p, long long stop, int upto, long long* sum) {
+  const int lane = threadIdx.x & 31;
+  long long before = 0;
+  for (int b0 = 0; b0 < upto; b0 += 32) {
+    const int b = b0 + lane;
+    int n = b < upto ? sequence_rows(p, b).count : 0, x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (stop >= 0) {
+      const unsigned beyond = __ballot_sync(0xffffffffu, (before + x) * p.c.Hk > stop);
+      if (beyond != 0) {
+        const int l = __ffs(beyond) - 1;
+        *sum = before + __shfl_sync(0xffffffffu, x - n, l);
+        return b0 + l;
+      }
+    }
+    before += __shfl_sync(0xffffffffu, x, 31);
+  }
+  *sum = before;
+  return upto;
+}
+
+// Where a run stands: block i of sequence b and KV head h.
+struct Walk {
+  int b, h, i;
+  Visible v;
+  __device__ __forceinline__ void start(const FewRows& p, long long u) {
+    long long before;
+    b = add_up(p, u, p.c.B, &before);
+    v = sequence_rows(p, b);
+    const int off = (int)(u - before * p.c.Hk);
+    h = off / v.count;
+    i = off - h * v.count;
+  }
+  __device__ __forceinline__ void next(const FewRows& p) {
+    if (++i < v.count) return;
+    i = 0;
+    if (++h < p.c.Hk) return;
+    h = 0;
+    do v = sequence_rows(p, ++b);
+    while (v.count == 0);  // (a run ends within the last sequence that has blocks)
+  }
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewRows p) {
+  using geo = Geo<D>;
+  constexpr int kHalves = D / 64;  // a row of D is 64 elements (128 swizzled bytes) at a time
+  extern __shared__ unsigned char raw[];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  unsigned char* gen = raw + (base - smem_u32(raw));
+  const uint32_t bar_full = base + geo::kBar, bar_empty = bar_full + 8 * geo::kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + geo::kBar + 16 * geo::kStages);
+  volatile unsigned* present = reinterpret_cast<volatile unsigned*>(gen + geo::kBar + 16 * geo::kStages + 8);  // [kStages]
+  float* s_m = reinterpret_cast<float*>(gen + geo::kBar + 256 + 4 * 16);  // [kWarps][kRows] maxima, then sums
+  float* s_l = s_m + kWarps * kRows;
+  float* s_o = reinterpret_cast<float*>(gen + geo::kJoin);                // [kWarps][kRows][D]
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+
+  if (tid == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < geo::kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, kWarps);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+
+  long long total;
+  add_up(p, -1, p.c.B, &total);
+  total *= p.c.Hk;
+  const int n_cta = gridDim.x, cta = blockIdx.x;
+  const long long u0 = run_start(total, n_cta, cta), u1 = run_start(total, n_cta, cta + 1);
+  if (u0 >= u1) return;
+  Walk w;
+  w.start(p, u0);
+
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ loads: one box of a page's rows per lane
+    const int box_rows = min(p.c.page, kKeys), boxes = kKeys / box_rows;
+    const int bx = lane % boxes, half = lane / boxes % kHalves, which = lane / (boxes * kHalves);
+    const bool loads = which < 2;
+    auto page_of = [&](const Walk& w) {
+      const int key = w.v.block(w.i) * kKeys + bx * box_rows;
+      return page_at(p.c, p.c.table + w.b * p.c.table_stride, p.c.width, key >> p.c.page_shift);
+    };
+    int page = page_of(w), s = 0;
+    uint32_t ph = 0;
+    for (long long u = u0; u < u1; ++u) {
+      Walk next = w;
+      int page_next = 0;
+      if (u + 1 < u1) {  // (the next block's table entries are on their way while this one's slot is waited for)
+        next.next(p);
+        page_next = page_of(next);
+      }
+      mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
+      __syncwarp();
+      const unsigned there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << boxes) - 1);
+      if (lane == 0) {
+        present[s] = there;
+        mbar_arrive_expect_tx(bar_full + 8 * s, geo::kStage);
+      }
+      __syncwarp();
+      if (loads) {
+        const int key = w.v.block(w.i) * kKeys + bx * box_rows;
+        // (a page that is not there: a coordinate behind the last one, for which the load brings zeros)
+        tma_load_4d(base + s * geo::kStage + which * geo::kTile + half * (kKeys * 128) + bx * box_rows * 128,
+                    which ? &tmap_v : &tmap_k, half * 64, key & (p.c.page - 1), w.h, page < 0 ? p.c.n_pages : page,
+                    bar_full + 8 * s);
+      }
+      w = next;
+      page = page_next;
+      if (++s == geo::kStages) { s = 0; ph ^= 1; }
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------- products: sixteen keys of every block to a warp
+  const int g = lane >> 2, quad = lane & 3;
+  const int box_shift = p.c.page_shift < 6 ? p.c.page_shift - 4 : 2;  // granule of sixteen keys -> box of the block
+  const int key_lane = 16 * warp + (lane >> 4) * 8 + (lane & 7);      // K: this lane's row for ldmatrix, chunk (lane >> 3) & 1
+  const int val_lane = 16 * warp + ((lane >> 3) & 1) * 8 + (lane & 7);  // V, transposed: row; chunk lane >> 4
+  int s = 0;
+  uint32_t ph = 0;
+  long long u = u0;
+  while (u < u1) {
+    // ---- one sequence and KV head, or what of them this run holds
+    const Visible v = w.v;
+    const int b = w.b, h = w.h, rows = v.rows * p.rep;
+    const int n_blocks = (int)min((long long)(v.count - w.i), u1 - u);
+    const bool whole = n_blocks == v.count;
+    uint32_t qf[D / 16][4];
+    int pos[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = g + 8 * r, tok = row / p.rep;
+      pos[r] = min(v.pmin + tok, v.pmax);
+      const __nv_bfloat16* q = p.q + (long long)(v.first + tok) * p.q_stride + (h * p.rep + row - tok * p.rep) * D + 2 * quad;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk][r] = row < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + 16 * kk)) : 0;
+        qf[kk][2 + r] = row < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + 16 * kk + 8)) : 0;
+      }
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
+#pragma unroll
+    for (int t = 0; t < D / 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+
+    for (int n = 0; n < n_blocks; ++n, ++u) {
+      const int j0 = v.block(w.i + n) * kKeys + 16 * warp;
+      mbar_wait(bar_full + 8 * s, ph, abort_flag);
+      __syncwarp();
+      const uint32_t sk = base + s * geo::kStage, sv = sk + geo::kTile;
+      const bool there = (present[s] >> (warp >> box_shift)) & 1;
+      float c[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[t][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t f[4];
+        const int chunk = 2 * (kk & 3) + ((lane >> 3) & 1);
+        ldmatrix4(sk + (kk >> 2) * (kKeys * 128) + key_lane * 128 + ((chunk ^ (key_lane & 7)) << 4), f);
+        mma_16816_bf16(c[0], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], f[0], f[1]);
+        mma_16816_bf16(c[1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], f[2], f[3]);
+      }
+      const bool full = there && v.all(p.mask, j0, 16);
+      uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;  // V's rows of this lane's fragments that some row sees
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[t][e] *= p.scale_log2;
+      if (!full) {
+        keep0 = keep1 = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = j0 + 8 * t + 2 * quad + e;
+            if (there && v.any(p.mask, j)) (t ? keep1 : keep0) |= 0xffffu << (16 * e);
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              if (!(there && v.sees(p.mask, j, pos[r]))) c[t][2 * r + e] = -INFINITY;
+          }
+        }
+      }
+      // ---- softmax: rows g and g + 8
+      uint32_t a[4];
+      bool moved = false;
+      float corr[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mx = fmaxf(fmaxf(c[0][2 * r], c[0][2 * r + 1]), fmaxf(c[1][2 * r], c[1][2 * r + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[r], mx), from = mn == -INFINITY ? 0.f : mn;
+        corr[r] = ex2(m[r] - from);
+        moved |= mn != m[r];
+        m[r] = mn;
+        float e[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) e[2 * t + x] = ex2(c[t][2 * r + x] - from);
+        l[r] = l[r] * corr[r] + (e[0] + e[1]) + (e[2] + e[3]);
+        a[r] = pack_bf16(e[0], e[1]);
+        a[2 + r] = pack_bf16(e[2], e[3]);
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int t = 0; t < D / 8; ++t) {
+          o[t][0] *= corr[0];
+          o[t][1] *= corr[0];
+          o[t][2] *= corr[1];
+          o[t][3] *= corr[1];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        uint32_t f[4];
+        const int chunk = 2 * (t & 3) + (lane >> 4);
+        ldmatrix4_trans(sv + (t >> 2) * (kKeys * 128) + val_lane * 128 + ((chunk ^ (val_lane & 7)) << 4), f);
+        if (!full) {  // what nobody sees may hold anything: 0 times an infinity is none
+          f[0] &= keep0;
+          f[2] &= keep0;
+          f[1] &= keep1;
+          f[3] &= keep1;
+        }
+        mma_16816_bf16(o[2 * t], a[0], a[1], a[2], a[3], f[0], f[1]);
+        mma_16816_bf16(o[2 * t + 1], a[0], a[1], a[2], a[3], f[2], f[3]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_empty + 8 * s);
+      if (++s == geo::kStages) { s = 0; ph ^= 1; }
+    }
+
+    // ---- the four warps' parts
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (quad == 0) {
+        s_m[warp * kRows + g + 8 * r] = m[r];
+        s_l[warp * kRows + g + 8 * r] = l[r];
+      }
+#pragma unroll
+      for (int t = 0; t < D / 8; ++t)
+        *reinterpret_cast<float2*>(s_o + (warp * kRows + g + 8 * r) * D + 8 * t + 2 * quad) =
+            make_float2(o[t][2 * r], o[t][2 * r + 1]);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+    const long long start = u - n_blocks;  // (a CTA begins at most one part, its first run, and ends at most one)
+    const long long slot = whole ? 2LL * n_cta + b * p.c.Hk + h : 2LL * cta + (start == u0 ? 0 : 1);
+    const bool final = whole && !p.parts_only;
+    constexpr int kQuads = D / 4;
+    for (int x = tid; x < rows * kQuads; x += 32 * kWarps) {
+      const int row = x / kQuads, d = 4 * (x - row * kQuads);
+      float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) mm = fmaxf(mm, s_m[k * kRows + row]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float f = s_m[k * kRows + row] == mm ? 1.f : ex2(s_m[k * kRows + row] - mm);
+        ll += f * s_l[k * kRows + row];
+        const float4 t = *reinterpret_cast<const float4*>(s_o + (k * kRows + row) * D + d);
+        acc.x += f * t.x;
+        acc.y += f * t.y;
+        acc.z += f * t.z;
+        acc.w += f * t.w;
+      }
+      if (final) {
+        const int tok = row / p.rep;
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;  // 0: the row sees nothing
+        *reinterpret_cast<uint2*>(p.out + (long long)(v.first + tok) * p.out_stride + (h * p.rep + row - tok * p.rep) * D + d) =
+            make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(p.part + (slot * kRows + row) * D + d) = acc;
+        if (d == 0) p.stat[slot * kRows + row] = make_float2(mm, ll);
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+    if (u < u1) {
+      w.i += n_blocks - 1;
+      w.next(p);
+    }
+  }
+  if (tid == 0 && *abort_flag && p.status) atomicCAS(p.status, 0, kStatusGemvTimeout);
+}
+
+// ---------------------------------------------------------------- joining parts
+// One CTA per row and KV head of a sequence; D threads.  The parts are taken in the order of their keys.
+struct JoinArgs {
+  FewRows own;                    // the sequences' own keys
+  int prefix_kind;                // 0: none, 1: the same kernel over the prefix, 2: the kernel for many rows
+  FewRows prefix;
+  const float* many_part;         // [tile, split][128][D]
+  const float2* many_stat;        // [tile, split][128]
+  int many_splits, many_tiles;
+};
+
+template <int D>
+struct Joined {
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  __device__ __forceinline__ void add(float2 st, float part) {
+    if (st.y == 0.f) return;
+    const float mn = fmaxf(m, st.x), was = m == mn ? 1.f : ex2(m - mn), f = st.x == mn ? 1.f : ex2(st.x - mn);
+    l = l * was + f * st.y;
+    o = o * was + f * part;
+    m = mn;
+  }
+  // n parts, slot(i) the i-th: eight loads on their way at a time.
+  template <typename Slot>
+  __device__ __forceinline__ void parts(const float2* stat, const float* part, int n, int rows, int row, int d, Slot slot) {
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float2 st[8];
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long long at = i0 + i < n ? slot(i0 + i) : -1;
+        st[i] = at >= 0 ? __ldcg(stat + at * rows + row) : make_float2(-INFINITY, 0.f);
+        x[i] = at >= 0 ? __ldcg(part + (at * rows + row) * D + d) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) add(st[i], x[i]);
+    }
+  }
+};
+
+// The parts of sequence b's KV head h, written by few_rows_kernel on n_cta CTAs; whole: that it is in one part, `item` of them.
+template <int D>
+__device__ __forceinline__ bool join_few(Joined<D>& j, const FewRows& p, int b, int h, int row, int d, bool always) {
+  long long total, before;
+  add_up(p, -1, p.c.B, &total);
+  add_up(p, -1, b, &before);
+  total *= p.c.Hk;
+  const int count = sequence_rows(p, b).count, n = p.n_cta;
+  if (count == 0) return false;
+  const long long s = before * p.c.Hk + (long long)h * count;
+  const int c0 = run_owner(total, n, s), c1 = run_owner(total, n, s + count - 1);
+  if (c0 == c1) {
+    if (!always) return false;
+    j.parts(p.stat, p.part, 1, kRows, row, d, [&](int) { return 2LL * n + b * p.c.Hk + h; });
+    return true;
+  }
+  j.parts(p.stat, p.part, c1 - c0 + 1, kRows, row, d, [&](int i) -> long long {
+    const long long at = run_start(total, n, c0 + i);
+    if (at == run_start(total, n, c0 + i + 1)) return -1;  // a CTA without a block
+    return 2LL * (c0 + i) + (at >= s ? 0 : 1);
+  });
+  return true;
+}
+
+template <int D>
+__global__ void __launch_bounds__(D) join_kernel(const JoinArgs a) {
+  const FewRows& p = a.own;
+  const int b = blockIdx.x / p.c.Hk, h = blockIdx.x % p.c.Hk, row = blockIdx.y, d = threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const Visible v = sequence_rows(p, b);
+  if (row >= v.rows * p.rep) return;
+  Joined<D> j;
+  if (a.prefix_kind == 1) {
+    join_few<D>(j, a.prefix, 0, h, b * p.rep + row, d, true);
+  } else if (a.prefix_kind == 2) {
+    const int r = b * p.rep + row;
+    const long long tile = (long long)h * a.many_tiles + r / 128;
+    j.parts(a.many_stat, a.many_part, a.many_splits, 128, r % 128, d, [&](int i) { return tile * a.many_splits + i; });
+  }
+  if (!join_few<D>(j, p, b, h, row, d, a.prefix_kind != 0) && a.prefix_kind == 0) return;  // written by its one CTA
+  const int tok = row / p.rep;
+  p.out[(long long)(v.first + tok) * p.out_stride + (h * p.rep + row - tok * p.rep) * D + d] =
+      __float2bfloat16(j.l == 0.f ? 0.f : j.o / j.l);
+}
+
+// ---------------------------------------------------------------- many rows
 // One warp per (row, query head); lanes split the head dimension.
 template <int D>
 struct RowState {
@@ -76,6 +523,57 @@ __global__ void __launch_bounds__(128) attention_kernel(const __nv_bfloat16* q, 
     out[t * out_stride + h * D + lane * E + e] = __float2bfloat16(r.l > 0.f ? r.acc[e] / r.l : 0.f);
 }
 
+// ---------------------------------------------------------------- host
+constexpr size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+size_t part_bytes(long long slots, int rows, int D) { return align256((size_t)slots * rows * D * 4) + align256((size_t)slots * rows * 8); }
+
+template <typename... Args>
+int launch_pdl(void (*kernel)(Args...), dim3 grid, int block, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int D>
+int launch_few(const FewRows& p, cudaStream_t s) {
+  CUtensorMap mk, mv;
+  if (!paged_tensor_maps(p.c, kKeys, &mk, &mv)) return kErrBadShape;
+  const int rc = (int)cudaFuncSetAttribute(few_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<D>::kSmem);
+  if (rc) return rc;
+  return launch_pdl(few_rows_kernel<D>, dim3(p.n_cta), kThreads, Geo<D>::kSmem, s, mk, mv, p);
+}
+
+FewRows few_rows(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int rep, float scale_log2,
+                 void* out, long long out_stride, void* parts, long long slots, int n_cta) {
+  FewRows p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride = q_stride;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_stride = out_stride;
+  p.c = c;
+  p.cu_tokens = cu_tokens;
+  p.rep = rep;
+  p.n_cta = n_cta;
+  p.scale_log2 = scale_log2;
+  p.part = static_cast<float*>(parts);
+  p.stat = reinterpret_cast<float2*>(static_cast<char*>(parts) + align256((size_t)slots * kRows * c.D * 4));
+  p.status = device_status_word_if_ready();
+  return p;
+}
+
+int join(const JoinArgs& a, int rows, cudaStream_t s) {
+  const dim3 grid((unsigned)(a.own.c.B * a.own.c.Hk), (unsigned)rows);
+  return a.own.c.D == 64 ? launch_pdl(join_kernel<64>, grid, 64, 0, s, a) : launch_pdl(join_kernel<128>, grid, 128, 0, s, a);
+}
+
 int check_rows(const void* q, long long q_stride, const PagedCache& c, int T, int Hq, const void* out, long long out_stride) {
   if (T < 1 || Hq < 1 || Hq % c.Hk || (c.D != 64 && c.D != 128)) return kErrBadShape;
   if (q_stride < (long long)Hq * c.D || q_stride % 8 || out_stride < (long long)Hq * c.D || out_stride % 8) return kErrBadShape;
@@ -83,41 +581,90 @@ int check_rows(const void* q, long long q_stride, const PagedCache& c, int T, in
   return 0;
 }
 
-int launch(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int T, int Hq, int window, int sinks,
-           float scale, void* out, long long out_stride, const int* prefix_table, int prefix_width, const int* prefix_len,
-           cudaStream_t s) {
-  const unsigned grid = (unsigned)(((long long)T * Hq + 3) / 4);
-  (c.D == 64 ? attention_kernel<64> : attention_kernel<128>)<<<grid, 128, 0, s>>>(
-      static_cast<const __nv_bfloat16*>(q), q_stride, c, cu_tokens, T, Hq, window, sinks, scale,
-      static_cast<__nv_bfloat16*>(out), out_stride, prefix_table, prefix_width, prefix_len);
-  return (int)cudaGetLastError();
-}
-
 }  // namespace
 
-size_t paged_attention_workspace(int, int, int, int, int, int, int) { return 0; }
-size_t shared_prefix_workspace(int, int, int, int, int) { return 0; }
+bool paged_tensor_maps(const PagedCache& c, int block, CUtensorMap* k, CUtensorMap* v) {
+  const uint64_t dims[4] = {(uint64_t)c.D, (uint64_t)c.page, (uint64_t)c.Hk, (uint64_t)c.n_pages};
+  // (the stride of a dimension of one is never used, but has to be one that a map may have)
+  const uint64_t strides[3] = {(uint64_t)c.token_stride, (uint64_t)(c.Hk > 1 ? c.head_stride : c.D),
+                               (uint64_t)(c.n_pages > 1 ? c.page_stride : c.D)};
+  const uint32_t box[2] = {64, (uint32_t)std::min(c.page, block)};
+  return make_tensor_map_4d(k, c.k, dims, strides, box) && make_tensor_map_4d(v, c.v, dims, strides, box);
+}
+
+size_t paged_attention_workspace(int T, int B, int max_tokens, int Hq, int Hk, int D, int sm_count) {
+  return part_bytes(2LL * sm_count, kRows, D);
+}
+size_t shared_prefix_workspace(int B, int Hq, int Hk, int D, int sm_count) {
+  return part_bytes(2LL * sm_count + (long long)B * Hk, kRows, D) + part_bytes(2LL * sm_count + Hk, kRows, D);
+}
 
 int paged_attention_launch(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int T,
                            int max_tokens, int Hq, int window, int sinks, float scale, void* out, long long out_stride,
-                           void*, size_t, int sm_count, cudaStream_t s) {
+                           void* workspace, size_t workspace_bytes, int sm_count, cudaStream_t s) {
   if (const int bad = check_rows(q, q_stride, c, T, Hq, out, out_stride)) return bad;
   if (max_tokens < 1 || window < 0 || sinks < 0 || (!cu_tokens && (T != c.B || max_tokens != 1))) return kErrBadShape;
   if (misaligned(cu_tokens, 4)) return kErrBadPointer;
   if (sm_count < 1) return -sm_count;
-  return launch(q, q_stride, c, cu_tokens, T, Hq, window, sinks, scale, out, out_stride, nullptr, 0, nullptr, s);
+  if (!workspace || misaligned(workspace, 16)) return kErrBadPointer;
+  if (workspace_bytes < paged_attention_workspace(T, c.B, max_tokens, Hq, c.Hk, c.D, sm_count)) return kErrWorkspace;
+  if (window >= 1 << 30) window = 0;  // (positions are below that)
+  const int rep = Hq / c.Hk;
+  const float scale_log2 = scale * 1.44269504088896340736f;
+  if ((long long)max_tokens * rep <= kRows) {
+    FewRows p = few_rows(q, q_stride, c, cu_tokens, rep, scale_log2, out, out_stride, workspace, 2LL * sm_count, sm_count);
+    p.mask = Mask{window, sinks, 0};
+    if (const int rc = c.D == 64 ? launch_few<64>(p, s) : launch_few<128>(p, s)) return rc;
+    JoinArgs a{};
+    a.own = p;
+    return join(a, max_tokens * rep, s);
+  }
+  const unsigned grid = (unsigned)(((long long)T * Hq + 3) / 4);
+  (c.D == 64 ? attention_kernel<64> : attention_kernel<128>)<<<grid, 128, 0, s>>>(
+      static_cast<const __nv_bfloat16*>(q), q_stride, c, cu_tokens, T, Hq, window, sinks, scale,
+      static_cast<__nv_bfloat16*>(out), out_stride, nullptr, 0, nullptr);
+  return (int)cudaGetLastError();
 }
 
 int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c, const int* prefix_table,
                          int prefix_width, const int* prefix_len, int Hq, float scale, void* out, long long out_stride,
-                         void*, size_t, int sm_count, cudaStream_t s) {
+                         void* workspace, size_t workspace_bytes, int sm_count, cudaStream_t s) {
   if (const int bad = check_rows(q, q_stride, c, c.B, Hq, out, out_stride)) return bad;
   if (prefix_width < 0) return kErrBadShape;
   if ((long long)prefix_width * c.page > (1LL << 30)) return kErrTooLarge;
   if (!prefix_len || (prefix_width > 0 && !prefix_table) || misaligned(prefix_table, 4) || misaligned(prefix_len, 4))
     return kErrBadPointer;
   if (sm_count < 1) return -sm_count;
-  return launch(q, q_stride, c, nullptr, c.B, Hq, 0, 0, scale, out, out_stride, prefix_table, prefix_width, prefix_len, s);
+  if (!workspace || misaligned(workspace, 16)) return kErrBadPointer;
+  if (workspace_bytes < shared_prefix_workspace(c.B, Hq, c.Hk, c.D, sm_count)) return kErrWorkspace;
+  const int rep = Hq / c.Hk;
+  const float scale_log2 = scale * 1.44269504088896340736f;
+  if (c.B * rep <= kRows) {
+    PagedCache pre = c;
+    pre.table = prefix_table;
+    pre.width = prefix_width;
+    pre.lens = prefix_len;
+    pre.B = 1;
+    const long long own_slots = 2LL * sm_count + (long long)c.B * c.Hk;
+    FewRows p = few_rows(q, q_stride, pre, nullptr, rep, scale_log2, out, out_stride,
+                         static_cast<char*>(workspace) + part_bytes(own_slots, kRows, c.D), 2LL * sm_count + c.Hk, sm_count);
+    p.mask = Mask{0, 0, c.B};
+    p.parts_only = 1;
+    if (const int rc = c.D == 64 ? launch_few<64>(p, s) : launch_few<128>(p, s)) return rc;
+    JoinArgs a{};
+    a.prefix_kind = 1;
+    a.prefix = p;
+    a.own = few_rows(q, q_stride, c, nullptr, rep, scale_log2, out, out_stride, workspace, own_slots, sm_count);
+    a.own.mask = Mask{0, 0, 0};
+    a.own.parts_only = 1;
+    if (const int rc = c.D == 64 ? launch_few<64>(a.own, s) : launch_few<128>(a.own, s)) return rc;
+    return join(a, rep, s);
+  }
+  const unsigned grid = (unsigned)(((long long)c.B * Hq + 3) / 4);
+  (c.D == 64 ? attention_kernel<64> : attention_kernel<128>)<<<grid, 128, 0, s>>>(
+      static_cast<const __nv_bfloat16*>(q), q_stride, c, nullptr, c.B, Hq, 0, 0, scale,
+      static_cast<__nv_bfloat16*>(out), out_stride, prefix_table, prefix_width, prefix_len);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace b2

@@ -167,6 +167,13 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const void* tmap,
       "l"(tmap), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst_smem, const void* tmap, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          dst_smem),
+      "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 // Brings a tile (or the 128-byte line of an address) into L2 only.  Nothing is read as far as the program can tell, so a
 // kernel that still runs may be writing it: what is loaded later is what L2 then holds.
 __device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int x, int y) {
