@@ -351,7 +351,7 @@ int b2_tp_wait(const void* wait_sig, const void* epoch, unsigned wait_per_epoch,
  *     qkv is not modified.  A row whose position is negative is left out.  head_dim % 16 == 0, at most 256.
  *   b2_paged_attention: out [T, Hq D] = softmax(scale q K^T) V; the row at position i sees the keys j <= i of its sequence and, with
  *     window > 0, of those only j > i - window and the first `sinks`.  A row that sees no key is zero.  head_dim 64 or 128,
- *     Hq % Hk == 0.  max_tokens: no sequence has more rows than that (rows beyond it are left as they are).
+ *     Hq % Hk == 0, 0 < scale < infinity.  max_tokens: no sequence has more rows than that (rows beyond it are left as they are).
  *   b2_shared_prefix_attention: one row per sequence, which sees the first *prefix_len (int32, on the device) tokens of the pages
  *     prefix_table [prefix_width], and all seq_lens[b] tokens (which may be none) of its own pages.  The prefix's keys and values
  *     are read once for all sequences.

@@ -53,9 +53,14 @@ __device__ __forceinline__ Visible sequence_rows(const FewRows& p, int b) {
   v.first = p.mask.flat ? 0 : p.cu_tokens ? __ldcg(p.cu_tokens + b) : b;
   v.rows = p.mask.flat ? p.mask.flat : p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - v.first : 1;
   v.set<kKeys>(p.mask, __ldcg(p.c.lens + b), p.c.width << p.c.page_shift);
-  v.rows = max(0, min(v.rows, kRows / p.rep));  // (more than the caller's bound says: left out)
+  v.rows = v.first < 0 ? 0 : max(0, min(min(v.rows, min(p.max_tokens, kRows / p.rep)), p.T - v.first));
   v.count = v.rows == 0 ? 0 : max(1, v.count);
   return v;
+}
+// The first query head of tile h of a sequence, and its rows.
+__device__ __forceinline__ int first_head(const FewRows& p, int h) { return h / p.groups * p.rep_all + h % p.groups * kRows; }
+__device__ __forceinline__ int tile_rows(const FewRows& p, const Visible& v, int h) {
+  return v.rows * min(p.rep, p.rep_all - h % p.groups * kRows);
 }
 // Blocks of sequences 0 .. b - 1 of one KV head, for the sequences of a warp's lanes in turn; the whole warp asks.
 // With `stop` >= 0 ends at the sequence that holds block `stop` of them (counted over all KV heads) and returns it.
@@ -71,7 +76,7 @@ __device__ __forceinline__ int add_up(const FewRows& p, long long stop, int upto
       if (lane >= o) x += y;
     }
     if (stop >= 0) {
-      const unsigned beyond = __ballot_sync(0xffffffffu, (before + x) * p.c.Hk > stop);
+      const unsigned beyond = __ballot_sync(0xffffffffu, (before + x) * p.heads > stop);
       if (beyond != 0) {
         const int l = __ffs(beyond) - 1;
         *sum = before + __shfl_sync(0xffffffffu, x - n, l);
@@ -92,14 +97,14 @@ struct Walk {
     long long before;
     b = add_up(p, u, p.c.B, &before);
     v = sequence_rows(p, b);
-    const int off = (int)(u - before * p.c.Hk);
+    const int off = (int)(u - before * p.heads);
     h = off / v.count;
     i = off - h * v.count;
   }
   __device__ __forceinline__ void next(const FewRows& p) {
     if (++i < v.count) return;
     i = 0;
-    if (++h < p.c.Hk) return;
+    if (++h < p.heads) return;
     h = 0;
     do v = sequence_rows(p, ++b);
     while (v.count == 0);  // (a run ends within the last sequence that has blocks)
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   long long total;
   add_up(p, -1, p.c.B, &total);
-  total *= p.c.Hk;
+  total *= p.heads;
   const int n_cta = gridDim.x, cta = blockIdx.x;
   const long long u0 = run_start(total, n_cta, cta), u1 = run_start(total, n_cta, cta + 1);
   if (u0 >= u1) return;
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int key = w.v.block(w.i) * kKeys + bx * box_rows;
         // (a page that is not there: a coordinate behind the last one, for which the load brings zeros)
         tma_load_4d(base + s * geo::kStage + which * geo::kTile + half * (kKeys * 128) + bx * box_rows * 128,
-                    which ? &tmap_v : &tmap_k, half * 64, key & (p.c.page - 1), w.h, page < 0 ? p.c.n_pages : page,
+                    which ? &tmap_v : &tmap_k, half * 64, key & (p.c.page - 1), w.h / p.groups, page < 0 ? p.c.n_pages : page,
                     bar_full + 8 * s);
       }
       w = next;
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   while (u < u1) {
     // ---- one sequence and KV head, or what of them this run holds
     const Visible v = w.v;
-    const int b = w.b, h = w.h, rows = v.rows * p.rep;
+    const int b = w.b, h = w.h, head0 = first_head(p, h), rows = tile_rows(p, v, h);
     const int n_blocks = (int)min((long long)(v.count - w.i), u1 - u);
     const bool whole = n_blocks == v.count;
     uint32_t qf[D / 16][4];
@@ -218,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int r = 0; r < 2; ++r) {
       const int row = g + 8 * r, tok = row / p.rep;
       pos[r] = min(v.pmin + tok, v.pmax);
-      const __nv_bfloat16* q = p.q + (long long)(v.first + tok) * p.q_stride + (h * p.rep + row - tok * p.rep) * D + 2 * quad;
+      const __nv_bfloat16* q = p.q + (long long)(v.first + tok) * p.q_stride + (head0 + row - tok * p.rep) * D + 2 * quad;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         qf[kk][r] = row < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + 16 * kk)) : 0;
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
     const long long start = u - n_blocks;  // (a CTA begins at most one part, its first run, and ends at most one)
-    const long long slot = whole ? 2LL * n_cta + b * p.c.Hk + h : 2LL * cta + (start == u0 ? 0 : 1);
+    const long long slot = whole ? 2LL * n_cta + b * p.heads + h : 2LL * cta + (start == u0 ? 0 : 1);
     const bool final = whole && !p.parts_only;
     constexpr int kQuads = D / 4;
     for (int x = tid; x < rows * kQuads; x += 32 * kWarps) {
@@ -358,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (final) {
         const int tok = row / p.rep;
         const float inv = ll == 0.f ? 0.f : 1.f / ll;  // 0: the row sees nothing
-        *reinterpret_cast<uint2*>(p.out + (long long)(v.first + tok) * p.out_stride + (h * p.rep + row - tok * p.rep) * D + d) =
+        *reinterpret_cast<uint2*>(p.out + (long long)(v.first + tok) * p.out_stride + (head0 + row - tok * p.rep) * D + d) =
             make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
       } else {
         *reinterpret_cast<float4*>(p.part + (slot * kRows + row) * D + d) = acc;
@@ -419,14 +424,14 @@ __device__ __forceinline__ bool join_few(Joined<D>& j, const FewRows& p, int b, 
   long long total, before;
   add_up(p, -1, p.c.B, &total);
   add_up(p, -1, b, &before);
-  total *= p.c.Hk;
+  total *= p.heads;
   const int count = sequence_rows(p, b).count, n = p.n_cta;
   if (count == 0) return false;
-  const long long s = before * p.c.Hk + (long long)h * count;
+  const long long s = before * p.heads + (long long)h * count;
   const int c0 = run_owner(total, n, s), c1 = run_owner(total, n, s + count - 1);
   if (c0 == c1) {
     if (!always) return false;
-    j.parts(p.stat, p.part, 1, kRows, row, d, [&](int) { return 2LL * n + b * p.c.Hk + h; });
+    j.parts(p.stat, p.part, 1, kRows, row, d, [&](int) { return 2LL * n + b * p.heads + h; });
     return true;
   }
   j.parts(p.stat, p.part, c1 - c0 + 1, kRows, row, d, [&](int i) -> long long {
@@ -440,110 +445,31 @@ __device__ __forceinline__ bool join_few(Joined<D>& j, const FewRows& p, int b, 
 template <int D>
 __global__ void __launch_bounds__(D) join_kernel(const JoinArgs a) {
   const FewRows& p = a.own;
-  const int b = blockIdx.x / p.c.Hk, h = blockIdx.x % p.c.Hk, row = blockIdx.y, d = threadIdx.x;
+  const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, row = blockIdx.y, d = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait_prior_grid();
   const Visible v = sequence_rows(p, b);
-  if (row >= v.rows * p.rep) return;
+  if (row >= tile_rows(p, v, h)) return;
   Joined<D> j;
   if (a.prefix_kind == 1) {
     join_few<D>(j, a.prefix, 0, h, b * p.rep + row, d, true);
   } else if (a.prefix_kind == 2) {
-    const int r = b * p.rep + row;
-    const long long tile = (long long)h * a.many_tiles + r / 128;
+    const int r = b * p.rep_all + (h % p.groups) * kRows + row;
+    const long long tile = (long long)(h / p.groups) * a.many_tiles + r / 128;
     j.parts(a.many_stat, a.many_part, a.many_splits, 128, r % 128, d, [&](int i) { return tile * a.many_splits + i; });
   }
   if (!join_few<D>(j, p, b, h, row, d, a.prefix_kind != 0) && a.prefix_kind == 0) return;  // written by its one CTA
   const int tok = row / p.rep;
-  p.out[(long long)(v.first + tok) * p.out_stride + (h * p.rep + row - tok * p.rep) * D + d] =
+  p.out[(long long)(v.first + tok) * p.out_stride + (first_head(p, h) + row - tok * p.rep) * D + d] =
       __float2bfloat16(j.l == 0.f ? 0.f : j.o / j.l);
-}
-
-// ---------------------------------------------------------------- many rows
-// One warp per (row, query head); lanes split the head dimension.
-template <int D>
-struct RowState {
-  static constexpr int E = D / 32;
-  float q[E], acc[E], m = -FLT_MAX, l = 0.f;
-  __device__ __forceinline__ void key(const __nv_bfloat16* k, const __nv_bfloat16* v, int lane) {
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      s += q[e] * __bfloat162float(__ushort_as_bfloat16(__ldcg(reinterpret_cast<const unsigned short*>(k) + lane * E + e)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float mn = fmaxf(m, s), corr = __expf(m - mn), p = __expf(s - mn);
-    l = l * corr + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      acc[e] = acc[e] * corr +
-               p * __bfloat162float(__ushort_as_bfloat16(__ldcg(reinterpret_cast<const unsigned short*>(v) + lane * E + e)));
-    m = mn;
-  }
-  __device__ void keys(const PagedCache& c, const int* table, int width, int kh, int j0, int j1, int lane) {
-    for (int j = j0; j < j1; ++j) {
-      const int col = j >> c.page_shift;
-      if (col >= width) return;
-      const int page = __ldcg(table + col);
-      if (page < 0 || page >= c.n_pages) continue;
-      const long long at = page * c.page_stride + kh * c.head_stride + (long long)(j & (c.page - 1)) * c.token_stride;
-      key(c.k + at, c.v + at, lane);
-    }
-  }
-};
-
-template <int D>
-__global__ void __launch_bounds__(128) attention_kernel(const __nv_bfloat16* q, long long q_stride, PagedCache c,
-                                                        const int* cu_tokens, int T, int Hq, int window, int sinks,
-                                                        float scale, __nv_bfloat16* out, long long out_stride,
-                                                        const int* prefix_table, int prefix_width, const int* prefix_len) {
-  const int lane = threadIdx.x & 31;
-  const long long row = blockIdx.x * 4LL + (threadIdx.x >> 5);
-  if (row >= (long long)T * Hq) return;
-  const int t = (int)(row / Hq), h = (int)(row - (long long)t * Hq), kh = h / (Hq / c.Hk);
-  int first;
-  const int b = sequence_of(cu_tokens, c.B, t, &first);
-  if (b < 0) return;
-  RowState<D> r;
-  constexpr int E = RowState<D>::E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    r.q[e] = scale * __bfloat162float(q[t * q_stride + h * D + lane * E + e]);
-    r.acc[e] = 0.f;
-  }
-  if (prefix_table) r.keys(c, prefix_table, prefix_width, kh, 0, __ldcg(prefix_len), lane);
-  const int n_new = cu_tokens ? __ldcg(cu_tokens + b + 1) - first : 1;
-  const int len = __ldcg(c.lens + b), pos = len - n_new + (t - first);
-  const int lo = window > 0 ? max(0, pos - window + 1) : 0;
-  const int* table = c.table + b * c.table_stride;
-  r.keys(c, table, c.width, kh, 0, min(min(sinks, lo), pos + 1), lane);
-  r.keys(c, table, c.width, kh, lo, pos + 1, lane);
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    out[t * out_stride + h * D + lane * E + e] = __float2bfloat16(r.l > 0.f ? r.acc[e] / r.l : 0.f);
 }
 
 // ---------------------------------------------------------------- host
 constexpr size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 size_t part_bytes(long long slots, int rows, int D) { return align256((size_t)slots * rows * D * 4) + align256((size_t)slots * rows * 8); }
 
-template <typename... Args>
-int launch_pdl(void (*kernel)(Args...), dim3 grid, int block, size_t smem, cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int D>
-int launch_few(const FewRows& p, cudaStream_t s) {
+int launch_few_of(const FewRows& p, cudaStream_t s) {
   CUtensorMap mk, mv;
   if (!paged_tensor_maps(p.c, kKeys, &mk, &mv)) return kErrBadShape;
   const int rc = (int)cudaFuncSetAttribute(few_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<D>::kSmem);
@@ -551,16 +477,23 @@ int launch_few(const FewRows& p, cudaStream_t s) {
   return launch_pdl(few_rows_kernel<D>, dim3(p.n_cta), kThreads, Geo<D>::kSmem, s, mk, mv, p);
 }
 
+int launch_few(const FewRows& p, cudaStream_t s) { return p.c.D == 64 ? launch_few_of<64>(p, s) : launch_few_of<128>(p, s); }
+
 FewRows few_rows(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int rep, float scale_log2,
-                 void* out, long long out_stride, void* parts, long long slots, int n_cta) {
+                 void* out, long long out_stride, void* parts, long long slots, int n_cta, int T, int max_tokens) {
   FewRows p{};
+  p.T = T;
+  p.max_tokens = max_tokens;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_stride = q_stride;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.out_stride = out_stride;
   p.c = c;
   p.cu_tokens = cu_tokens;
-  p.rep = rep;
+  p.rep_all = rep;
+  p.rep = std::min(rep, kRows);
+  p.groups = (rep + kRows - 1) / kRows;
+  p.heads = c.Hk * p.groups;
   p.n_cta = n_cta;
   p.scale_log2 = scale_log2;
   p.part = static_cast<float*>(parts);
@@ -570,12 +503,13 @@ FewRows few_rows(const void* q, long long q_stride, const PagedCache& c, const i
 }
 
 int join(const JoinArgs& a, int rows, cudaStream_t s) {
-  const dim3 grid((unsigned)(a.own.c.B * a.own.c.Hk), (unsigned)rows);
+  const dim3 grid((unsigned)(a.own.c.B * a.own.heads), (unsigned)std::min(rows, kRows));
   return a.own.c.D == 64 ? launch_pdl(join_kernel<64>, grid, 64, 0, s, a) : launch_pdl(join_kernel<128>, grid, 128, 0, s, a);
 }
 
-int check_rows(const void* q, long long q_stride, const PagedCache& c, int T, int Hq, const void* out, long long out_stride) {
-  if (T < 1 || Hq < 1 || Hq % c.Hk || (c.D != 64 && c.D != 128)) return kErrBadShape;
+int check_rows(const void* q, long long q_stride, const PagedCache& c, int T, int Hq, float scale, const void* out,
+               long long out_stride) {
+  if (!(scale > 0.f) || scale > FLT_MAX || T < 1 || Hq < 1 || Hq % c.Hk || (c.D != 64 && c.D != 128)) return kErrBadShape;
   if (q_stride < (long long)Hq * c.D || q_stride % 8 || out_stride < (long long)Hq * c.D || out_stride % 8) return kErrBadShape;
   if (!q || !out || misaligned(q, 16) || misaligned(out, 16)) return kErrBadPointer;
   return 0;
@@ -592,44 +526,107 @@ bool paged_tensor_maps(const PagedCache& c, int block, CUtensorMap* k, CUtensorM
   return make_tensor_map_4d(k, c.k, dims, strides, box) && make_tensor_map_4d(v, c.v, dims, strides, box);
 }
 
+namespace {
+
+// How the kernel for many rows cuts a call up: tiles of 128 rows, two to a CTA where sequences have more; CTAs that would leave
+// SMs idle share the keys of a tile, down to four blocks of 128 each.
+struct ManyPlan {
+  int two, slots, splits;
+};
+ManyPlan many_plan(long long rows, int B, long long most_rows, int Hk, long long most_keys, int sm_count) {
+  ManyPlan m;
+  m.two = most_rows > 128;
+  const int size = m.two ? 256 : 128;
+  const long long tiles = std::min(rows / size + B, B * ((most_rows + size - 1) / size));  // no fewer than there are
+  const long long likely = std::max<long long>(1, std::max((rows + size - 1) / size, tiles - B / 2));
+  m.slots = (int)(m.two ? 2 * tiles : tiles);
+  m.splits = (int)std::max<long long>(1, std::min<long long>(sm_count / (likely * Hk), most_keys / 512));
+  return m;
+}
+size_t many_bytes(const ManyPlan& m, int Hk, int D) { return part_bytes((long long)m.slots * Hk * m.splits, 128, D); }
+
+ManyRows many_rows(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int rep, int T,
+                   int max_tokens, const ManyPlan& m, float scale_log2, void* out, long long out_stride, void* parts) {
+  ManyRows p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride = q_stride;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_stride = out_stride;
+  p.c = c;
+  p.cu_tokens = cu_tokens;
+  p.rep = rep;
+  p.T = T;
+  p.max_tokens = max_tokens;
+  p.two = m.two;
+  p.slots = m.slots;
+  p.splits = m.splits;
+  p.scale_log2 = scale_log2;
+  if (parts) {
+    p.part = static_cast<float*>(parts);
+    p.stat = reinterpret_cast<float2*>(static_cast<char*>(parts) +
+                                       align256((size_t)m.slots * c.Hk * m.splits * 128 * c.D * 4));
+  }
+  p.status = device_status_word_if_ready();
+  return p;
+}
+
+// Whether a sequence's rows of a KV head are the few-row kernel's.  (One token of more than sixteen heads takes two tiles or more,
+// each of which reads the keys.)
+bool few(int max_tokens, int rep) { return max_tokens == 1 || (long long)max_tokens * rep <= kRows; }
+
+constexpr long long kMostKeys = 1LL << 30;
+
+}  // namespace
+
 size_t paged_attention_workspace(int T, int B, int max_tokens, int Hq, int Hk, int D, int sm_count) {
-  return part_bytes(2LL * sm_count, kRows, D);
+  max_tokens = std::min(max_tokens, T);
+  const int rep = Hq / Hk;
+  if (few(max_tokens, rep)) return part_bytes(2LL * sm_count, kRows, D);
+  const ManyPlan m = many_plan((long long)T * rep, B, (long long)max_tokens * rep, Hk, kMostKeys, sm_count);
+  return std::max<size_t>(256, m.splits > 1 ? many_bytes(m, Hk, D) : 0);
 }
 size_t shared_prefix_workspace(int B, int Hq, int Hk, int D, int sm_count) {
-  return part_bytes(2LL * sm_count + (long long)B * Hk, kRows, D) + part_bytes(2LL * sm_count + Hk, kRows, D);
+  const int rep = Hq / Hk;
+  const size_t own = part_bytes(2LL * sm_count + (long long)B * Hk * ((rep + kRows - 1) / kRows), kRows, D);
+  if ((long long)B * rep <= kRows) return own + part_bytes(2LL * sm_count + Hk, kRows, D);
+  return own + many_bytes(many_plan((long long)B * rep, 1, (long long)B * rep, Hk, kMostKeys, sm_count), Hk, D);
 }
 
 int paged_attention_launch(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int T,
                            int max_tokens, int Hq, int window, int sinks, float scale, void* out, long long out_stride,
                            void* workspace, size_t workspace_bytes, int sm_count, cudaStream_t s) {
-  if (const int bad = check_rows(q, q_stride, c, T, Hq, out, out_stride)) return bad;
+  if (const int bad = check_rows(q, q_stride, c, T, Hq, scale, out, out_stride)) return bad;
   if (max_tokens < 1 || window < 0 || sinks < 0 || (!cu_tokens && (T != c.B || max_tokens != 1))) return kErrBadShape;
   if (misaligned(cu_tokens, 4)) return kErrBadPointer;
   if (sm_count < 1) return -sm_count;
   if (!workspace || misaligned(workspace, 16)) return kErrBadPointer;
+  max_tokens = std::min(max_tokens, T);
   if (workspace_bytes < paged_attention_workspace(T, c.B, max_tokens, Hq, c.Hk, c.D, sm_count)) return kErrWorkspace;
   if (window >= 1 << 30) window = 0;  // (positions are below that)
   const int rep = Hq / c.Hk;
+  const Mask mask{window, std::min(sinks, 1 << 30), 0};
   const float scale_log2 = scale * 1.44269504088896340736f;
-  if ((long long)max_tokens * rep <= kRows) {
-    FewRows p = few_rows(q, q_stride, c, cu_tokens, rep, scale_log2, out, out_stride, workspace, 2LL * sm_count, sm_count);
-    p.mask = Mask{window, sinks, 0};
-    if (const int rc = c.D == 64 ? launch_few<64>(p, s) : launch_few<128>(p, s)) return rc;
+  if (few(max_tokens, rep)) {
     JoinArgs a{};
-    a.own = p;
+    a.own = few_rows(q, q_stride, c, cu_tokens, rep, scale_log2, out, out_stride, workspace, 2LL * sm_count, sm_count, T,
+                     max_tokens);
+    a.own.mask = mask;
+    if (const int rc = launch_few(a.own, s)) return rc;
     return join(a, max_tokens * rep, s);
   }
-  const unsigned grid = (unsigned)(((long long)T * Hq + 3) / 4);
-  (c.D == 64 ? attention_kernel<64> : attention_kernel<128>)<<<grid, 128, 0, s>>>(
-      static_cast<const __nv_bfloat16*>(q), q_stride, c, cu_tokens, T, Hq, window, sinks, scale,
-      static_cast<__nv_bfloat16*>(out), out_stride, nullptr, 0, nullptr);
-  return (int)cudaGetLastError();
+  const ManyPlan m = many_plan((long long)T * rep, c.B, (long long)max_tokens * rep, c.Hk, (long long)c.width * c.page, sm_count);
+  ManyRows p = many_rows(q, q_stride, c, cu_tokens, rep, T, max_tokens, m, scale_log2, out, out_stride,
+                         m.splits > 1 ? workspace : nullptr);
+  p.mask = mask;
+  const int rc = many_rows_launch(p, s);
+  return rc || m.splits == 1 ? rc : join_many_launch(p, s);
 }
 
 int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c, const int* prefix_table,
                          int prefix_width, const int* prefix_len, int Hq, float scale, void* out, long long out_stride,
                          void* workspace, size_t workspace_bytes, int sm_count, cudaStream_t s) {
-  if (const int bad = check_rows(q, q_stride, c, c.B, Hq, out, out_stride)) return bad;
+  if (const int bad = check_rows(q, q_stride, c, c.B, Hq, scale, out, out_stride)) return bad;
+  const int rep = Hq / c.Hk;
   if (prefix_width < 0) return kErrBadShape;
   if ((long long)prefix_width * c.page > (1LL << 30)) return kErrTooLarge;
   if (!prefix_len || (prefix_width > 0 && !prefix_table) || misaligned(prefix_table, 4) || misaligned(prefix_len, 4))
@@ -637,34 +634,39 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
   if (sm_count < 1) return -sm_count;
   if (!workspace || misaligned(workspace, 16)) return kErrBadPointer;
   if (workspace_bytes < shared_prefix_workspace(c.B, Hq, c.Hk, c.D, sm_count)) return kErrWorkspace;
-  const int rep = Hq / c.Hk;
   const float scale_log2 = scale * 1.44269504088896340736f;
+  const long long own_slots = 2LL * sm_count + (long long)c.B * c.Hk * ((rep + kRows - 1) / kRows);
+  char* prefix_parts = static_cast<char*>(workspace) + part_bytes(own_slots, kRows, c.D);
+  PagedCache pre = c;
+  pre.table = prefix_table;
+  pre.width = prefix_width;
+  pre.lens = prefix_len;
+  pre.B = 1;
+  JoinArgs a{};
   if (c.B * rep <= kRows) {
-    PagedCache pre = c;
-    pre.table = prefix_table;
-    pre.width = prefix_width;
-    pre.lens = prefix_len;
-    pre.B = 1;
-    const long long own_slots = 2LL * sm_count + (long long)c.B * c.Hk;
-    FewRows p = few_rows(q, q_stride, pre, nullptr, rep, scale_log2, out, out_stride,
-                         static_cast<char*>(workspace) + part_bytes(own_slots, kRows, c.D), 2LL * sm_count + c.Hk, sm_count);
-    p.mask = Mask{0, 0, c.B};
-    p.parts_only = 1;
-    if (const int rc = c.D == 64 ? launch_few<64>(p, s) : launch_few<128>(p, s)) return rc;
-    JoinArgs a{};
     a.prefix_kind = 1;
-    a.prefix = p;
-    a.own = few_rows(q, q_stride, c, nullptr, rep, scale_log2, out, out_stride, workspace, own_slots, sm_count);
-    a.own.mask = Mask{0, 0, 0};
-    a.own.parts_only = 1;
-    if (const int rc = c.D == 64 ? launch_few<64>(a.own, s) : launch_few<128>(a.own, s)) return rc;
-    return join(a, rep, s);
+    a.prefix = few_rows(q, q_stride, pre, nullptr, rep, scale_log2, out, out_stride, prefix_parts, 2LL * sm_count + c.Hk,
+                        sm_count, c.B, c.B);
+    a.prefix.mask = Mask{0, 0, c.B};
+    a.prefix.parts_only = 1;
+    if (const int rc = launch_few(a.prefix, s)) return rc;
+  } else {
+    const long long rows = (long long)c.B * rep;
+    const ManyPlan m = many_plan(rows, 1, rows, c.Hk, (long long)prefix_width * c.page, sm_count);
+    ManyRows p = many_rows(q, q_stride, pre, nullptr, rep, c.B, c.B, m, scale_log2, out, out_stride, prefix_parts);
+    p.mask = Mask{0, 0, c.B};
+    if (const int rc = many_rows_launch(p, s)) return rc;
+    a.prefix_kind = 2;
+    a.many_part = p.part;
+    a.many_stat = p.stat;
+    a.many_splits = m.splits;
+    a.many_tiles = m.slots;
   }
-  const unsigned grid = (unsigned)(((long long)c.B * Hq + 3) / 4);
-  (c.D == 64 ? attention_kernel<64> : attention_kernel<128>)<<<grid, 128, 0, s>>>(
-      static_cast<const __nv_bfloat16*>(q), q_stride, c, nullptr, c.B, Hq, 0, 0, scale,
-      static_cast<__nv_bfloat16*>(out), out_stride, prefix_table, prefix_width, prefix_len);
-  return (int)cudaGetLastError();
+  a.own = few_rows(q, q_stride, c, nullptr, rep, scale_log2, out, out_stride, workspace, own_slots, sm_count, c.B, 1);
+  a.own.mask = Mask{0, 0, 0};
+  a.own.parts_only = 1;
+  if (const int rc = launch_few(a.own, s)) return rc;
+  return join(a, rep, s);
 }
 
 }  // namespace b2

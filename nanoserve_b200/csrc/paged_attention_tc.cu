@@ -1,0 +1,566 @@
+// Attention over a paged cache, many rows (prompts, several new tokens, a batch behind a shared prefix): tcgen05.
+//
+// Rows (token, query head) of a sequence that share a KV head are the M side of both products, 128 to a tile:
+//   S (128 x 128 keys, fp32 in tensor memory) = Q (shared memory) . K^T (shared memory)
+//   P = 2^(S scale/ln2 - m), rounded to bf16, over S in tensor memory
+//   O (128 x D, fp32 in tensor memory) += P (tensor memory) . V (shared memory, keys along the contraction as they lie)
+// A CTA holds two tiles' worth of tensor memory (S and O twice, all 512 columns), so that the tensor core works on one while
+// the other's softmax runs:
+//   two tiles (TWO)  two neighbouring row tiles share every block of keys
+//   one tile         up to 128 rows: the two halves take blocks of keys in turn, and are joined at the end
+// warps 0-3 / 4-7   softmax of the first / second half: one thread per row, 128 scores of it in registers
+// warp 8            loads: a ring of tiles of 128 keys (K, V in the order in which they are used), a page's rows per box
+// warp 9            issues the products (10, 11: nothing)
+// The running maximum moves only when a row's new one is over 2^8 times as much in weight (sums stay far inside fp32's range
+// and the bf16 of a weight is as exact at 2^8 as at 1); O is then rescaled in tensor memory by the softmax warps, between the
+// two products that use it.
+// Every wait is bounded; a time-out is recorded in the device's status word.
+#include <algorithm>
+
+#include "paged_attention.cuh"
+#include "ptx.cuh"
+#include "w4_internal.h"
+
+namespace b2 {
+namespace {
+
+constexpr int kKeys = 128;     // keys per block
+constexpr int kThreads = 384;  // three warpgroups: registers are handed over in wholes of them
+constexpr int kRegsSoftmax = 232, kRegsOther = 40;  // 2 * 232 + 40 = 3 * 168, what the launch gives
+constexpr int kPresent = 16;   // blocks whose presence bits are kept
+
+template <int D, bool TWO>
+struct Geo {
+  static constexpr int kTile = 128 * D * 2;                  // 128 rows of Q, K or V
+  static constexpr int kQ = (TWO ? 2 : 1) * kTile;
+  static constexpr int kBufs = std::min(12, (224 * 1024 - kQ) / kTile);
+  static constexpr int kBar = kQ + kBufs * kTile;
+  static constexpr int kSmem = kBar + 1024 + 1024;           // barriers; room to align to 1024
+  static constexpr int kRowsPerCta = TWO ? 256 : 128;
+};
+
+// D[tmem] (+)= A[tmem] . B[smem]
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// V as it lies: rows of keys (the contraction) of 64 elements of D, 128-byte swizzle.  The next 64 elements lie a tile of 128
+// rows further (leading offset), the next eight keys 1024 bytes (stride offset).
+__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
+  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>((128 * 128) >> 4) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+
+// Ones in the bits below x.
+__device__ __forceinline__ unsigned below(int x) { return x <= 0 ? 0u : x >= 32 ? ~0u : (1u << x) - 1; }
+
+// The sequence and first row of tile `t` (tiles of `size` rows, sequence after sequence); false: there is none.
+__device__ __forceinline__ bool find_tile(const ManyRows& p, int size, int t, int* b_out, int* r_out) {
+  const int lane = threadIdx.x & 31;
+  if (p.mask.flat) {
+    *b_out = 0;
+    *r_out = t * size;
+    return *r_out < p.mask.flat * p.rep;
+  }
+  int before = 0;
+  for (int b0 = 0; b0 < p.c.B; b0 += 32) {
+    const int b = b0 + lane;
+    int n = 0;
+    if (b < p.c.B) {
+      n = p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - __ldcg(p.cu_tokens + b) : 1;
+      n = (max(0, min(n, p.max_tokens)) * p.rep + size - 1) / size;
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const unsigned beyond = __ballot_sync(0xffffffffu, before + x > t);
+    if (beyond != 0) {
+      const int l = __ffs(beyond) - 1;
+      *b_out = b0 + l;
+      *r_out = (t - before - __shfl_sync(0xffffffffu, x - n, l)) * size;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, x, 31);
+  }
+  return false;
+}
+
+// Rows r0 .. of sequence b as a tile of the kernel: what they see, and how many there are.
+struct Tile {
+  Visible v;     // rows: of the tile, counted in (token, head)
+  int n_new, p0;  // tokens of the sequence in this call, position of the first
+  __device__ __forceinline__ void set(const ManyRows& p, int b, int r0, int size) {
+    v.first = p.mask.flat ? 0 : p.cu_tokens ? __ldcg(p.cu_tokens + b) : b;
+    n_new = p.mask.flat ? p.mask.flat : p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - v.first : 1;
+    v.rows = n_new;
+    v.set<kKeys>(p.mask, __ldcg(p.c.lens + b), p.c.width << p.c.page_shift);
+    p0 = v.pmin;
+    const int all = v.first < 0 ? 0 : min(min(n_new, p.max_tokens), p.T - v.first) * p.rep;
+    v.rows = max(0, min(size, all - r0));
+    if (!p.mask.flat) {
+      v.pmax = p0 + (r0 + max(v.rows, 1) - 1) / p.rep;
+      v.pmin = p0 + r0 / p.rep;
+      v.span<kKeys>(p.mask);
+    }
+  }
+};
+
+template <int D, bool TWO>
+__global__ void __launch_bounds__(kThreads, 1)
+    many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const ManyRows p) {
+  using geo = Geo<D, TWO>;
+  constexpr int kHalves = D / 64;
+  constexpr int kAhead = TWO ? 1 : 2;  // blocks whose scores are under way before the first weights are there
+  extern __shared__ unsigned char raw[];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  unsigned char* gen = raw + (base - smem_u32(raw));
+  const uint32_t ring = base + geo::kQ;
+  const uint32_t bar_full = base + geo::kBar, bar_empty = bar_full + 8 * geo::kBufs;
+  const uint32_t bar_s = bar_empty + 8 * geo::kBufs, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_q = bar_o + 16;
+  unsigned char* misc = gen + geo::kBar + 16 * geo::kBufs + 56;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 4);
+  volatile unsigned* present = reinterpret_cast<volatile unsigned*>(misc + 8);  // [kPresent]
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+
+  if (tid == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < geo::kBufs; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar_s + 8 * t, 1);
+      mbar_init(bar_p + 8 * t, 4);
+      mbar_init(bar_o + 8 * t, 1);
+    }
+    mbar_init(bar_q, 8);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+
+  // the longest tiles of a prompt are its last
+  const int z = blockIdx.x % p.splits, h = blockIdx.x / p.splits % p.c.Hk;
+  const int tile = gridDim.x / (p.splits * p.c.Hk) - 1 - blockIdx.x / (p.splits * p.c.Hk);
+  int b = 0, r0 = 0;
+  const bool exists = find_tile(p, geo::kRowsPerCta, tile, &b, &r0);
+  Tile tl;
+  int i0 = 0, n = 0;
+  if (exists) {
+    tl.set(p, b, r0, geo::kRowsPerCta);
+    i0 = (int)((long long)tl.v.count * z / p.splits);
+    n = (int)((long long)tl.v.count * (z + 1) / p.splits) - i0;
+  }
+  const Visible& v = tl.v;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (exists && warp == 8) {
+    // ------------------------------------------------------------ loads
+    const int box_rows = min(p.c.page, kKeys), boxes = kKeys / box_rows;
+    const int bx = lane % boxes, half = lane / boxes;
+    const int* table = p.c.table + b * p.c.table_stride;
+    // loads 0 .. kAhead - 1: K of these blocks; then V of block i, K of block i + kAhead, in turn
+    const int ahead = min(kAhead, n), total = 2 * n;
+    auto what = [&](int x, int* block) {
+      if (x < ahead) {
+        *block = x;
+        return 0;
+      }
+      const int y = x - ahead;
+      if (y < 2 * (n - ahead)) {
+        *block = (y >> 1) + ((y & 1) ? ahead : 0);
+        return (y & 1) ? 0 : 1;
+      }
+      *block = n - ahead + (y - 2 * (n - ahead));  // V of the last blocks
+      return 1;
+    };
+    auto page_of = [&](int x) {
+      int block;
+      what(x, &block);
+      return page_at(p.c, table, p.c.width, (v.block(i0 + block) * kKeys + bx * box_rows) >> p.c.page_shift);
+    };
+    int page = total > 0 ? page_of(0) : 0, s = 0;
+    uint32_t ph = 0;
+    for (int x = 0; x < total; ++x) {
+      const int page_next = x + 1 < total ? page_of(x + 1) : 0;
+      int block;
+      const int is_v = what(x, &block);
+      mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
+      __syncwarp();
+      const unsigned there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << boxes) - 1);
+      if (lane == 0) {
+        if (!is_v) present[block % kPresent] = there;
+        mbar_arrive_expect_tx(bar_full + 8 * s, geo::kTile);
+      }
+      __syncwarp();
+      if (half < kHalves)
+        tma_load_4d(ring + s * geo::kTile + half * (128 * 128) + bx * box_rows * 128, is_v ? &tmap_v : &tmap_k, half * 64,
+                    (v.block(i0 + block) * kKeys + bx * box_rows) & (p.c.page - 1), h, page < 0 ? p.c.n_pages : page,
+                    bar_full + 8 * s);
+      page = page_next;
+      if (++s == geo::kBufs) { s = 0; ph ^= 1; }
+    }
+  } else if (exists && warp == 9) {
+    // ------------------------------------------------------------ products
+    constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128);
+    constexpr uint32_t idesc_o = umma_idesc_bf16(128, D) | (1u << 16);  // B along N as it lies
+    int s = 0;
+    uint32_t ph = 0;
+    auto scores = [&](int t, uint32_t buf) {
+      const uint64_t dq = umma_desc_k128(base + (TWO ? t * geo::kTile : 0)), dk = umma_desc_k128(buf);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        umma_f16_ss(tmem + 128 * t, dq + (kk >> 2) * ((128 * 128) >> 4) + 2 * (kk & 3),
+                    dk + (kk >> 2) * ((128 * 128) >> 4) + 2 * (kk & 3), idesc_s, kk > 0);
+      umma_commit(bar_s + 8 * t);
+    };
+    auto values = [&](int t, uint32_t buf, bool first) {
+      const uint64_t dv = desc_v(buf);
+#pragma unroll
+      for (int kk = 0; kk < kKeys / 16; ++kk)
+        umma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * kk, dv + kk * (2048 >> 4), idesc_o, !first || kk > 0);
+    };
+    auto loaded = [&] {
+      mbar_wait(bar_full + 8 * s, ph, abort_flag);
+      __syncwarp();
+      tc_fence_after_sync();
+      return ring + s * geo::kTile;
+    };
+    auto used = [&] {  // (the elected lane): the buffer is free once what was issued is done
+      umma_commit(bar_empty + 8 * s);
+    };
+    auto step = [&] {
+      if (++s == geo::kBufs) { s = 0; ph ^= 1; }
+    };
+    if (n > 0) mbar_wait(bar_q, 0, abort_flag);
+    for (int i = 0; i < min(kAhead, n); ++i) {
+      const uint32_t buf = loaded();
+      if (elect_one()) {
+        scores(TWO ? 0 : i, buf);
+        if (TWO) scores(1, buf);
+        used();
+      }
+      __syncwarp();
+      step();
+    }
+    for (int i = 0; i < n; ++i) {
+      const uint32_t buf_v = loaded();
+      const int j0 = v.block(i0 + i) * kKeys;
+      // keys that no row sees may hold anything, and 0 times an infinity is none: their values become zeros
+      if (!(v.any(p.mask, j0) && v.any(p.mask, j0 + kKeys - 1) &&
+            (p.mask.window == 0 || j0 > v.pmin - p.mask.window || j0 + kKeys <= p.mask.sinks))) {
+        for (int x = lane; x < kKeys * kHalves * 8; x += 32) {
+          const int key = x / (kHalves * 8), half = x / 8 % kHalves;
+          if (!v.any(p.mask, j0 + key))
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(buf_v + half * (128 * 128) + key * 128 + (x & 7) * 16),
+                         "r"(0)
+                         : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      const int s_v = s;
+      step();
+      if constexpr (TWO) {
+        uint32_t buf_k = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          mbar_wait(bar_p + 8 * t, i & 1, abort_flag);
+          __syncwarp();
+          if (t == 0 && i + 1 < n) buf_k = loaded();
+          tc_fence_after_sync();
+          if (elect_one()) {
+            values(t, buf_v, i == 0);
+            if (t == 1) umma_commit(bar_empty + 8 * s_v);
+            if (i + 1 < n) {
+              scores(t, buf_k);
+              if (t == 1) used();
+            } else {
+              umma_commit(bar_o + 8 * t);
+            }
+          }
+          __syncwarp();
+        }
+        if (i + 1 < n) step();
+      } else {
+        const int t = i & 1;
+        mbar_wait(bar_p + 8 * t, (i >> 1) & 1, abort_flag);
+        __syncwarp();
+        tc_fence_after_sync();
+        if (elect_one()) {
+          values(t, buf_v, i < 2);
+          umma_commit(bar_empty + 8 * s_v);
+          if (i + 2 >= n) umma_commit(bar_o + 8 * t);
+        }
+        __syncwarp();
+        if (i + 2 < n) {
+          const uint32_t buf_k = loaded();
+          if (elect_one()) {
+            scores(t, buf_k);
+            used();
+          }
+          __syncwarp();
+          step();
+        }
+      }
+    }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    if (exists) {
+    // ------------------------------------------------------------ softmax: a row per thread
+    const int t = warp >> 2, row = tid & 127;
+    const int r = r0 + (TWO ? 128 * t : 0) + row, tok = r / p.rep, head = h * p.rep + r - tok * p.rep;
+    const bool real = (TWO ? 128 * t : 0) + row < v.rows;
+    {
+      // Q: a row per thread, or half of one; chunk c of sixteen bytes of row r lies at c ^ (r & 7)
+      constexpr int kChunks = TWO ? D / 8 : D / 16;
+      const __nv_bfloat16* q = p.q + (long long)(v.first + tok) * p.q_stride + head * D;
+      const uint32_t dst = base + (TWO ? t * geo::kTile : 0) + row * 128;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int cc = TWO ? c : t * kChunks + c;
+        const uint4 x = real ? __ldcg(reinterpret_cast<const uint4*>(q) + cc) : make_uint4(0, 0, 0, 0);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (cc >> 3) * (128 * 128) +
+                                                                      (((cc & 7) ^ (row & 7)) << 4)),
+                     "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                     : "memory");
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q);
+    }
+    const int pos = p.mask.flat ? v.pmax : tl.p0 + tok;
+    // positions of this warp's rows
+    const int w0 = r0 + (TWO ? 128 * t : 0) + (warp & 3) * 32;
+    Visible wv = v;
+    if (!p.mask.flat) {
+      wv.pmin = tl.p0 + w0 / p.rep;
+      wv.pmax = tl.p0 + (w0 + 31) / p.rep;
+    }
+    const int all_present = (1 << (kKeys / min(p.c.page, kKeys))) - 1;
+    const int box_shift = min(p.c.page_shift, 7);
+    const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
+    const uint32_t t_s = tmem + lanes + 128 * t, t_o = tmem + lanes + 256 + 128 * t;
+    float m = -INFINITY, l = 0.f;
+    int k = 0;  // blocks that this half has had
+    for (int i = TWO ? 0 : t; i < n; i += TWO ? 1 : 2, ++k) {
+      const int j0 = v.block(i0 + i) * kKeys;
+      mbar_wait(bar_s + 8 * t, k & 1, abort_flag);
+      __syncwarp();
+      tc_fence_after_sync();
+      float s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+      tmem_ld_wait();
+      const unsigned there = present[i % kPresent];
+      if (there != (unsigned)all_present || !wv.all(p.mask, j0, kKeys)) {
+        // visible columns: first ones up to `few`, and those from `lo` to `hi`
+        const int hi = min(pos, v.end - 1) - j0;
+        const int lo = p.mask.window ? pos - p.mask.window + 1 - j0 : 0;
+        const int few = p.mask.window ? min(p.mask.sinks - j0, hi + 1) : 0;
+        unsigned gone = 0;  // sixteen keys to a bit
+#pragma unroll 1
+        for (int g = 0; g < 8; ++g)
+          gone |= ((there >> (16 * g >> box_shift)) & 1) ? 0u : 1u << g;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          unsigned keep = (below(hi + 1 - 32 * w) & ~below(lo - 32 * w)) | below(few - 32 * w);
+          keep &= ((gone >> (2 * w)) & 1 ? 0xffff0000u : ~0u) & ((gone >> (2 * w)) & 2 ? 0xffffu : ~0u);
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (!((keep >> c) & 1)) s[32 * w + c] = -INFINITY;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 128; ++c) mx = fmaxf(mx, s[c]);
+      const bool move = (mx - m) * p.scale_log2 > 8.f;  // (the first maximum that is one: m is -inf)
+      const float mn = move ? mx : m;
+      if (__any_sync(0xffffffffu, move)) {
+        const float corr = m == -INFINITY ? 0.f : ex2((m - mn) * p.scale_log2);
+        l *= corr;
+        if (k > 0) {
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x16(t_o + 16 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st_32x16(t_o + 16 * c, o);
+          }
+        }
+        m = mn;
+      }
+      const float neg = m == -INFINITY ? 0.f : -m * p.scale_log2;
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float2 x = make_float2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]);
+          x = fma_f32x2(x, make_float2(p.scale_log2, p.scale_log2), make_float2(neg, neg));
+          x = make_float2(ex2(x.x), ex2(x.y));
+          sum = add_f32x2(sum, x);
+          const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
+          w[e] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        tmem_st_32x32(t_s + 32 * c, w);
+      }
+      l += sum.x + sum.y;
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_p + 8 * t);
+    }
+    // ------------------------------------------------------------ results
+    if constexpr (TWO) {
+      if (n > 0) mbar_wait(bar_o + 8 * t, 0, abort_flag);
+      __syncwarp();
+      tc_fence_after_sync();
+    } else {
+      // the second half's rows through the ring, which both halves' products have left
+      if (n > 0) mbar_wait(bar_o, 0, abort_flag);
+      if (n > 1) mbar_wait(bar_o + 8, 0, abort_flag);
+      __syncwarp();
+      tc_fence_after_sync();
+      float* other = reinterpret_cast<float*>(gen + geo::kQ);  // [D + 2][128]
+      if (t == 1 && n > 1) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_o + 32 * c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) other[(32 * c + e) * 128 + row] = __uint_as_float(o[e]);
+        }
+        other[D * 128 + row] = m;
+        other[(D + 1) * 128 + row] = l;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    if (TWO || t == 0) {
+      float f0 = 1.f, f1 = 0.f;
+      const float* other = reinterpret_cast<const float*>(gen + geo::kQ);
+      if (!TWO && n > 1) {
+        const float m1 = other[D * 128 + row], l1 = other[(D + 1) * 128 + row], mn = fmaxf(m, m1);
+        f0 = m == mn ? 1.f : ex2((m - mn) * p.scale_log2);
+        f1 = m1 == mn ? 1.f : ex2((m1 - mn) * p.scale_log2);
+        l = f0 * l + f1 * l1;
+        m = mn;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const long long slot = (((long long)h * p.slots + (TWO ? 2 * tile + t : tile)) * p.splits + z) * 128 + row;
+      __nv_bfloat16* out = p.out + (long long)(v.first + tok) * p.out_stride + head * D;
+      if (p.part != nullptr && real) p.stat[slot] = make_float2(m * p.scale_log2, l);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        if (n > 0) {
+          tmem_ld_32x32(t_o + 32 * c, o);
+          tmem_ld_wait();
+        }
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          x[e] = n > 0 ? __uint_as_float(o[e]) : 0.f;
+          if (!TWO && n > 1) x[e] = f0 * x[e] + f1 * other[(32 * c + e) * 128 + row];
+        }
+        if (real && p.part != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(p.part + slot * D + 32 * c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        } else if (real) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float y[8];
+#pragma unroll
+            for (int a = 0; a < 8; ++a) y[a] = inv == 0.f ? 0.f : x[e + a] * inv;
+            store8(out + 32 * c + e, y);
+          }
+        }
+      }
+    }
+  }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (tid == 0 && *abort_flag && p.status) atomicCAS(p.status, 0, kStatusGemmTimeout);
+}
+
+// Splits of the keys joined, in their order: a CTA of D threads per eight rows of a tile of 128.
+template <int D>
+__global__ void __launch_bounds__(D) join_many_kernel(const ManyRows p) {
+  const int d = threadIdx.x, h = blockIdx.x / p.slots, slot = blockIdx.x % p.slots;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const int size = p.two ? 256 : 128;
+  int b, r0;
+  if (!find_tile(p, size, p.two ? slot >> 1 : slot, &b, &r0)) return;
+  Tile tl;
+  tl.set(p, b, r0, size);
+  const int off = p.two ? 128 * (slot & 1) : 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const int row = blockIdx.y * 8 + i, r = r0 + off + row;
+    if (off + row >= tl.v.rows) return;
+    const long long at = ((long long)h * p.slots + slot) * p.splits * 128 + row;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+    for (int z = 0; z < p.splits; ++z) m = fmaxf(m, __ldcg(&p.stat[at + z * 128].x));
+    for (int z = 0; z < p.splits; ++z) {
+      const float2 st = __ldcg(&p.stat[at + z * 128]);
+      if (st.y == 0.f) continue;
+      const float f = st.x == m ? 1.f : ex2(st.x - m);
+      l += f * st.y;
+      o += f * __ldcg(p.part + (at + z * 128) * D + d);
+    }
+    const int tok = r / p.rep;
+    p.out[(long long)(tl.v.first + tok) * p.out_stride + (h * p.rep + r - tok * p.rep) * D + d] =
+        __float2bfloat16(l == 0.f ? 0.f : o / l);
+  }
+}
+
+template <int D, bool TWO>
+int launch(const ManyRows& p, cudaStream_t s) {
+  CUtensorMap mk, mv;
+  if (!paged_tensor_maps(p.c, kKeys, &mk, &mv)) return kErrBadShape;
+  using geo = Geo<D, TWO>;
+  const int rc = (int)cudaFuncSetAttribute(many_rows_kernel<D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, geo::kSmem);
+  if (rc) return rc;
+  const int tiles = TWO ? p.slots / 2 : p.slots;
+  return launch_pdl(many_rows_kernel<D, TWO>, dim3((unsigned)(tiles * p.c.Hk * p.splits)), kThreads, geo::kSmem, s, mk, mv, p);
+}
+
+}  // namespace
+
+int many_rows_launch(const ManyRows& p, cudaStream_t s) {
+  if (p.c.D == 64) return p.two ? launch<64, true>(p, s) : launch<64, false>(p, s);
+  return p.two ? launch<128, true>(p, s) : launch<128, false>(p, s);
+}
+int join_many_launch(const ManyRows& p, cudaStream_t s) {
+  const dim3 grid((unsigned)(p.slots * p.c.Hk), 16);
+  return p.c.D == 64 ? launch_pdl(join_many_kernel<64>, grid, 64, 0, s, p) : launch_pdl(join_many_kernel<128>, grid, 128, 0, s, p);
+}
+
+}  // namespace b2
