@@ -38,21 +38,39 @@ struct Geo {
   static constexpr int kStage = 2 * kTile;
   static constexpr int kStages = D == 128 ? 6 : 12;
   static constexpr int kJoin = kStages * kStage;              // the warps' 16 x D sums, joined here
-  static constexpr int kBar = kJoin + kWarps * kRows * D * 4;
+  static constexpr int kPitch = D + 4;                        // floats from row to row there: rows start in different banks
+  static constexpr int kBar = kJoin + kWarps * kRows * kPitch * 4;
   static constexpr int kSmem = kBar + 1024 + 1024;            // barriers, statistics; room to align to 1024
 };
 
-// The run of blocks of CTA c, of n CTAs, out of `total`.
-__device__ __forceinline__ long long run_start(long long total, int n, int c) { return total * c / n; }
-// The CTA whose run block u is in.
-__device__ __forceinline__ int run_owner(long long total, int n, long long u) { return (int)(((u + 1) * n - 1) / total); }
+// Equal runs of `total` blocks over n CTAs: where CTA c's begins, and the CTA whose run block u is in.
+struct Runs {
+  unsigned each, more;  // the first `more` CTAs have one block more than `each`
+  __device__ __forceinline__ Runs(unsigned total, unsigned n) : each(total / n), more(total - each * n) {}
+  __device__ __forceinline__ unsigned start(unsigned c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ unsigned owner(unsigned u) const {
+    const unsigned longer = more * (each + 1);
+    return u < longer ? u / (each + 1) : more + (u - longer) / each;
+  }
+};
 
+// What the device says about a sequence.
+struct Told {
+  int first, rows, len;
+};
+__device__ __forceinline__ Told told(const FewRows& p, int b) {
+  Told t;
+  t.first = p.mask.flat ? 0 : p.cu_tokens ? __ldcg(p.cu_tokens + b) : b;
+  t.rows = p.mask.flat ? p.mask.flat : p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - t.first : 1;
+  t.len = __ldcg(p.c.lens + b);
+  return t;
+}
 // A sequence's rows and what they see; at least one block, so that somebody writes the rows that see nothing.
-__device__ __forceinline__ Visible sequence_rows(const FewRows& p, int b) {
+__device__ __forceinline__ Visible sequence_rows(const FewRows& p, const Told& t) {
   Visible v;
-  v.first = p.mask.flat ? 0 : p.cu_tokens ? __ldcg(p.cu_tokens + b) : b;
-  v.rows = p.mask.flat ? p.mask.flat : p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - v.first : 1;
-  v.set<kKeys>(p.mask, __ldcg(p.c.lens + b), p.c.width << p.c.page_shift);
+  v.first = t.first;
+  v.rows = t.rows;
+  v.set<kKeys>(p.mask, t.len, p.c.width << p.c.page_shift);
   v.rows = v.first < 0 ? 0 : max(0, min(min(v.rows, min(p.max_tokens, kRows / p.rep)), p.T - v.first));
   v.count = v.rows == 0 ? 0 : max(1, v.count);
   return v;
@@ -62,51 +80,82 @@ __device__ __forceinline__ int first_head(const FewRows& p, int h) { return h / 
 __device__ __forceinline__ int tile_rows(const FewRows& p, const Visible& v, int h) {
   return v.rows * min(p.rep, p.rep_all - h % p.groups * kRows);
 }
-// Blocks of sequences 0 .. b - 1 of one KV head, for the sequences of a warp's lanes in turn; the whole warp asks.
-// With `stop` >= 0 ends at the sequence that holds block `stop` of them (counted over all KV heads) and returns it.
-__device__ __forceinline__ int add_up(const FewRows& p, long long stop, int upto, long long* sum) {
-  const int lane = threadIdx.x & 31;
-  long long before = 0;
-  for (int b0 = 0; b0 < upto; b0 += 32) {
-    const int b = b0 + lane;
-    int n = b < upto ? sequence_rows(p, b).count : 0, x = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+// The sequences as a warp sees them, 32 at a time, one to a lane; the first 32 are kept.  The whole warp asks.
+struct Sequences {
+  Told kept;
+  int kept_n;  // this lane's blocks of a KV head
+  unsigned total;  // blocks of all sequences and KV heads
+  __device__ __forceinline__ Sequences(const FewRows& p) {
+    const int lane = threadIdx.x & 31;
+    unsigned sum = 0;
+    for (int b0 = 0; b0 < p.c.B; b0 += 32) {
+      Told t{};
+      int n = 0;
+      if (b0 + lane < p.c.B) {
+        t = told(p, b0 + lane);
+        n = sequence_rows(p, t).count;
+      }
+      if (b0 == 0) kept = t, kept_n = n;
+      sum += __reduce_add_sync(0xffffffffu, (unsigned)n);
     }
-    if (stop >= 0) {
-      const unsigned beyond = __ballot_sync(0xffffffffu, (before + x) * p.heads > stop);
+    total = sum * p.heads;
+  }
+  __device__ __forceinline__ Visible rows(const FewRows& p, int b) const {
+    Told t;
+    if (b < 32) {
+      t.first = __shfl_sync(0xffffffffu, kept.first, b);
+      t.rows = __shfl_sync(0xffffffffu, kept.rows, b);
+      t.len = __shfl_sync(0xffffffffu, kept.len, b);
+    } else {
+      t = told(p, b);
+    }
+    return sequence_rows(p, t);
+  }
+  // Blocks of one KV head in front of the sequence that holds block `stop` of them all, which is returned, or in front of
+  // sequence `upto`.
+  __device__ __forceinline__ int add_up(const FewRows& p, unsigned stop, int upto, unsigned* before) const {
+    const int lane = threadIdx.x & 31;
+    unsigned sum = 0;
+    for (int b0 = 0; b0 < upto; b0 += 32) {
+      const int b = b0 + lane;
+      const unsigned n = b >= upto ? 0 : b0 == 0 ? kept_n : sequence_rows(p, told(p, b)).count;
+      unsigned x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const unsigned beyond = __ballot_sync(0xffffffffu, (sum + x) * p.heads > stop);
       if (beyond != 0) {
         const int l = __ffs(beyond) - 1;
-        *sum = before + __shfl_sync(0xffffffffu, x - n, l);
+        *before = sum + __shfl_sync(0xffffffffu, x - n, l);
         return b0 + l;
       }
+      sum += __shfl_sync(0xffffffffu, x, 31);
     }
-    before += __shfl_sync(0xffffffffu, x, 31);
+    *before = sum;
+    return upto;
   }
-  *sum = before;
-  return upto;
-}
+};
 
-// Where a run stands: block i of sequence b and KV head h.
+// Where a run stands: block i of sequence b and tile h of it.
 struct Walk {
   int b, h, i;
   Visible v;
-  __device__ __forceinline__ void start(const FewRows& p, long long u) {
-    long long before;
-    b = add_up(p, u, p.c.B, &before);
-    v = sequence_rows(p, b);
+  __device__ __forceinline__ void start(const FewRows& p, const Sequences& all, unsigned u) {
+    unsigned before;
+    b = all.add_up(p, u, p.c.B, &before);
+    v = all.rows(p, b);
     const int off = (int)(u - before * p.heads);
     h = off / v.count;
     i = off - h * v.count;
   }
-  __device__ __forceinline__ void next(const FewRows& p) {
+  __device__ __forceinline__ void next(const FewRows& p, const Sequences& all) {
     if (++i < v.count) return;
     i = 0;
     if (++h < p.heads) return;
     h = 0;
-    do v = sequence_rows(p, ++b);
+    do v = all.rows(p, ++b);
     while (v.count == 0);  // (a run ends within the last sequence that has blocks)
   }
 };
@@ -137,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile unsigned* present = reinterpret_cast<volatile unsigned*>(gen + geo::kBar + 16 * geo::kStages + 8);  // [kStages]
   float* s_m = reinterpret_cast<float*>(gen + geo::kBar + 256 + 4 * 16);  // [kWarps][kRows] maxima, then sums
   float* s_l = s_m + kWarps * kRows;
-  float* s_o = reinterpret_cast<float*>(gen + geo::kJoin);                // [kWarps][kRows][D]
+  float* s_o = reinterpret_cast<float*>(gen + geo::kJoin);                // [kWarps][kRows][kPitch]
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
@@ -151,17 +200,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmap_v);
   }
   __syncthreads();
+  if (!p.late_wait) pdl_wait_prior_grid();
   pdl_launch_dependents();
-  pdl_wait_prior_grid();
 
-  long long total;
-  add_up(p, -1, p.c.B, &total);
-  total *= p.heads;
+  const Sequences all(p);
   const int n_cta = gridDim.x, cta = blockIdx.x;
-  const long long u0 = run_start(total, n_cta, cta), u1 = run_start(total, n_cta, cta + 1);
-  if (u0 >= u1) return;
+  const Runs runs(all.total, n_cta);
+  const unsigned u0 = runs.start(cta), u1 = runs.start(cta + 1);
+  if (u0 >= u1) {
+    if (p.late_wait) pdl_wait_prior_grid();
+    return;
+  }
   Walk w;
-  w.start(p, u0);
+  w.start(p, all, u0);
 
   if (warp == kWarps) {
     // ------------------------------------------------------------ loads: one box of a page's rows per lane
@@ -174,11 +225,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     int page = page_of(w), s = 0;
     uint32_t ph = 0;
-    for (long long u = u0; u < u1; ++u) {
+    for (unsigned u = u0; u < u1; ++u) {
       Walk next = w;
       int page_next = 0;
       if (u + 1 < u1) {  // (the next block's table entries are on their way while this one's slot is waited for)
-        next.next(p);
+        next.next(p, all);
         page_next = page_of(next);
       }
       mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
@@ -210,12 +261,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int val_lane = 16 * warp + ((lane >> 3) & 1) * 8 + (lane & 7);  // V, transposed: row; chunk lane >> 4
   int s = 0;
   uint32_t ph = 0;
-  long long u = u0;
+  unsigned u = u0;
   while (u < u1) {
     // ---- one sequence and KV head, or what of them this run holds
     const Visible v = w.v;
     const int b = w.b, h = w.h, head0 = first_head(p, h), rows = tile_rows(p, v, h);
-    const int n_blocks = (int)min((long long)(v.count - w.i), u1 - u);
+    const int n_blocks = (int)min((unsigned)(v.count - w.i), u1 - u);
     const bool whole = n_blocks == v.count;
     uint32_t qf[D / 16][4];
     int pos[2];
@@ -336,11 +387,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 #pragma unroll
       for (int t = 0; t < D / 8; ++t)
-        *reinterpret_cast<float2*>(s_o + (warp * kRows + g + 8 * r) * D + 8 * t + 2 * quad) =
+        *reinterpret_cast<float2*>(s_o + (warp * kRows + g + 8 * r) * geo::kPitch + 8 * t + 2 * quad) =
             make_float2(o[t][2 * r], o[t][2 * r + 1]);
     }
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
-    const long long start = u - n_blocks;  // (a CTA begins at most one part, its first run, and ends at most one)
+    const unsigned start = u - n_blocks;  // (a CTA has at most two parts: what its run begins with, and what it ends with)
     const long long slot = whole ? 2LL * n_cta + b * p.heads + h : 2LL * cta + (start == u0 ? 0 : 1);
     const bool final = whole && !p.parts_only;
     constexpr int kQuads = D / 4;
@@ -354,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; k < kWarps; ++k) {
         const float f = s_m[k * kRows + row] == mm ? 1.f : ex2(s_m[k * kRows + row] - mm);
         ll += f * s_l[k * kRows + row];
-        const float4 t = *reinterpret_cast<const float4*>(s_o + (k * kRows + row) * D + d);
+        const float4 t = *reinterpret_cast<const float4*>(s_o + (k * kRows + row) * geo::kPitch + d);
         acc.x += f * t.x;
         acc.y += f * t.y;
         acc.z += f * t.z;
@@ -373,10 +424,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
     if (u < u1) {
       w.i += n_blocks - 1;
-      w.next(p);
+      w.next(p, all);
     }
   }
   if (tid == 0 && *abort_flag && p.status) atomicCAS(p.status, 0, kStatusGemvTimeout);
+  if (p.late_wait) pdl_wait_prior_grid();
 }
 
 // ---------------------------------------------------------------- joining parts
@@ -390,78 +442,110 @@ struct JoinArgs {
   int many_splits, many_tiles;
 };
 
-template <int D>
-struct Joined {
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  __device__ __forceinline__ void add(float2 st, float part) {
-    if (st.y == 0.f) return;
-    const float mn = fmaxf(m, st.x), was = m == mn ? 1.f : ex2(m - mn), f = st.x == mn ? 1.f : ex2(st.x - mn);
-    l = l * was + f * st.y;
-    o = o * was + f * part;
-    m = mn;
+// The parts of tile h of sequence b, written by few_rows_kernel: n of them, part i in slot(i).
+struct FewParts {
+  int c0, n, n_cta;
+  unsigned s, each, more;
+  long long whole;
+  __device__ __forceinline__ FewParts(const FewRows& p, const Sequences& all, const Visible& v, int b, int h)
+      : n_cta(p.n_cta), whole(2LL * p.n_cta + b * p.heads + h) {
+    unsigned before;
+    all.add_up(p, 0xffffffffu, b, &before);
+    const Runs runs(all.total, n_cta);
+    each = runs.each;
+    more = runs.more;
+    s = before * p.heads + (unsigned)h * v.count;
+    c0 = (int)runs.owner(s);
+    n = (int)runs.owner(s + v.count - 1) - c0 + 1;
   }
-  // n parts, slot(i) the i-th: eight loads on their way at a time.
-  template <typename Slot>
-  __device__ __forceinline__ void parts(const float2* stat, const float* part, int n, int rows, int row, int d, Slot slot) {
-    for (int i0 = 0; i0 < n; i0 += 8) {
-      float2 st[8];
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const long long at = i0 + i < n ? slot(i0 + i) : -1;
-        st[i] = at >= 0 ? __ldcg(stat + at * rows + row) : make_float2(-INFINITY, 0.f);
-        x[i] = at >= 0 ? __ldcg(part + (at * rows + row) * D + d) : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) add(st[i], x[i]);
-    }
+  __device__ __forceinline__ long long slot(int i) const {
+    if (n == 1) return whole;
+    const unsigned c = c0 + i;
+    return 2LL * c + (c * each + min(c, more) >= s ? 0 : 1);
   }
 };
 
-// The parts of sequence b's KV head h, written by few_rows_kernel on n_cta CTAs; whole: that it is in one part, `item` of them.
-template <int D>
-__device__ __forceinline__ bool join_few(Joined<D>& j, const FewRows& p, int b, int h, int row, int d, bool always) {
-  long long total, before;
-  add_up(p, -1, p.c.B, &total);
-  add_up(p, -1, b, &before);
-  total *= p.heads;
-  const int count = sequence_rows(p, b).count, n = p.n_cta;
-  if (count == 0) return false;
-  const long long s = before * p.heads + (long long)h * count;
-  const int c0 = run_owner(total, n, s), c1 = run_owner(total, n, s + count - 1);
-  if (c0 == c1) {
-    if (!always) return false;
-    j.parts(p.stat, p.part, 1, kRows, row, d, [&](int) { return 2LL * n + b * p.heads + h; });
-    return true;
-  }
-  j.parts(p.stat, p.part, c1 - c0 + 1, kRows, row, d, [&](int i) -> long long {
-    const long long at = run_start(total, n, c0 + i);
-    if (at == run_start(total, n, c0 + i + 1)) return -1;  // a CTA without a block
-    return 2LL * (c0 + i) + (at >= s ? 0 : 1);
-  });
-  return true;
-}
+constexpr int kMostParts = 1024;  // a tile's: one from each CTA that shares it, of the prefix and of its own keys
 
 template <int D>
 __global__ void __launch_bounds__(D) join_kernel(const JoinArgs a) {
+  __shared__ float s_w[kMostParts];
+  __shared__ float s_x[2][D / 32];
   const FewRows& p = a.own;
   const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, row = blockIdx.y, d = threadIdx.x;
-  pdl_launch_dependents();
   pdl_wait_prior_grid();
-  const Visible v = sequence_rows(p, b);
+  pdl_launch_dependents();
+  const Sequences all(p);
+  const Visible v = all.rows(p, b);
   if (row >= tile_rows(p, v, h)) return;
-  Joined<D> j;
+  const FewParts own(p, all, v, b, h);
+  if (own.n == 1 && a.prefix_kind == 0) return;  // written by its one CTA
+  // the prefix's parts in front, then its own: which rows of which arrays
+  int n_pre = 0, pre_rows = 1;
+  long long pre0 = 0;
+  const float2* pre_stat = nullptr;
+  const float* pre_part = nullptr;
+  FewParts pre = own;
   if (a.prefix_kind == 1) {
-    join_few<D>(j, a.prefix, 0, h, b * p.rep + row, d, true);
+    const Sequences one(a.prefix);
+    pre = FewParts(a.prefix, one, one.rows(a.prefix, 0), 0, h);
+    n_pre = pre.n;
+    pre_rows = kRows;
+    pre0 = b * p.rep + row;
+    pre_stat = a.prefix.stat;
+    pre_part = a.prefix.part;
   } else if (a.prefix_kind == 2) {
     const int r = b * p.rep_all + (h % p.groups) * kRows + row;
-    const long long tile = (long long)(h / p.groups) * a.many_tiles + r / 128;
-    j.parts(a.many_stat, a.many_part, a.many_splits, 128, r % 128, d, [&](int i) { return tile * a.many_splits + i; });
+    n_pre = a.many_splits;
+    pre_rows = 128;
+    pre0 = ((long long)(h / p.groups) * a.many_tiles + r / 128) * a.many_splits * 128 + r % 128;
+    pre_stat = a.many_stat;
+    pre_part = a.many_part;
   }
-  if (!join_few<D>(j, p, b, h, row, d, a.prefix_kind != 0) && a.prefix_kind == 0) return;  // written by its one CTA
+  const int n = n_pre + own.n;
+  auto at = [&](int i) { return i < n_pre ? pre0 + (a.prefix_kind == 1 ? pre.slot(i) : i) * pre_rows : own.slot(i - n_pre) * kRows + row; };
+  // ---- every part's weight, a thread to a part
+  float m = -INFINITY;
+  for (int i = d; i < n; i += D) {
+    const float2 st = __ldcg((i < n_pre ? pre_stat : p.stat) + at(i));
+    m = fmaxf(m, st.x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((d & 31) == 0) s_x[0][d >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < D / 32; ++w) m = fmaxf(m, s_x[0][w]);
+  float l = 0.f;
+  for (int i = d; i < n; i += D) {
+    const float2 st = __ldcg((i < n_pre ? pre_stat : p.stat) + at(i));
+    const float f = st.y == 0.f ? 0.f : st.x == m ? 1.f : ex2(st.x - m);
+    s_w[i] = f;
+    l += f * st.y;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if ((d & 31) == 0) s_x[1][d >> 5] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < D / 32; ++w) l += s_x[1][w];
+  // ---- the parts' rows, sixteen on their way at a time, added up in their order
+  float o = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 16) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      x[i] = i0 + i < n ? __ldcg((i0 + i < n_pre ? pre_part : p.part) + at(i0 + i) * D + d) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float f = i0 + i < n ? s_w[i0 + i] : 0.f;
+      if (f != 0.f) o += f * x[i];
+    }
+  }
   const int tok = row / p.rep;
   p.out[(long long)(v.first + tok) * p.out_stride + (first_head(p, h) + row - tok * p.rep) * D + d] =
-      __float2bfloat16(j.l == 0.f ? 0.f : j.o / j.l);
+      __float2bfloat16(l == 0.f ? 0.f : o / l);
 }
 
 // ---------------------------------------------------------------- host
@@ -512,6 +596,8 @@ int check_rows(const void* q, long long q_stride, const PagedCache& c, int T, in
   if (!(scale > 0.f) || scale > FLT_MAX || T < 1 || Hq < 1 || Hq % c.Hk || (c.D != 64 && c.D != 128)) return kErrBadShape;
   if (q_stride < (long long)Hq * c.D || q_stride % 8 || out_stride < (long long)Hq * c.D || out_stride % 8) return kErrBadShape;
   if (!q || !out || misaligned(q, 16) || misaligned(out, 16)) return kErrBadPointer;
+  // blocks are counted in 31 bits
+  if (((long long)c.width * c.page / kKeys + 2) * c.B * Hq > 0x7fffffffLL) return kErrTooLarge;
   return 0;
 }
 
@@ -665,6 +751,7 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
   a.own = few_rows(q, q_stride, c, nullptr, rep, scale_log2, out, out_stride, workspace, own_slots, sm_count, c.B, 1);
   a.own.mask = Mask{0, 0, 0};
   a.own.parts_only = 1;
+  a.own.late_wait = 1;
   if (const int rc = launch_few(a.own, s)) return rc;
   return join(a, rep, s);
 }

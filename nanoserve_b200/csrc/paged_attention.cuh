@@ -28,6 +28,8 @@ struct FewRows {
   int rep;           // of these in a tile: all, or sixteen of more (one row per sequence then)
   int groups, heads; // tiles per KV head of a sequence; KV heads times that
   int n_cta;
+  int late_wait;     // the kernel in front writes nothing that this one reads, and has seen what is in front of it complete:
+                     // it is waited for at the end
   int parts_only;    // whole sequences are left as parts too (slots 2 n_cta + sequence and KV head)
   float scale_log2;  // scale / ln 2
   float* part;       // [slot][16][D], not divided by the sum
