@@ -14,6 +14,7 @@ CSRC = os.path.join(ROOT, "nanoserve_b200", "csrc")
 LIB_DIR = os.path.join(ROOT, "build")
 LIB_PATH = os.path.join(LIB_DIR, "libnanoserve.so")
 CALL_SRC = os.path.join(CSRC, "binding.cpp")
+CALL_DEPS = (CALL_SRC, os.path.join(ROOT, "include", "nanoserve_b200.h"))
 CALL_PATH = os.path.join(LIB_DIR, "nanoserve_call.so")  # Python extension: the host side of an eager call
 
 NVCC_FLAGS = [
@@ -54,7 +55,7 @@ def build_call(force: bool = False) -> str:
     """Compile the Python extension (host code on torch's C++ objects; no CUDA sources) if its source is newer or it was built
     for another torch or Python."""
     if not force and os.path.exists(CALL_PATH) and call_matches(CALL_PATH) and \
-            os.path.getmtime(CALL_PATH) >= os.path.getmtime(CALL_SRC):
+            os.path.getmtime(CALL_PATH) >= max(os.path.getmtime(f) for f in CALL_DEPS):
         return CALL_PATH
     import sysconfig
     import torch

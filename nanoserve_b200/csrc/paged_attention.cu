@@ -556,8 +556,8 @@ template <int D>
 int launch_few_of(const FewRows& p, cudaStream_t s) {
   CUtensorMap mk, mv;
   if (!paged_tensor_maps(p.c, kKeys, &mk, &mv)) return kErrBadShape;
-  const int rc = (int)cudaFuncSetAttribute(few_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<D>::kSmem);
-  if (rc) return rc;
+  static SharedMemoryOnce once;
+  if (const int rc = once.allow(few_rows_kernel<D>, Geo<D>::kSmem)) return rc;
   return launch_pdl(few_rows_kernel<D>, dim3(p.n_cta), kThreads, Geo<D>::kSmem, s, mk, mv, p);
 }
 

@@ -3,6 +3,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "paged.h"
 #include "paged_rows.cuh"
 
@@ -57,6 +59,21 @@ struct ManyRows {
 };
 int many_rows_launch(const ManyRows& p, cudaStream_t s);
 int join_many_launch(const ManyRows& p, cudaStream_t s);
+
+// Dynamic shared memory beyond 48 KB is allowed a kernel once per device.
+struct SharedMemoryOnce {
+  std::atomic<unsigned long long> done{0};
+  template <typename K>
+  int allow(K* kernel, size_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (e != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return (int)e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return (int)e;
+  }
+};
 
 template <typename... Args>
 int launch_pdl(void (*kernel)(Args...), dim3 grid, int block, size_t smem, cudaStream_t s, Args... args) {

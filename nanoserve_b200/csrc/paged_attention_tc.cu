@@ -572,8 +572,8 @@ int launch(const ManyRows& p, cudaStream_t s) {
   CUtensorMap mk, mv;
   if (!paged_tensor_maps(p.c, kKeys, &mk, &mv)) return kErrBadShape;
   using geo = Geo<D, TWO>;
-  const int rc = (int)cudaFuncSetAttribute(many_rows_kernel<D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, geo::kSmem);
-  if (rc) return rc;
+  static SharedMemoryOnce once;
+  if (const int rc = once.allow(many_rows_kernel<D, TWO>, geo::kSmem)) return rc;
   const int tiles = TWO ? p.slots / 2 : p.slots;
   return launch_pdl(many_rows_kernel<D, TWO>, dim3((unsigned)(tiles * p.c.Hk * p.splits)), kThreads, geo::kSmem, s, mk, mv, p);
 }

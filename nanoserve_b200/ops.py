@@ -10,6 +10,7 @@ There is no CPU path: if the shared library is missing or a tensor is not on a C
 raises.
 """
 import ctypes
+import functools
 import os
 import warnings
 
@@ -162,6 +163,14 @@ def load_library(path: str = _LIB_DEFAULT) -> ctypes.CDLL:
     return lib
 
 
+# the operators of batched serving in the extension: their methods' names, and the entry points that they take the addresses of
+_SERVING = {"paged_kv_append": ("b2_paged_kv_append",),
+            "paged_attention": ("b2_paged_attention", "b2_paged_attention_workspace_bytes"),
+            "shared_prefix_attention": ("b2_shared_prefix_attention", "b2_shared_prefix_workspace_bytes"),
+            "sample": ("b2_sample",)}
+_serving = {}
+
+
 def _load_call():
     """The native host side of w4_linear and w4_quantize (csrc/binding.cpp), built beside the default library; None where it was
     not built, was built for another torch or Python, or does not load: calls then go through ctypes, to the same kernels."""
@@ -175,6 +184,7 @@ def _load_call():
             raise ImportError("built for another torch or Python")
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
+        _serving.update({name: getattr(module, name) for name in _SERVING})
         return module.w4_linear, module.w4_quantize
     except (ImportError, OSError, AttributeError) as e:
         warnings.warn(f"{path} does not load, eager calls go through ctypes (python -m nanoserve_b200.build --force "
@@ -201,6 +211,10 @@ class Kernels:
         address = lambda name: (ctypes.cast(getattr(self.lib, name), ctypes.c_void_p).value
                                 if native and hasattr(self.lib, name) else None)
         self._linear, self._quantize = address("b2_w4_linear"), address("ns_w4_quantize")
+        # (None: ctypes)
+        self._append, self._attend, self._prefix, self._sample = (
+            functools.partial(_serving[name], *map(address, symbols))
+            if name in _serving and all(map(address, symbols)) else None for name, symbols in _SERVING.items())
         for name in ("ns_rmsnorm", "ns_rope", "ns_swiglu", "ns_flash_fwd", "ns_w4_quantize", "ns_w4_linear"):
             getattr(self.lib, name)  # AttributeError if the library is not a drop-in
 
@@ -434,6 +448,11 @@ class Kernels:
         sequences' pages (caches [n_pages, Hk, page, D], block_table [B, width] and seq_lens [B] int32, the new tokens
         counted).  cu_tokens [B + 1] (int32): the first row of every sequence and the end of the last; None: one row each.
         Returns the rotated q, [T, Hq D]."""
+        if self._append is not None:
+            done = self._append(qkv, bias, inv_freq, cache_k, cache_v, block_table, seq_lens, n_heads, n_kv_heads, head_dim,
+                                cu_tokens, q_out)
+            if done is not NotImplemented:
+                return done
         what = "paged_kv_append"
         c = self._paged(what, cache_k, cache_v, block_table, seq_lens, n_kv_heads, head_dim)
         width = (n_heads + 2 * n_kv_heads) * head_dim
@@ -459,6 +478,11 @@ class Kernels:
         two share): causal attention, each row over its sequence up to itself, with `window` > 0 over the last `window` keys
         and the first `sinks`.  max_tokens: no sequence has more rows (None: T, or 1 without cu_tokens; a close bound lets
         short calls run the kernel for few rows).  scale: head_dim ** -0.5 unless given.  Returns [T, Hq D]."""
+        if self._attend is not None:
+            done = self._attend(q, cache_k, cache_v, block_table, seq_lens, n_heads, n_kv_heads, head_dim, cu_tokens, max_tokens,
+                                window, sinks, scale, out)
+            if done is not NotImplemented:
+                return done
         what = "paged_attention"
         c = self._paged(what, cache_k, cache_v, block_table, seq_lens, n_kv_heads, head_dim)
         cu = self._rows(what, q, n_heads * head_dim, cu_tokens, c.n_seqs)
@@ -483,6 +507,11 @@ class Kernels:
         """q [B, Hq D], one new token per sequence: attention over the first prefix_len (int32 [1], on the device) tokens of
         the pages prefix_table [width], which all sequences share, and over each sequence's own seq_lens[b] tokens (its new
         one among them).  The prefix is read once for all.  Returns [B, Hq D]."""
+        if self._prefix is not None:
+            done = self._prefix(q, cache_k, cache_v, prefix_table, prefix_len, block_table, seq_lens, n_heads, n_kv_heads, head_dim,
+                                scale, out)
+            if done is not NotImplemented:
+                return done
         what = "shared_prefix_attention"
         c = self._paged(what, cache_k, cache_v, block_table, seq_lens, n_kv_heads, head_dim)
         self._rows(what, q, n_heads * head_dim, None, c.n_seqs)
@@ -508,6 +537,10 @@ class Kernels:
         of their probability.  Each parameter is a number or a tensor [B] on the device (top_k int32, the others fp32);
         temperature 0 picks the largest logit, top_k 0, top_p 1 and min_p 0 leave all.  Returns int64 [B]; -1 where a row
         has no logit above minus infinity."""
+        if self._sample is not None:
+            done = self._sample(logits, u, temperature, top_k, top_p, min_p, out)
+            if done is not NotImplemented:
+                return done
         self._here(logits, u, out)
         self._need("sample", logits.dim() == 2, logits.dtype in (torch.bfloat16, torch.float32),
                    logits.stride(1) == 1 or logits.shape[1] == 1)
