@@ -70,10 +70,10 @@ struct Shared {
   u64 found[3];
 };
 
-__device__ __forceinline__ u32 peer_u32(const u32* p, u32 rank) {
-  u32 v;
-  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
-               : "=r"(v) : "r"(smem_u32(p)), "r"(rank) : "memory");
+__device__ __forceinline__ uint4 peer_u4(const u32* p, u32 rank) {
+  uint4 v;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [a];\n\t}"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem_u32(p)), "r"(rank) : "memory");
   return v;
 }
 __device__ __forceinline__ u64 peer_u64(const u64* p, u32 rank) {
@@ -106,8 +106,8 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* scan, u64* total) {
   return before + x - v;
 }
 
-template <typename L>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int C, int chunk) {
+template <typename L, int C>
+__global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int chunk) {
   using K = Keys<L>;
   using Stored = typename K::Stored;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   Stored* keys = reinterpret_cast<Stored*>(raw + sizeof(Shared));
   const int tid = threadIdx.x;
   const u32 rank = blockIdx.x % C;
-  const int row = blockIdx.x / C;
+  const int row = (int)(blockIdx.x / C);
   const int slice = kThreads * chunk, base = rank * slice;  // this CTA's logits: [base, base + slice), a chunk per thread
   const int n = max(0, min(p.V - base, slice));
   const Stored* mine = keys + tid * chunk;
@@ -124,11 +124,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   auto ask = [&](u64 v, u64* before) {
     if (tid == 0) sh.exchange[question] = v;
     cluster_barrier();
-    u64 sum = 0;
+    u64 told[C], sum = 0;
+#pragma unroll
+    for (u32 r = 0; r < (u32)C; ++r) told[r] = peer_u64(&sh.exchange[question], r);
     *before = 0;
+#pragma unroll
     for (u32 r = 0; r < (u32)C; ++r) {
       if (r == rank) *before = sum;
-      sum += peer_u64(&sh.exchange[question], r);
+      sum += told[r];
     }
     ++question;
     return sum;
@@ -137,7 +140,26 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   // ---- the row's slice as keys, and the largest
   const L* src = static_cast<const L*>(p.logits) + row * p.stride + base;
   u32 top = 0;
-  for (int i = tid; i < slice; i += kThreads) {
+  constexpr int kVec = 16 / sizeof(L);
+  const int vectors = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? n / kVec : 0;
+  for (int i = tid; i < vectors; i += kThreads) {
+    const uint4 x = __ldcg(reinterpret_cast<const uint4*>(src) + i);
+    const u32 w[4] = {x.x, x.y, x.z, x.w};
+    u32 out[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (K::kPerWord == 1) {
+        out[e] = key_of(__uint_as_float(w[e]));
+        top = max(top, out[e]);
+      } else {
+        const u32 lo = key_of(__uint_as_float(w[e] << 16)) >> 16, hi = key_of(__uint_as_float(w[e] & 0xffff0000u)) >> 16;
+        out[e] = lo | hi << 16;
+        top = max(top, max(lo, hi));
+      }
+    }
+    reinterpret_cast<uint4*>(keys)[i] = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+  for (int i = vectors * kVec + tid; i < slice; i += kThreads) {
     const u32 k = i < n ? key_of(K::load(src, i)) : 0;
     keys[i] = (Stored)K::stored(k);
     top = max(top, K::stored(k));
@@ -150,6 +172,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   if (tid == 0) sh.exchange[question] = sh.found[0];
   cluster_barrier();
   top = 0;
+#pragma unroll
   for (u32 r = 0; r < (u32)C; ++r) top = max(top, (u32)peer_u64(&sh.exchange[question], r));
   ++question;
   const float largest = K::logit(top);
@@ -162,9 +185,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   if (!(T > 0.f)) k = 1, T = 1.f;
   if (k <= 0 || k > p.V) k = p.V;
   const double per_T = 1.0 / (double)T;
+  // (a weight of e^-31.5 is under half of 2^-44; keys below this one need not be asked)
+  const u32 nothing = K::stored(key_of(largest - 40.f * T));
   // the weight of a stored key, in multiples of 2^-44
   auto weight = [&](u32 s) -> u64 {
     if (s == top) return (u64)kOne;
+    if (s < nothing) return 0;
     const double x = ((double)K::logit(s) - (double)largest) * per_T;
     return x < -31.5 ? 0 : (u64)rint(exp(x) * kOne);  // (not finite: below, or nan, which compares false and converts to 0)
   };
@@ -191,7 +217,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       const int bits = min(left, 11), shift = left - bits;
       u32 *lo = sh.lo[level & 1], *hi = sh.hi[level & 1];
       ++level;
-      for (int i = tid; i < (1 << bits); i += kThreads) lo[i] = 0, hi[i] = 0;
+      for (int i = tid; i < kBins / 4; i += kThreads) {
+        reinterpret_cast<uint4*>(lo)[i] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(hi)[i] = make_uint4(0, 0, 0, 0);
+      }
       __syncthreads();
       for (int i = 0; i < chunk; ++i) {
         const u32 s = mine[i];
@@ -206,22 +235,35 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
         }
       }
       cluster_barrier();
-      // bins in falling order, kBins / kThreads to a thread
-      constexpr int kEach = kBins / kThreads;
-      u64 sum[kEach], mass = 0;
+      // bins in falling order, four to a thread: bins top_bin - 3 .. top_bin
+      constexpr int kEach = 4;
+      static_assert(kBins == kEach * kThreads, "a thread reads its bins at once");
+      const int top_bin = (1 << bits) - 1 - tid * kEach;
+      u64 sum[kEach] = {}, mass = 0;
+      if (top_bin > 0) {
+        uint4 a[C], c[C];
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int bin = (1 << bits) - 1 - (tid * kEach + e);
-        sum[e] = 0;
-        if (bin >= 0) {
-          for (u32 r = 0; r < (u32)C; ++r) {
-            sum[e] += peer_u32(&lo[bin], r);
-            if (wide) sum[e] += (u64)peer_u32(&hi[bin], r) << 32;
-          }
-          const u32 here = l > 0 ? (prefix << bits) | (u32)bin : (u32)bin;
-          if (rf && (kf >> shift) == here) sum[e] += part;
+        for (u32 r = 0; r < (u32)C; ++r) {
+          a[r] = peer_u4(&lo[top_bin - 3], r);
+          c[r] = wide ? peer_u4(&hi[top_bin - 3], r) : make_uint4(0, 0, 0, 0);
         }
-        mass += sum[e];
+#pragma unroll
+        for (u32 r = 0; r < (u32)C; ++r) {
+          sum[0] += a[r].w + ((u64)c[r].w << 32);
+          sum[1] += a[r].z + ((u64)c[r].z << 32);
+          sum[2] += a[r].y + ((u64)c[r].y << 32);
+          sum[3] += a[r].x + ((u64)c[r].x << 32);
+        }
+        if (rf) {
+          const u32 first = (l > 0 ? prefix << bits : 0) | (u32)top_bin, at = first - (kf >> shift);
+          if (at < kEach) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+              if (at == (u32)e) sum[e] += part;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) mass += sum[e];
       }
       u64 total;
       u64 before = block_scan(mass, sh.scan, &total);
@@ -234,7 +276,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
           if (before < want && before + sum[e] >= want) {
-            sh.found[0] = (1 << bits) - 1 - (tid * kEach + e);
+            sh.found[0] = top_bin - e;
             sh.found[1] = before;
             sh.found[2] = sum[e];
           }
@@ -337,15 +379,12 @@ int chunk_of(int V, int C) {
   return (words | 1) * per;
 }
 
-template <typename L>
-int launch(const Sampling& p, cudaStream_t s) {
-  int C = 1;
-  while (C < 8 && (p.rows * C < 148 || (size_t)kThreads * chunk_of<L>(p.V, C) * sizeof(typename Keys<L>::Stored) > kSliceBytes))
-    C *= 2;
+template <typename L, int C>
+int launch_on(const Sampling& p, cudaStream_t s) {
   const int chunk = chunk_of<L>(p.V, C);
   const size_t smem = sizeof(Shared) + (size_t)kThreads * chunk * sizeof(typename Keys<L>::Stored);
   if (smem > 227 * 1024) return kErrTooLarge;
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<L, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.rows * C));
@@ -358,7 +397,20 @@ int launch(const Sampling& p, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, sample_kernel<L>, p, C, chunk);
+  return (int)cudaLaunchKernelEx(&cfg, sample_kernel<L, C>, p, chunk);
+}
+
+template <typename L>
+int launch(const Sampling& p, cudaStream_t s) {
+  const size_t row = (size_t)p.V * sizeof(typename Keys<L>::Stored);
+  int C = 1;
+  while (C < 8 && (p.rows * C < 148 || row / C > kSliceBytes)) C *= 2;
+  switch (C) {
+    case 1: return launch_on<L, 1>(p, s);
+    case 2: return launch_on<L, 2>(p, s);
+    case 4: return launch_on<L, 4>(p, s);
+    default: return launch_on<L, 8>(p, s);
+  }
 }
 
 }  // namespace
