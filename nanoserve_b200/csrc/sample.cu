@@ -9,9 +9,15 @@
 // as whole multiples of 2^-44: the sums do not depend on the order of the additions, and not on how a row is cut up.
 // (In 32 bits one draw in a few hundred ended on a neighbouring token.)
 //
-// A row is read once: a cluster of C CTAs keeps it in shared memory as sortable keys.  The borders are found by radix
-// selection on the keys (11 bits at a time; bf16 has 16, fp32 32): a histogram of counts for top_k and of weights for
-// top_p per CTA, added up over the cluster through distributed shared memory by every CTA for itself.
+// A row is read once: a cluster of C CTAs keeps it in shared memory as sortable keys.
+//   1. the largest key; a histogram of the others' distance from it in 2048 equal steps up to 40 T (beyond, a weight is 0 here):
+//      counts alone, one atomic an element.  Every CTA adds up a C-th of the bins over the cluster and sends the sums to all.
+//   2. counts bound both borders: exactly the bin of the top_k-th logit, and, since weights within a bin are e^(-40/2048) or
+//      nearer to one another, bins between which the top_p border lies.
+//   3. what is in front of the borders' far end is all that the rest looks at.  Up to 4096 logits are gathered, in the order
+//      of the vocabulary, in one CTA, which goes on alone; more stay where they are, and each step ends in a cluster barrier.
+//   4. the exact borders by radix selection on the keys (eight bits at a time), with counts and exact weights; the draw by
+//      prefix sums.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -21,12 +27,16 @@
 namespace b2 {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kThreads = 1024;
+constexpr int kBins = 2048;      // of the first histogram, of distances
+constexpr int kDigit = 256;      // of the selections on keys
+constexpr int kAtOnce = 4;       // elements of a thread whose weights are formed side by side
+constexpr int kList = 4096;      // logits that one CTA looks at alone
+constexpr float kReach = 40.f;   // distances beyond it, in T, have a weight under 2^-57: none
 constexpr int kMaxVocab = 1 << 18;
-constexpr int kSliceBytes = 160 * 1024;
+constexpr int kSliceBytes = 150 * 1024;
 constexpr double kOne = 17592186044416.0;  // 2^44: a weight of 1
+constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52: a double added to it is rounded to a whole number, in its low bits
 
 using u32 = unsigned;
 using u64 = unsigned long long;
@@ -63,18 +73,28 @@ struct Keys<__nv_bfloat16> {
   static __device__ __forceinline__ float logit(u32 s) { return logit_of((s << 16) | ((s & 0x8000u) ? 0u : 0xffffu)); }
 };
 
-struct Shared {
-  u32 lo[2][kBins], hi[2][kBins];  // a histogram (counts: lo alone), two in turn: peers may still read the other
-  u64 exchange[8];                 // what this CTA tells the others, a place per question
-  u64 scan[kWarps + 1];
+constexpr int kLimb = 15;  // a bin's weight in three sums of fifteen bits each: up to 2^17 elements leave them in 32 bits
+struct alignas(16) Shared {
+  u32 count[kBins];                // this CTA's, then (sums) the cluster's up to each bin, within the part of it one CTA adds up
+  u32 sums[kBins];
+  u32 limb[2][3][kDigit];          // a selection's bins (counts: the first alone), two in turn: peers may still read the other
+  double power[256];               // 2^44 2^(j / 256)
+  u64 exchange[12];                // what this CTA tells the others, a place per question
+  u64 scan[32], scanned[32];
   u64 found[3];
+  u32 list_key[kList], list_at[kList];  // keys and their places in the vocabulary
 };
 
-__device__ __forceinline__ uint4 peer_u4(const u32* p, u32 rank) {
-  uint4 v;
-  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [a];\n\t}"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem_u32(p)), "r"(rank) : "memory");
+__device__ __forceinline__ u32 peer_u32(const u32* p, u32 rank) {
+  u32 v;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
+               : "=r"(v) : "r"(smem_u32(p)), "r"(rank) : "memory");
   return v;
+}
+__device__ __forceinline__ void to_peer_u32(u32* p, u32 rank, u32 v) {
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.u32 [a], %2;\n\t}" ::"r"(smem_u32(p)),
+               "r"(rank), "r"(v)
+               : "memory");
 }
 __device__ __forceinline__ u64 peer_u64(const u64* p, u32 rank) {
   u64 v;
@@ -84,26 +104,24 @@ __device__ __forceinline__ u64 peer_u64(const u64* p, u32 rank) {
 }
 
 // Sum of v over the threads in front of the calling one; total: over all.
-__device__ __forceinline__ u64 block_scan(u64 v, u64* scan, u64* total) {
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, Shared& sh, T* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 x = v;
+  auto inclusive = [&](T x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const T y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  const T x = inclusive(v);
+  if (lane == 31) sh.scan[warp] = x;
   __syncthreads();
-  if (lane == 31) scan[warp] = x;
+  if (warp == 0) sh.scanned[lane] = inclusive((T)sh.scan[lane]);
   __syncthreads();
-  u64 before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const u64 y = scan[w];
-    if (w < warp) before += y;
-    all += y;
-  }
-  *total = all;
-  return before + x - v;
+  *total = (T)sh.scanned[31];
+  return (warp > 0 ? (T)sh.scanned[warp - 1] : 0) + x - v;
 }
 
 template <typename L, int C>
@@ -112,32 +130,44 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   using Stored = typename K::Stored;
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
+  static_assert(sizeof(Shared) % 16 == 0, "the keys behind it are read sixteen bytes at a time");
   Stored* keys = reinterpret_cast<Stored*>(raw + sizeof(Shared));
   const int tid = threadIdx.x;
   const u32 rank = blockIdx.x % C;
   const int row = (int)(blockIdx.x / C);
-  const int slice = kThreads * chunk, base = rank * slice;  // this CTA's logits: [base, base + slice), a chunk per thread
+  const int slice = kThreads * chunk, base = rank * slice;  // this CTA's logits: [base, base + slice)
   const int n = max(0, min(p.V - base, slice));
-  const Stored* mine = keys + tid * chunk;
+  u32 ranks = C;  // CTAs that take part
   int question = 0;
-  // Everybody's answer to the next question, added up (or the largest); what the CTAs in front of this one said: before.
-  auto ask = [&](u64 v, u64* before) {
-    if (tid == 0) sh.exchange[question] = v;
-    cluster_barrier();
+  auto meet = [&] {
+    if (ranks > 1)
+      cluster_barrier();
+    else
+      __syncthreads();
+  };
+  // Everybody's answer to the next question, added up; what the CTAs in front of this one said: before.
+  auto heard = [&](int at, u64* before) {
     u64 told[C], sum = 0;
 #pragma unroll
-    for (u32 r = 0; r < (u32)C; ++r) told[r] = peer_u64(&sh.exchange[question], r);
+    for (u32 r = 0; r < (u32)C; ++r) told[r] = r < ranks ? peer_u64(&sh.exchange[at], ranks > 1 ? r : rank) : 0;
     *before = 0;
 #pragma unroll
     for (u32 r = 0; r < (u32)C; ++r) {
       if (r == rank) *before = sum;
       sum += told[r];
     }
-    ++question;
     return sum;
   };
+  auto ask = [&](u64 v, u64* before) {
+    if (tid == 0) sh.exchange[question] = v;
+    meet();
+    return heard(question++, before);
+  };
 
-  // ---- the row's slice as keys, and the largest
+  // ---- 1. the row's slice as keys, and the largest
+  for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0;
+  if (tid < 256) sh.power[tid] = exp2(tid / 256.0) * kOne;
+  if (tid == 0) sh.found[0] = 0;
   const L* src = static_cast<const L*>(p.logits) + row * p.stride + base;
   u32 top = 0;
   constexpr int kVec = 16 / sizeof(L);
@@ -164,35 +194,45 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
     keys[i] = (Stored)K::stored(k);
     top = max(top, K::stored(k));
   }
+  // the row's settings are on their way while the largest key is agreed on
+  float T = p.temperature ? __ldcg(p.temperature + row) : p.temperature_all;
+  int k = p.top_k ? __ldcg(p.top_k + row) : p.top_k_all;
+  const float top_p = p.top_p ? __ldcg(p.top_p + row) : p.top_p_all;
+  const float min_p = p.min_p ? __ldcg(p.min_p + row) : p.min_p_all;
+  float u = __ldcg(p.u + row);
   top = __reduce_max_sync(0xffffffffu, top);
-  if (tid == 0) sh.found[0] = 0;
   __syncthreads();
-  if ((tid & 31) == 0) atomicMax(&sh.found[0], (u64)top);
+  if ((tid & 31) == 0 && top) atomicMax(&sh.found[0], (u64)top);
   __syncthreads();
   if (tid == 0) sh.exchange[question] = sh.found[0];
-  cluster_barrier();
+  meet();
   top = 0;
 #pragma unroll
   for (u32 r = 0; r < (u32)C; ++r) top = max(top, (u32)peer_u64(&sh.exchange[question], r));
   ++question;
   const float largest = K::logit(top);
-  if (largest == __uint_as_float(0xff800000u)) top = 0;  // nothing but minus infinity
+  if (top == 0 || largest == __uint_as_float(0xff800000u)) {  // not a number, or nothing above minus infinity
+    if (rank == 0 && tid == 0) p.tokens[row] = -1;
+    meet();
+    return;
+  }
 
-  float T = p.temperature ? __ldcg(p.temperature + row) : p.temperature_all;
-  int k = p.top_k ? __ldcg(p.top_k + row) : p.top_k_all;
-  const float top_p = p.top_p ? __ldcg(p.top_p + row) : p.top_p_all;
-  const float min_p = p.min_p ? __ldcg(p.min_p + row) : p.min_p_all;
   if (!(T > 0.f)) k = 1, T = 1.f;
+  T = fminf(T, 1e36f);  // (40 T has to be a number)
   if (k <= 0 || k > p.V) k = p.V;
-  const double per_T = 1.0 / (double)T;
-  // (a weight of e^-31.5 is under half of 2^-44; keys below this one need not be asked)
-  const u32 nothing = K::stored(key_of(largest - 40.f * T));
-  // the weight of a stored key, in multiples of 2^-44
+  // (keys below this one have no weight, and minus infinity is below it)
+  const u32 nothing = max(K::stored(key_of(largest - kReach * T)), K::stored(key_of(__uint_as_float(0xff800000u))) + 1);
+  // The weight of a stored key in multiples of 2^-44.  2^(x / 256) with x = whole + r, |r| <= 1/2: the whole part's low eight bits
+  // from a table, the others into the exponent, and (r ln2 / 256)^n / n! up to n = 4 (the next term is under 2^-54).
+  const double per_T = 256.0 * 1.4426950408889634074 / (double)T, high = (double)largest;
   auto weight = [&](u32 s) -> u64 {
-    if (s == top) return (u64)kOne;
-    if (s < nothing) return 0;
-    const double x = ((double)K::logit(s) - (double)largest) * per_T;
-    return x < -31.5 ? 0 : (u64)rint(exp(x) * kOne);  // (not finite: below, or nan, which compares false and converts to 0)
+    constexpr double a = 0.69314718055994530942 / 256.0;
+    const double x = ((double)K::logit(s) - high) * per_T, t = x + kWhole, r = x - (t - kWhole);
+    const int j = __double2loint(t);
+    const double y = fma(fma(fma(fma(a * a * a * a / 24.0, r, a * a * a / 6.0), r, a * a / 2.0), r, a), r, 1.0) * sh.power[j & 255];
+    const double scaled = __hiloint2double(__double2hiint(y) + ((j >> 8) << 20), __double2loint(y));
+    const u64 v = (u64)__double_as_longlong(scaled + 4503599627370496.0) & ((1ull << 52) - 1);  // to the nearest whole
+    return s == top ? (u64)kOne : s < nothing ? 0 : v;
   };
 
   // kept: keys above kf, and the first rf (in order of index) of those that equal it
@@ -204,90 +244,257 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
     const u32 s = K::kBits == 32 ? least : (least >> 16) + (K::logit(least >> 16) < logit_of(least) ? 1 : 0);
     if (s > 0) kf = min(s, top) - 1;
   }
+  kf = max(kf, nothing - 1);  // (a logit without weight cannot be drawn, and counts for no border)
 
-  // Radix selection, level after level, among the kept keys in falling order: the key at which the sum of `measure` reaches
-  // `target(total)`, the sum in front of it, and the sum of all its equals.  False: it is not reached.
+  const bool by_count = k < p.V, by_weight = !(top_p >= 1.f);
+  u64 all_weight = 0;       // of everything above kf, where top_p alone asks for it
+  u32 least = kf + 1;       // keys below it are not kept
+  u32 n_work = 0xffffffffu;  // elements from there on
+  // f(key, place) for every element of the slice, four or eight to a read, in no order
+  auto each = [&](auto f) {
+    const uint4* v = reinterpret_cast<const uint4*>(keys);
+    for (int i = tid; i < slice / kVec; i += kThreads) {
+      const uint4 x = v[i];
+      const u32 w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (K::kPerWord == 1) {
+          f(w[e]);
+        } else {
+          f(w[e] & 0xffffu);
+          f(w[e] >> 16);
+        }
+      }
+    }
+  };
+
+  if (by_count || by_weight) {
+    // ---- 2. distances, counted
+    const float steps = kBins / (kReach * T);
+    // falls with the key (each operation keeps the order); kBins and above: not counted
+    auto bin_of = [&](u32 s) { return s == top ? 0 : (int)fminf((largest - K::logit(s)) * steps, (float)kBins); };
+    each([&](u32 s) {
+      if (s <= kf) return;
+      const int b = bin_of(s);
+      if (b < kBins) atomicAdd(&sh.count[b], 1u);
+    });
+    meet();
+    constexpr int kPart = kBins / C;  // bins this CTA adds up, two to a thread (C = 1), or one
+    {
+      constexpr int kEach = kPart > kThreads ? kPart / kThreads : 1;
+      u32 x[kEach], mine = 0, total;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        x[e] = 0;
+        const int at = tid * kEach + e;
+        if (at < kPart) {
+          u32 y[C];
+#pragma unroll
+          for (u32 r = 0; r < (u32)C; ++r) y[r] = peer_u32(&sh.count[rank * kPart + at], r);
+#pragma unroll
+          for (u32 r = 0; r < (u32)C; ++r) x[e] += y[r];
+        }
+        mine += x[e];
+      }
+      u32 before = block_scan(mine, sh, &total);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        before += x[e];
+        if (tid * kEach + e < kPart) {
+#pragma unroll
+          for (u32 r = 0; r < (u32)C; ++r) to_peer_u32(&sh.sums[rank * kPart + tid * kEach + e], r, before);
+        }
+      }
+    }
+    meet();
+    // every CTA has all sums now: this thread's two bins, and what is up to and with them
+    u32 base_count = 0;
+    const int b0 = 2 * tid;
+#pragma unroll
+    for (int r = 0; r < C - 1; ++r)
+      if ((r + 1) * kPart <= b0) base_count += sh.sums[(r + 1) * kPart - 1];
+    const u32 upto1 = base_count + sh.sums[b0 + 1], upto0 = base_count + sh.sums[b0];
+    const u32 front0 = b0 % kPart ? base_count + sh.sums[b0 - 1] : base_count;
+    u32 counted;
+    {
+      u32 x = 0;
+#pragma unroll
+      for (int r = 0; r < C; ++r) x += sh.sums[(r + 1) * kPart - 1];
+      counted = x;
+    }
+    int last_bin = kBins - 1;
+    n_work = counted;
+    if (tid == 0) sh.found[0] = kBins - 1, sh.found[1] = counted;
+    if (by_count) {
+      __syncthreads();
+      if (front0 < (u32)k && upto0 >= (u32)k) sh.found[0] = b0, sh.found[1] = upto0;
+      if (upto0 < (u32)k && upto1 >= (u32)k) sh.found[0] = b0 + 1, sh.found[1] = upto1;
+    } else {
+      // bins' weights at their near ends, in 2^-36: the true ones are at least e^(-40/2048) of that
+      constexpr double kWidth = (double)kReach / kBins;
+      const double near0 = exp(-kWidth * b0), w0 = near0 * (upto0 - front0), w1 = near0 * exp(-kWidth) * (upto1 - upto0);
+      const u64 x0 = (u64)(w0 * 68719476736.0) + 1, x1 = (u64)(w1 * 68719476736.0) + 1;
+      u64 total;
+      const u64 before = block_scan(x0 + x1, sh, &total);
+      // the border is no further than where the least that the bins can hold reaches top_p of the most (1e-4: the steps' rounding)
+      const double goal = fmin(1.0, (double)fmaxf(top_p, 0.f) * (exp(kWidth) * 1.0001)) * (double)total;
+      if (tid == 0 && goal <= 0.0) sh.found[0] = 0, sh.found[1] = upto0;
+      if ((double)before < goal && (double)(before + x0) >= goal) sh.found[0] = b0, sh.found[1] = upto0;
+      if ((double)(before + x0) < goal && (double)(before + x0 + x1) >= goal) sh.found[0] = b0 + 1, sh.found[1] = upto1;
+    }
+    __syncthreads();
+    last_bin = (int)sh.found[0];
+    n_work = (u32)sh.found[1];
+    if (last_bin < kBins - 1) {
+      u32 lo = kf + 1, hi = top;  // the smallest key of a bin up to last_bin
+      while (lo < hi) {
+        const u32 mid = lo + (hi - lo) / 2;
+        if (bin_of(mid) <= last_bin)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      least = lo;
+    }
+    if (by_weight && !by_count) {  // the whole's weight, exactly
+      u64 mine = 0, before, total;
+      each([&](u32 s) {
+        const u64 v = weight(s);
+        mine += s > kf ? v : 0;
+      });
+      block_scan(mine, sh, &total);
+      if (n_work > kList)
+        all_weight = ask(total, &before);
+      else if (tid == 0)
+        sh.exchange[question] = total;  // (with the list's length below)
+    }
+  }
+
+  // ---- 3. what is looked at from here on: a list in one CTA, or what the CTAs hold
+  bool listed = false;
+  int width = chunk;  // elements to a thread, one behind the other
+  if (n_work <= kList) {
+    const Stored* mine = keys + tid * chunk;
+    u32 some = 0, total;
+    for (int i = 0; i < chunk; ++i) some += mine[i] >= least;
+    u32 at = block_scan(some, sh, &total);
+    if (some)
+      for (int i = 0; i < chunk; ++i)
+        if (mine[i] >= least) {
+          sh.list_key[at] = mine[i];
+          sh.list_at[at++] = base + tid * chunk + i;
+        }
+    if (tid == 0) sh.exchange[question + 1] = total;
+    meet();
+    u64 before;
+    if (by_weight && !by_count) all_weight = heard(question, &before);
+    if (rank != 0) {
+      cluster_barrier();  // (the first CTA has read its list)
+      return;
+    }
+    if constexpr (C > 1) {
+      u32 len[C], end = total;
+#pragma unroll
+      for (u32 r = 1; r < (u32)C; ++r) len[r] = (u32)peer_u64(&sh.exchange[question + 1], r);
+#pragma unroll
+      for (u32 r = 1; r < (u32)C; ++r) {
+        for (u32 i = tid; i < len[r]; i += kThreads) {
+          sh.list_key[end + i] = peer_u32(&sh.list_key[i], r);
+          sh.list_at[end + i] = peer_u32(&sh.list_at[i], r);
+        }
+        end += len[r];
+      }
+      __syncthreads();
+      cluster_arrive();  // (waited for at the end)
+      n_work = end;
+    }
+    question += 2;
+    ranks = 1;
+    listed = true;
+    width = (int)(n_work + kThreads - 1) / kThreads;
+    __syncthreads();
+  }
+  auto key_at = [&](int i) -> u32 {
+    if (!listed) return keys[tid * width + i];
+    const u32 x = tid * width + i;
+    return x < n_work ? sh.list_key[x] : 0;
+  };
+  auto place_of = [&](int i) -> int { return listed ? (int)sh.list_at[tid * width + i] : base + tid * width + i; };
+
+  // ---- 4. Radix selection, level after level, among the kept keys in falling order: the key at which the sum of `measure`
+  // reaches `target(total)`, the sum in front of it, and the sum of all its equals.  False: it is not reached.
   int level = 0;
   auto select = [&](auto measure, auto target, bool wide, u32* key, u64* front, u64* own) {
     u32 prefix = 0;
     u64 goal = 0, above = 0, held = 0;
     const u64 part = rf ? rf * measure(kf) : 0;  // the kept equals of kf are no elements of the histograms
-    int left = K::kBits;
-    for (int l = 0; left > 0; ++l) {
-      const int bits = min(left, 11), shift = left - bits;
-      u32 *lo = sh.lo[level & 1], *hi = sh.hi[level & 1];
+    for (int left = K::kBits; left > 0; left -= 8) {
+      const int shift = left - 8;
+      u32(*limb)[kDigit] = sh.limb[level & 1];
       ++level;
-      for (int i = tid; i < kBins / 4; i += kThreads) {
-        reinterpret_cast<uint4*>(lo)[i] = make_uint4(0, 0, 0, 0);
-        reinterpret_cast<uint4*>(hi)[i] = make_uint4(0, 0, 0, 0);
-      }
+      for (int i = tid; i < 3 * kDigit; i += kThreads) limb[0][i] = 0;
       __syncthreads();
-      for (int i = 0; i < chunk; ++i) {
-        const u32 s = mine[i];
-        if (s <= kf || (l > 0 && (s >> left) != prefix)) continue;
-        const u64 v = measure(s);
-        if (v == 0) continue;
-        const u32 bin = (s >> shift) & ((1u << bits) - 1), x = (u32)v;
-        const u32 old = atomicAdd(&lo[bin], x);
-        if (wide) {
-          const u32 up = (u32)(v >> 32) + (old + x < old);
-          if (up) atomicAdd(&hi[bin], up);
-        }
-      }
-      cluster_barrier();
-      // bins in falling order, four to a thread: bins top_bin - 3 .. top_bin
-      constexpr int kEach = 4;
-      static_assert(kBins == kEach * kThreads, "a thread reads its bins at once");
-      const int top_bin = (1 << bits) - 1 - tid * kEach;
-      u64 sum[kEach] = {}, mass = 0;
-      if (top_bin > 0) {
-        uint4 a[C], c[C];
+      for (int i = 0; i < width; i += kAtOnce) {
+        u32 at[kAtOnce];
+        bool some = false;
 #pragma unroll
-        for (u32 r = 0; r < (u32)C; ++r) {
-          a[r] = peer_u4(&lo[top_bin - 3], r);
-          c[r] = wide ? peer_u4(&hi[top_bin - 3], r) : make_uint4(0, 0, 0, 0);
+        for (int e = 0; e < kAtOnce; ++e) {
+          at[e] = i + e < width ? key_at(i + e) : 0;
+          if (at[e] <= kf || at[e] < least || (left < K::kBits && (at[e] >> left) != prefix)) at[e] = 0;
+          some |= at[e] != 0;
         }
+        if (!__any_sync(0xffffffffu, some)) continue;
+        u64 v[kAtOnce];
 #pragma unroll
-        for (u32 r = 0; r < (u32)C; ++r) {
-          sum[0] += a[r].w + ((u64)c[r].w << 32);
-          sum[1] += a[r].z + ((u64)c[r].z << 32);
-          sum[2] += a[r].y + ((u64)c[r].y << 32);
-          sum[3] += a[r].x + ((u64)c[r].x << 32);
-        }
-        if (rf) {
-          const u32 first = (l > 0 ? prefix << bits : 0) | (u32)top_bin, at = first - (kf >> shift);
-          if (at < kEach) {
+        for (int e = 0; e < kAtOnce; ++e) v[e] = measure(at[e]);
 #pragma unroll
-            for (int e = 0; e < kEach; ++e)
-              if (at == (u32)e) sum[e] += part;
+        for (int e = 0; e < kAtOnce; ++e) {
+          if (at[e] == 0) continue;
+          const u32 bin = (at[e] >> shift) & (kDigit - 1);
+          if (!wide) {
+            atomicAdd(&limb[0][bin], (u32)v[e]);
+          } else {
+            constexpr u32 kMask = (1u << kLimb) - 1;
+            const u32 low = (u32)v[e] & kMask, mid = (u32)(v[e] >> kLimb) & kMask, up = (u32)(v[e] >> (2 * kLimb));
+            atomicAdd(&limb[0][bin], low);
+            if (mid) atomicAdd(&limb[1][bin], mid);
+            if (up) atomicAdd(&limb[2][bin], up);
           }
         }
+      }
+      meet();
+      // bins in falling order, one to a thread
+      const int bin = kDigit - 1 - tid;
+      u64 sum = 0;
+      if (bin >= 0) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) mass += sum[e];
+        for (int w = 0; w < 3; ++w) {
+          if (w > 0 && !wide) break;
+          u32 a[C];
+#pragma unroll
+          for (u32 r = 0; r < (u32)C; ++r) a[r] = r < ranks ? peer_u32(&limb[w][bin], ranks > 1 ? r : rank) : 0;
+#pragma unroll
+          for (u32 r = 0; r < (u32)C; ++r) sum += (u64)a[r] << (kLimb * w);
+        }
+        const u32 here = (left < K::kBits ? prefix << 8 : 0) | (u32)bin;
+        if (rf && (kf >> shift) == here) sum += part;
       }
       u64 total;
-      u64 before = block_scan(mass, sh.scan, &total);
-      if (l == 0) {
+      const u64 before = block_scan(sum, sh, &total);
+      if (left == K::kBits) {
         goal = target(total);
         if (total < goal || goal == 0) return false;  // (the same in every CTA)
       }
       const u64 want = goal - above;  // at least 1, and reached in this level
-      if (before < want && before + mass >= want) {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          if (before < want && before + sum[e] >= want) {
-            sh.found[0] = top_bin - e;
-            sh.found[1] = before;
-            sh.found[2] = sum[e];
-          }
-          before += sum[e];
-        }
+      if (before < want && before + sum >= want) {
+        sh.found[0] = bin;
+        sh.found[1] = before;
+        sh.found[2] = sum;
       }
       __syncthreads();
-      prefix = l > 0 ? (prefix << bits) | (u32)sh.found[0] : (u32)sh.found[0];
+      prefix = (left < K::kBits ? prefix << 8 : 0) | (u32)sh.found[0];
       above += sh.found[1];
       held = sh.found[2];
-      left = shift;
       __syncthreads();
     }
     *key = prefix;
@@ -298,7 +505,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
 
   u32 key;
   u64 front, own;
-  if (top != 0 && k < p.V) {
+  if (by_count) {
     // (goal k: the k-th key in falling order)
     if (select([](u32) -> u64 { return 1; }, [&](u64 total) { return total < (u64)k ? 0 : (u64)k; }, false, &key, &front, &own)) {
       kf = key;
@@ -306,9 +513,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       equal = (u32)own;
     }
   }
-  if (top != 0 && !(top_p >= 1.f)) {
+  if (by_weight) {
     u64 reach = 0;
     auto goal = [&](u64 total) {
+      if (!by_count) total = all_weight;
       const double g = ceil((double)(top_p > 0.f ? top_p : 0.f) * (double)total);
       return reach = g < 1.0 ? 1 : (u64)g > total ? total : (u64)g;
     };
@@ -320,56 +528,68 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       rf = some;
     }
   }
-  // fewer than all of the border's equals: those up to an index
+  // fewer than all of the border's equals: those up to a place
   int last = 0x7fffffff;
   if (rf != 0 && rf < equal) {
-    u64 mine_n = 0, total, before;
-    for (int i = 0; i < chunk; ++i) mine_n += mine[i] == kf;
-    const u64 at = block_scan(mine_n, sh.scan, &total);
+    u32 mine = 0, total;
+    for (int i = 0; i < width; ++i) mine += key_at(i) == kf;
+    const u32 at = block_scan(mine, sh, &total);
+    u64 before;
     ask(total, &before);
     if (tid == 0) sh.exchange[question] = 0;
     __syncthreads();
-    if (before + at < rf && before + at + mine_n >= rf) {
-      u64 need = rf - before - at;
-      for (int i = 0; i < chunk; ++i)
-        if (mine[i] == kf && --need == 0) sh.exchange[question] = (u64)(base + tid * chunk + i) + 1;
+    if (before + at < rf && before + at + mine >= rf) {
+      u32 need = rf - (u32)before - at;
+      for (int i = 0; i < width; ++i)
+        if (key_at(i) == kf && --need == 0) sh.exchange[question] = (u64)place_of(i) + 1;
     }
-    cluster_barrier();
-    for (u32 r = 0; r < (u32)C; ++r) {
-      const u64 e = peer_u64(&sh.exchange[question], r);
-      if (e) last = (int)e - 1;
-    }
-    ++question;
+    meet();
+    u64 unused;
+    last = (int)heard(question++, &unused) - 1;  // (one CTA's answer, and zeros)
   }
   // ---- the draw, in the order of the vocabulary
-  const int first = base + tid * chunk;
-  auto kept = [&](int i, u32 s) { return s > kf || (s == kf && rf != 0 && first + i <= last); };
+  auto kept = [&](int i, u32 s) { return s > kf || (s == kf && rf != 0 && place_of(i) <= last); };
   u64 mass = 0, total, before;
-  for (int i = 0; i < chunk; ++i) {
-    const u32 s = mine[i];
-    if (kept(i, s)) mass += weight(s);
+  for (int i = 0; i < width; i += kAtOnce) {
+    u32 at[kAtOnce];
+    bool some = false;
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) {
+      at[e] = i + e < width ? key_at(i + e) : 0;
+      if (at[e] == 0 || !kept(i + e, at[e])) at[e] = 0;
+      some |= at[e] != 0;
+    }
+    if (!__any_sync(0xffffffffu, some)) continue;
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) {
+      const u64 v = weight(at[e]);
+      mass += at[e] != 0 ? v : 0;
+    }
   }
-  u64 at = block_scan(mass, sh.scan, &total);
+  u64 at = block_scan(mass, sh, &total);
   const u64 sum = ask(total, &before);
   at += before;
-  float u = __ldcg(p.u + row);
   u = u > 0.f ? u : 0.f;
   u64 goal = (u64)((double)u * (double)sum);
   if (goal >= sum) goal = sum - 1;
-  if (sum == 0) {
-    if (rank == 0 && tid == 0) p.tokens[row] = -1;  // nothing to draw from
-  } else if (at <= goal && at + mass > goal) {
-    for (int i = 0; i < chunk; ++i) {
-      const u32 s = mine[i];
-      if (!kept(i, s)) continue;
+  if (at <= goal && at + mass > goal) {
+    for (int i = 0; i < width; ++i) {
+      const u32 s = key_at(i);
+      if (s == 0 || !kept(i, s)) continue;
       at += weight(s);
       if (at > goal) {
-        p.tokens[row] = first + i;
+        p.tokens[row] = place_of(i);
         break;
       }
     }
   }
-  cluster_barrier();  // nobody leaves while another may read its memory
+  if constexpr (C > 1) {  // nobody leaves while another may read its memory
+    __syncwarp();
+    if (listed)
+      cluster_wait();
+    else
+      cluster_barrier();
+  }
 }
 
 // Elements to a thread: an odd number of 32-bit words, so that the threads' chunks start in different banks.
@@ -404,7 +624,7 @@ template <typename L>
 int launch(const Sampling& p, cudaStream_t s) {
   const size_t row = (size_t)p.V * sizeof(typename Keys<L>::Stored);
   int C = 1;
-  while (C < 8 && (p.rows * C < 148 || row / C > kSliceBytes)) C *= 2;
+  while (C < 8 && ((p.rows * C < 148 && p.V / C > 4096) || row / C > kSliceBytes)) C *= 2;
   switch (C) {
     case 1: return launch_on<L, 1>(p, s);
     case 2: return launch_on<L, 2>(p, s);
