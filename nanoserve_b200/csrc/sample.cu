@@ -14,10 +14,10 @@
 //      counts alone, one atomic an element.  Every CTA adds up a C-th of the bins over the cluster and sends the sums to all.
 //   2. counts bound both borders: exactly the bin of the top_k-th logit, and, since weights within a bin are e^(-40/2048) or
 //      nearer to one another, bins between which the top_p border lies.
-//   3. what is in front of the borders' far end is all that the rest looks at.  Up to 4096 logits are gathered, in the order
-//      of the vocabulary, in one CTA, which goes on alone; more stay where they are, and each step ends in a cluster barrier.
-//   4. the exact borders by radix selection on the keys (eight bits at a time), with counts and exact weights; the draw by
-//      prefix sums.
+//   3. where no more than 1024 logits are in front of the borders' far end, they are gathered in one CTA, which goes on alone:
+//      it sorts them, and prefix sums give both borders and the draw.
+//   4. else the logits stay where they are.  The exact borders are found by radix selection (eight bits at a time) among the
+//      few keys of the bins that the borders lie in, and the draw by prefix sums over all CTAs.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -30,8 +30,8 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kBins = 2048;      // of the first histogram, of distances
 constexpr int kDigit = 256;      // of the selections on keys
-constexpr int kAtOnce = 4;       // elements of a thread whose weights are formed side by side
-constexpr int kList = 4096;      // logits that one CTA looks at alone
+constexpr int kPowers = 1024;    // of the table of 2^(j / kPowers)
+constexpr int kList = kThreads;  // logits that one CTA looks at alone, one to a thread
 constexpr float kReach = 40.f;   // distances beyond it, in T, have a weight under 2^-57: none
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kSliceBytes = 150 * 1024;
@@ -75,13 +75,14 @@ struct Keys<__nv_bfloat16> {
 
 constexpr int kLimb = 15;  // a bin's weight in three sums of fifteen bits each: up to 2^17 elements leave them in 32 bits
 struct alignas(16) Shared {
-  u32 count[kBins];                // this CTA's, then (sums) the cluster's up to each bin, within the part of it one CTA adds up
-  u32 sums[kBins];
+  // this CTA's, then (sums) the cluster's up to each bin, within the part of it one CTA adds up
+  alignas(8) u32 count[kBins];
+  alignas(8) u32 sums[kBins];
   u32 limb[2][3][kDigit];          // a selection's bins (counts: the first alone), two in turn: peers may still read the other
-  double power[256];               // 2^44 2^(j / 256)
+  double power[kPowers];           // 2^44 2^(j / kPowers)
   u64 exchange[12];                // what this CTA tells the others, a place per question
   u64 scan[32], scanned[32];
-  u64 found[3];
+  u64 found[6];
   u32 list_key[kList], list_at[kList];  // keys and their places in the vocabulary
 };
 
@@ -137,10 +138,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   const int row = (int)(blockIdx.x / C);
   const int slice = kThreads * chunk, base = rank * slice;  // this CTA's logits: [base, base + slice)
   const int n = max(0, min(p.V - base, slice));
-  u32 ranks = C;  // CTAs that take part
   int question = 0;
   auto meet = [&] {
-    if (ranks > 1)
+    if constexpr (C > 1)
       cluster_barrier();
     else
       __syncthreads();
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   auto heard = [&](int at, u64* before) {
     u64 told[C], sum = 0;
 #pragma unroll
-    for (u32 r = 0; r < (u32)C; ++r) told[r] = r < ranks ? peer_u64(&sh.exchange[at], ranks > 1 ? r : rank) : 0;
+    for (u32 r = 0; r < (u32)C; ++r) told[r] = peer_u64(&sh.exchange[at], r);
     *before = 0;
 #pragma unroll
     for (u32 r = 0; r < (u32)C; ++r) {
@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
 
   // ---- 1. the row's slice as keys, and the largest
   for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0;
-  if (tid < 256) sh.power[tid] = exp2(tid / 256.0) * kOne;
+  static_assert(kPowers == kThreads, "a thread per entry");
+  sh.power[tid] = exp2(tid / (double)kPowers) * kOne;
   if (tid == 0) sh.found[0] = 0;
   const L* src = static_cast<const L*>(p.logits) + row * p.stride + base;
   u32 top = 0;
@@ -222,17 +223,21 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   if (k <= 0 || k > p.V) k = p.V;
   // (keys below this one have no weight, and minus infinity is below it)
   const u32 nothing = max(K::stored(key_of(largest - kReach * T)), K::stored(key_of(__uint_as_float(0xff800000u))) + 1);
-  // The weight of a stored key in multiples of 2^-44.  2^(x / 256) with x = whole + r, |r| <= 1/2: the whole part's low eight bits
-  // from a table, the others into the exponent, and (r ln2 / 256)^n / n! up to n = 4 (the next term is under 2^-54).
-  const double per_T = 256.0 * 1.4426950408889634074 / (double)T, high = (double)largest;
+  // The weight of a stored key in multiples of 2^-44.  2^(x / 1024) with x = whole + r, |r| <= 1/2: the whole part's low ten bits
+  // from a table, the others into its exponent, and (r ln2 / 1024)^n / n! up to n = 3 (the next term is under 2^-50).  The last
+  // product is added to 2^52, which rounds it to a whole number.
+  const double per_T = kPowers * 1.4426950408889634074 / (double)T, offset = -(double)largest * per_T;
   auto weight = [&](u32 s) -> u64 {
-    constexpr double a = 0.69314718055994530942 / 256.0;
-    const double x = ((double)K::logit(s) - high) * per_T, t = x + kWhole, r = x - (t - kWhole);
+    constexpr double a = 0.69314718055994530942 / kPowers;
+    // fp32 to fp64 by its bits (a conversion takes as long as four products; numbers under 2^-126 become another such one)
+    const u32 bits = __float_as_uint(K::logit(s));
+    const double l = __hiloint2double((bits & 0x80000000u) | (((bits & 0x7fffffffu) >> 3) + (896u << 20)), bits << 29);
+    const double x = fma(l, per_T, offset), t = x + kWhole, r = x - (t - kWhole);
     const int j = __double2loint(t);
-    const double y = fma(fma(fma(fma(a * a * a * a / 24.0, r, a * a * a / 6.0), r, a * a / 2.0), r, a), r, 1.0) * sh.power[j & 255];
-    const double scaled = __hiloint2double(__double2hiint(y) + ((j >> 8) << 20), __double2loint(y));
-    const u64 v = (u64)__double_as_longlong(scaled + 4503599627370496.0) & ((1ull << 52) - 1);  // to the nearest whole
-    return s == top ? (u64)kOne : s < nothing ? 0 : v;
+    const double power = sh.power[j & (kPowers - 1)];
+    const double scaled = __hiloint2double(__double2hiint(power) + ((j >> 10) << 20), __double2loint(power));
+    const double v = fma(fma(fma(fma(a * a * a / 6.0, r, a * a / 2.0), r, a), r, 1.0), scaled, 4503599627370496.0);
+    return s == top ? (u64)kOne : s < nothing ? 0 : (u64)__double_as_longlong(v) & ((1ull << 52) - 1);
   };
 
   // kept: keys above kf, and the first rf (in order of index) of those that equal it
@@ -247,10 +252,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   kf = max(kf, nothing - 1);  // (a logit without weight cannot be drawn, and counts for no border)
 
   const bool by_count = k < p.V, by_weight = !(top_p >= 1.f);
-  u64 all_weight = 0;       // of everything above kf, where top_p alone asks for it
-  u32 least = kf + 1;       // keys below it are not kept
-  u32 n_work = 0xffffffffu;  // elements from there on
-  // f(key, place) for every element of the slice, four or eight to a read, in no order
+  // f(key) for every element of the slice, sixteen bytes to a read, in no order
   auto each = [&](auto f) {
     const uint4* v = reinterpret_cast<const uint4*>(keys);
     for (int i = tid; i < slice / kVec; i += kThreads) {
@@ -267,12 +269,39 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       }
     }
   };
+  // f(four keys, place of the first in the slice) for this thread's elements, one behind the other
+  const int words = chunk / K::kPerWord;
+  auto in_order = [&](auto f) {
+    const u32* mine = reinterpret_cast<const u32*>(keys) + tid * words;
+    constexpr int kWords = 4 / K::kPerWord;
+    for (int i = 0; i < words; i += kWords) {
+      u32 s[4];
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) {
+        const u32 w = i + e < words ? mine[i + e] : 0;
+        if constexpr (K::kPerWord == 1)
+          s[e] = w;
+        else
+          s[2 * e] = w & 0xffffu, s[2 * e + 1] = w >> 16;
+      }
+      f(s, tid * chunk + i * K::kPerWord);
+    }
+  };
+  // top_p of a weight, rounded up to a whole number, at least the first
+  auto share = [&](u64 total) -> u64 {
+    const double g = ceil((double)(top_p > 0.f ? top_p : 0.f) * (double)total);
+    return g < 1.0 ? 1 : (u64)g > total ? total : (u64)g;
+  };
+
+  const float steps = kBins / (kReach * T);
+  // falls with the key (each operation keeps the order); kBins and above: not counted
+  auto bin_of = [&](u32 s) { return s == top ? 0 : (int)fminf((largest - K::logit(s)) * steps, (float)kBins); };
+  bool cut = false;  // top_k leaves some out:
+  int bin_k = kBins - 1, bin_lo = 0, bin_hi = kBins - 1;  // the bin of the top_k-th, and those that hold the top_p border
+  u32 front_k = 0;   // logits in front of bin_k
 
   if (by_count || by_weight) {
     // ---- 2. distances, counted
-    const float steps = kBins / (kReach * T);
-    // falls with the key (each operation keeps the order); kBins and above: not counted
-    auto bin_of = [&](u32 s) { return s == top ? 0 : (int)fminf((largest - K::logit(s)) * steps, (float)kBins); };
     each([&](u32 s) {
       if (s <= kf) return;
       const int b = bin_of(s);
@@ -307,161 +336,186 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       }
     }
     meet();
-    // every CTA has all sums now: this thread's two bins, and what is up to and with them
-    u32 base_count = 0;
+    // every CTA has all sums now: this thread's two bins, and the logits up to each of them and in front
     const int b0 = 2 * tid;
+    u32 base_count = 0, counted = 0;
 #pragma unroll
-    for (int r = 0; r < C - 1; ++r)
-      if ((r + 1) * kPart <= b0) base_count += sh.sums[(r + 1) * kPart - 1];
-    const u32 upto1 = base_count + sh.sums[b0 + 1], upto0 = base_count + sh.sums[b0];
-    const u32 front0 = b0 % kPart ? base_count + sh.sums[b0 - 1] : base_count;
-    u32 counted;
-    {
-      u32 x = 0;
-#pragma unroll
-      for (int r = 0; r < C; ++r) x += sh.sums[(r + 1) * kPart - 1];
-      counted = x;
+    for (int r = 0; r < C; ++r) {
+      const u32 x = sh.sums[(r + 1) * kPart - 1];
+      if ((r + 1) * kPart <= b0) base_count += x;
+      counted += x;
     }
-    int last_bin = kBins - 1;
-    n_work = counted;
-    if (tid == 0) sh.found[0] = kBins - 1, sh.found[1] = counted;
-    if (by_count) {
-      __syncthreads();
-      if (front0 < (u32)k && upto0 >= (u32)k) sh.found[0] = b0, sh.found[1] = upto0;
-      if (upto0 < (u32)k && upto1 >= (u32)k) sh.found[0] = b0 + 1, sh.found[1] = upto1;
-    } else {
+    const u32 upto[2] = {base_count + sh.sums[b0], base_count + sh.sums[b0 + 1]};
+    const u32 front[2] = {b0 % kPart ? base_count + sh.sums[b0 - 1] : base_count, upto[0]};
+    cut = by_count && counted > (u32)k;
+    const u32 left = cut ? (u32)k : counted;
+    if (tid == 0) {
+      sh.found[0] = kBins - 1, sh.found[1] = 0, sh.found[2] = counted;
+      sh.found[3] = 0, sh.found[4] = kBins - 1, sh.found[5] = counted;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (cut && front[e] < left && upto[e] >= left) sh.found[0] = b0 + e, sh.found[1] = front[e], sh.found[2] = upto[e];
+    if (by_weight) {
       // bins' weights at their near ends, in 2^-36: the true ones are at least e^(-40/2048) of that
       constexpr double kWidth = (double)kReach / kBins;
-      const double near0 = exp(-kWidth * b0), w0 = near0 * (upto0 - front0), w1 = near0 * exp(-kWidth) * (upto1 - upto0);
-      const u64 x0 = (u64)(w0 * 68719476736.0) + 1, x1 = (u64)(w1 * 68719476736.0) + 1;
+      const double near0 = exp(-kWidth * b0) * 68719476736.0;
+      u64 x[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        x[e] = (u64)(near0 * (e ? exp(-kWidth) : 1.0) * (min(upto[e], left) - min(front[e], left))) + 1;
       u64 total;
-      const u64 before = block_scan(x0 + x1, sh, &total);
-      // the border is no further than where the least that the bins can hold reaches top_p of the most (1e-4: the steps' rounding)
-      const double goal = fmin(1.0, (double)fmaxf(top_p, 0.f) * (exp(kWidth) * 1.0001)) * (double)total;
-      if (tid == 0 && goal <= 0.0) sh.found[0] = 0, sh.found[1] = upto0;
-      if ((double)before < goal && (double)(before + x0) >= goal) sh.found[0] = b0, sh.found[1] = upto0;
-      if ((double)(before + x0) < goal && (double)(before + x0 + x1) >= goal) sh.found[0] = b0 + 1, sh.found[1] = upto1;
+      u64 before = block_scan(x[0] + x[1], sh, &total);
+      // the border is where the most that the bins can hold reaches top_p of the least, or further, and where the least reaches
+      // top_p of the most, or nearer (1e-4: the steps' rounding)
+      const double of_all = (double)fmaxf(top_p, 0.f) * (double)total;
+      const double lo = of_all * exp(-kWidth) * 0.9999, hi = fmin((double)total, of_all * exp(kWidth) * 1.0001);
+      if (tid == 0 && hi <= 0.0) sh.found[4] = 0, sh.found[5] = upto[0];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const double with = (double)(before + x[e]);
+        if ((double)before < lo && with >= lo) sh.found[3] = b0 + e;
+        if ((double)before < hi && with >= hi) sh.found[4] = b0 + e, sh.found[5] = upto[e];
+        before += x[e];
+      }
     }
     __syncthreads();
-    last_bin = (int)sh.found[0];
-    n_work = (u32)sh.found[1];
-    if (last_bin < kBins - 1) {
-      u32 lo = kf + 1, hi = top;  // the smallest key of a bin up to last_bin
-      while (lo < hi) {
-        const u32 mid = lo + (hi - lo) / 2;
-        if (bin_of(mid) <= last_bin)
-          hi = mid;
-        else
-          lo = mid + 1;
-      }
-      least = lo;
-    }
-    if (by_weight && !by_count) {  // the whole's weight, exactly
-      u64 mine = 0, before, total;
-      each([&](u32 s) {
-        const u64 v = weight(s);
-        mine += s > kf ? v : 0;
-      });
-      block_scan(mine, sh, &total);
-      if (n_work > kList)
-        all_weight = ask(total, &before);
-      else if (tid == 0)
-        sh.exchange[question] = total;  // (with the list's length below)
-    }
-  }
+    bin_k = (int)sh.found[0];
+    front_k = (u32)sh.found[1];
+    bin_lo = (int)sh.found[3];
+    bin_hi = (int)sh.found[4];
+    const u32 n_work = (u32)sh.found[by_count ? 2 : 5];
+    const int last_bin = by_count ? bin_k : bin_hi;
 
-  // ---- 3. what is looked at from here on: a list in one CTA, or what the CTAs hold
-  bool listed = false;
-  int width = chunk;  // elements to a thread, one behind the other
-  if (n_work <= kList) {
-    const Stored* mine = keys + tid * chunk;
-    u32 some = 0, total;
-    for (int i = 0; i < chunk; ++i) some += mine[i] >= least;
-    u32 at = block_scan(some, sh, &total);
-    if (some)
-      for (int i = 0; i < chunk; ++i)
-        if (mine[i] >= least) {
-          sh.list_key[at] = mine[i];
-          sh.list_at[at++] = base + tid * chunk + i;
+    if (n_work <= kList) {
+      // ---- 3. the logits up to last_bin, gathered in the first CTA in the order of the vocabulary, and finished there
+      if (by_weight && !by_count) {  // the whole's weight, exactly
+        u64 mine = 0, total;
+        each([&](u32 s) {
+          const u64 v = weight(s);
+          mine += s > kf ? v : 0;
+        });
+        block_scan(mine, sh, &total);
+        if (tid == 0) sh.exchange[question] = total;
+      }
+      u32 some = 0, mine_n;
+      in_order([&](const u32(&s)[4], int) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) some += s[e] > kf && bin_of(s[e]) <= last_bin;
+      });
+      u32 at = block_scan(some, sh, &mine_n);
+      if (some)
+        in_order([&](const u32(&s)[4], int place) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (s[e] > kf && bin_of(s[e]) <= last_bin) {
+              sh.list_key[at] = s[e];
+              sh.list_at[at++] = base + place + e;
+            }
+        });
+      if (tid == 0) sh.exchange[question + 1] = mine_n;
+      meet();
+      if (rank != 0) {
+        meet();  // (the first CTA has read this one's list)
+        return;
+      }
+      u64 unused;
+      const u64 all_weight = by_weight && !by_count ? heard(question, &unused) : 0;
+      int n_list = (int)mine_n;
+      if constexpr (C > 1) {
+        u32 end[C];
+#pragma unroll
+        for (u32 r = 0; r < (u32)C; ++r) end[r] = (u32)peer_u64(&sh.exchange[question + 1], r);
+#pragma unroll
+        for (u32 r = 1; r < (u32)C; ++r) end[r] += end[r - 1];
+        n_list = (int)end[C - 1];
+        if (tid >= (int)mine_n && tid < n_list) {
+          u32 from = 0, first = 0;
+#pragma unroll
+          for (u32 r = 0; r < (u32)C - 1; ++r)
+            if (tid >= (int)end[r]) from = r + 1, first = end[r];
+          const u32 a = peer_u32(&sh.list_key[tid - first], from), b = peer_u32(&sh.list_at[tid - first], from);
+          sh.list_key[tid] = a;
+          sh.list_at[tid] = b;
         }
-    if (tid == 0) sh.exchange[question + 1] = total;
-    meet();
-    u64 before;
-    if (by_weight && !by_count) all_weight = heard(question, &before);
-    if (rank != 0) {
-      cluster_barrier();  // (the first CTA has read its list)
+        meet();
+      } else {
+        __syncthreads();
+      }
+      // sorted: falling keys, equal ones by rising place
+      u64* other = reinterpret_cast<u64*>(sh.count);  // [kThreads]
+      u64 x = tid < n_list ? (u64)sh.list_key[tid] << 32 | (0xffffffffu - tid) : 0;
+      for (int size = 2; size < 2 * n_list; size *= 2)
+        for (int dist = size / 2; dist > 0; dist /= 2) {
+          u64 y;
+          if (dist < 32) {
+            y = __shfl_xor_sync(0xffffffffu, x, dist);
+          } else {
+            other[tid] = x;
+            __syncthreads();
+            y = other[tid ^ dist];
+            __syncthreads();
+          }
+          x = (((tid & size) == 0) == ((tid & dist) == 0)) == (x > y) ? x : y;
+        }
+      const int n_kept = by_count ? min(n_list, k) : n_list;
+      u64 w = tid < n_kept ? weight((u32)(x >> 32)) : 0, total;
+      const u64 before = block_scan(w, sh, &total);
+      if (by_weight && before >= share(by_count ? total : all_weight)) w = 0;
+      u64* of_place = reinterpret_cast<u64*>(sh.sums);  // [kThreads]
+      if (tid < n_list) of_place[0xffffffffu - (u32)x] = w;
+      __syncthreads();
+      w = tid < n_list ? of_place[tid] : 0;
+      const u64 from = block_scan(w, sh, &total);
+      u = u > 0.f ? u : 0.f;
+      u64 goal = (u64)((double)u * (double)total);
+      if (goal >= total) goal = total - 1;
+      if (from <= goal && from + w > goal) p.tokens[row] = (int)sh.list_at[tid];
       return;
     }
-    if constexpr (C > 1) {
-      u32 len[C], end = total;
-#pragma unroll
-      for (u32 r = 1; r < (u32)C; ++r) len[r] = (u32)peer_u64(&sh.exchange[question + 1], r);
-#pragma unroll
-      for (u32 r = 1; r < (u32)C; ++r) {
-        for (u32 i = tid; i < len[r]; i += kThreads) {
-          sh.list_key[end + i] = peer_u32(&sh.list_key[i], r);
-          sh.list_at[end + i] = peer_u32(&sh.list_at[i], r);
-        }
-        end += len[r];
-      }
-      __syncthreads();
-      cluster_arrive();  // (waited for at the end)
-      n_work = end;
-    }
-    question += 2;
-    ranks = 1;
-    listed = true;
-    width = (int)(n_work + kThreads - 1) / kThreads;
-    __syncthreads();
   }
-  auto key_at = [&](int i) -> u32 {
-    if (!listed) return keys[tid * width + i];
-    const u32 x = tid * width + i;
-    return x < n_work ? sh.list_key[x] : 0;
-  };
-  auto place_of = [&](int i) -> int { return listed ? (int)sh.list_at[tid * width + i] : base + tid * width + i; };
 
-  // ---- 4. Radix selection, level after level, among the kept keys in falling order: the key at which the sum of `measure`
-  // reaches `target(total)`, the sum in front of it, and the sum of all its equals.  False: it is not reached.
+  // ---- 4. more logits than that: they stay where they are
+  // The smallest key of a bin up to b: a point to a lane.
+  auto first_key = [&](int b) {
+    u32 lo = 1, hi = top;
+    while (lo < hi) {
+      const u32 step = (hi - lo + 30) / 31, at = lo + min((u32)(tid & 31) * step, hi - lo);
+      const int f = __ffs(__ballot_sync(0xffffffffu, bin_of(at) <= b)) - 1;
+      hi = lo + min((u32)f * step, hi - lo);
+      if (f > 0) lo += (f - 1) * step + 1;
+    }
+    return lo;
+  };
+  // Radix selection, level after level, among the keys from `least` to below `sure` (above kf) in falling order: the key at which the
+  // sum of `measure` reaches `goal` (1 or more), the sum in front of it, and the sum of all its equals.  False: it is not reached.
   int level = 0;
-  auto select = [&](auto measure, auto target, bool wide, u32* key, u64* front, u64* own) {
+  auto select = [&](auto measure, u32 least, u32 sure, u64 goal, bool wide, u32* key, u64* front, u64* own) {
     u32 prefix = 0;
-    u64 goal = 0, above = 0, held = 0;
+    u64 above = 0, held = 0;
     const u64 part = rf ? rf * measure(kf) : 0;  // the kept equals of kf are no elements of the histograms
+    least = max(least, kf + 1);
     for (int left = K::kBits; left > 0; left -= 8) {
       const int shift = left - 8;
       u32(*limb)[kDigit] = sh.limb[level & 1];
       ++level;
       for (int i = tid; i < 3 * kDigit; i += kThreads) limb[0][i] = 0;
       __syncthreads();
-      for (int i = 0; i < width; i += kAtOnce) {
-        u32 at[kAtOnce];
-        bool some = false;
-#pragma unroll
-        for (int e = 0; e < kAtOnce; ++e) {
-          at[e] = i + e < width ? key_at(i + e) : 0;
-          if (at[e] <= kf || at[e] < least || (left < K::kBits && (at[e] >> left) != prefix)) at[e] = 0;
-          some |= at[e] != 0;
+      each([&](u32 s) {
+        if (s < least || s >= sure || (left < K::kBits && (s >> left) != prefix)) return;
+        const u64 v = measure(s);
+        const u32 bin = (s >> shift) & (kDigit - 1);
+        if (!wide) {
+          atomicAdd(&limb[0][bin], (u32)v);
+        } else {
+          constexpr u32 kMask = (1u << kLimb) - 1;
+          const u32 low = (u32)v & kMask, mid = (u32)(v >> kLimb) & kMask, up = (u32)(v >> (2 * kLimb));
+          atomicAdd(&limb[0][bin], low);
+          if (mid) atomicAdd(&limb[1][bin], mid);
+          if (up) atomicAdd(&limb[2][bin], up);
         }
-        if (!__any_sync(0xffffffffu, some)) continue;
-        u64 v[kAtOnce];
-#pragma unroll
-        for (int e = 0; e < kAtOnce; ++e) v[e] = measure(at[e]);
-#pragma unroll
-        for (int e = 0; e < kAtOnce; ++e) {
-          if (at[e] == 0) continue;
-          const u32 bin = (at[e] >> shift) & (kDigit - 1);
-          if (!wide) {
-            atomicAdd(&limb[0][bin], (u32)v[e]);
-          } else {
-            constexpr u32 kMask = (1u << kLimb) - 1;
-            const u32 low = (u32)v[e] & kMask, mid = (u32)(v[e] >> kLimb) & kMask, up = (u32)(v[e] >> (2 * kLimb));
-            atomicAdd(&limb[0][bin], low);
-            if (mid) atomicAdd(&limb[1][bin], mid);
-            if (up) atomicAdd(&limb[2][bin], up);
-          }
-        }
-      }
+      });
       meet();
       // bins in falling order, one to a thread
       const int bin = kDigit - 1 - tid;
@@ -472,7 +526,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
           if (w > 0 && !wide) break;
           u32 a[C];
 #pragma unroll
-          for (u32 r = 0; r < (u32)C; ++r) a[r] = r < ranks ? peer_u32(&limb[w][bin], ranks > 1 ? r : rank) : 0;
+          for (u32 r = 0; r < (u32)C; ++r) a[r] = peer_u32(&limb[w][bin], r);
 #pragma unroll
           for (u32 r = 0; r < (u32)C; ++r) sum += (u64)a[r] << (kLimb * w);
         }
@@ -481,10 +535,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       }
       u64 total;
       const u64 before = block_scan(sum, sh, &total);
-      if (left == K::kBits) {
-        goal = target(total);
-        if (total < goal || goal == 0) return false;  // (the same in every CTA)
-      }
+      if (left == K::kBits && total < goal) return false;  // (the same in every CTA)
       const u64 want = goal - above;  // at least 1, and reached in this level
       if (before < want && before + sum >= want) {
         sh.found[0] = bin;
@@ -505,24 +556,33 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
 
   u32 key;
   u64 front, own;
-  if (by_count) {
-    // (goal k: the k-th key in falling order)
-    if (select([](u32) -> u64 { return 1; }, [&](u64 total) { return total < (u64)k ? 0 : (u64)k; }, false, &key, &front, &own)) {
+  if (cut) {
+    const u64 goal = k - front_k;
+    if (select([](u32) -> u64 { return 1; }, first_key(bin_k), bin_k > 0 ? first_key(bin_k - 1) : top + 1, goal, false, &key,
+               &front, &own)) {
       kf = key;
-      rf = (u32)(k - front);
+      rf = (u32)(goal - front);
       equal = (u32)own;
     }
   }
   if (by_weight) {
-    u64 reach = 0;
-    auto goal = [&](u64 total) {
-      if (!by_count) total = all_weight;
-      const double g = ceil((double)(top_p > 0.f ? top_p : 0.f) * (double)total);
-      return reach = g < 1.0 ? 1 : (u64)g > total ? total : (u64)g;
-    };
-    if (select(weight, goal, true, &key, &front, &own)) {
+    // the weight of all that is left, and of what is surely in front of the border
+    const u32 least = first_key(bin_hi), sure = bin_lo > 0 ? first_key(bin_lo - 1) : top + 1;
+    u64 mine = 0, mine_sure = 0, total, total_sure, unused;
+    each([&](u32 s) {
+      const u64 v = weight(s);
+      if (s > kf) mine += v;
+      if (s >= sure) mine_sure += v;
+    });
+    block_scan(mine, sh, &total);
+    block_scan(mine_sure, sh, &total_sure);
+    if (tid == 0) sh.exchange[question + 1] = total_sure;
+    total = ask(total, &unused);
+    total_sure = heard(question++, &unused);
+    const u64 reach = share(total + (rf ? rf * weight(kf) : 0));
+    if (reach > total_sure && select(weight, least, sure, reach - total_sure, true, &key, &front, &own)) {
       const u64 w = weight(key);
-      const u32 some = (u32)((reach - front + w - 1) / w), all = (u32)(own / w);
+      const u32 some = (u32)((reach - total_sure - front + w - 1) / w), all = (u32)(own / w);
       if (key != kf) equal = all;
       kf = key;
       rf = some;
@@ -532,7 +592,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   int last = 0x7fffffff;
   if (rf != 0 && rf < equal) {
     u32 mine = 0, total;
-    for (int i = 0; i < width; ++i) mine += key_at(i) == kf;
+    in_order([&](const u32(&s)[4], int) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine += s[e] == kf;
+    });
     const u32 at = block_scan(mine, sh, &total);
     u64 before;
     ask(total, &before);
@@ -540,32 +603,30 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
     __syncthreads();
     if (before + at < rf && before + at + mine >= rf) {
       u32 need = rf - (u32)before - at;
-      for (int i = 0; i < width; ++i)
-        if (key_at(i) == kf && --need == 0) sh.exchange[question] = (u64)place_of(i) + 1;
+      in_order([&](const u32(&s)[4], int place) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (s[e] == kf && --need == 0) sh.exchange[question] = (u64)(base + place + e) + 1;
+      });
     }
     meet();
     u64 unused;
     last = (int)heard(question++, &unused) - 1;  // (one CTA's answer, and zeros)
   }
-  // ---- the draw, in the order of the vocabulary
-  auto kept = [&](int i, u32 s) { return s > kf || (s == kf && rf != 0 && place_of(i) <= last); };
+  // the draw, in the order of the vocabulary
+  auto kept = [&](u32 s, int place) { return s > kf || (s == kf && rf != 0 && base + place <= last); };
   u64 mass = 0, total, before;
-  for (int i = 0; i < width; i += kAtOnce) {
-    u32 at[kAtOnce];
+  in_order([&](const u32(&s)[4], int place) {
     bool some = false;
 #pragma unroll
-    for (int e = 0; e < kAtOnce; ++e) {
-      at[e] = i + e < width ? key_at(i + e) : 0;
-      if (at[e] == 0 || !kept(i + e, at[e])) at[e] = 0;
-      some |= at[e] != 0;
-    }
-    if (!__any_sync(0xffffffffu, some)) continue;
+    for (int e = 0; e < 4; ++e) some |= kept(s[e], place + e);
+    if (!__any_sync(0xffffffffu, some)) return;
 #pragma unroll
-    for (int e = 0; e < kAtOnce; ++e) {
-      const u64 v = weight(at[e]);
-      mass += at[e] != 0 ? v : 0;
+    for (int e = 0; e < 4; ++e) {
+      const u64 v = weight(s[e]);
+      if (kept(s[e], place + e)) mass += v;
     }
-  }
+  });
   u64 at = block_scan(mass, sh, &total);
   const u64 sum = ask(total, &before);
   at += before;
@@ -573,22 +634,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   u64 goal = (u64)((double)u * (double)sum);
   if (goal >= sum) goal = sum - 1;
   if (at <= goal && at + mass > goal) {
-    for (int i = 0; i < width; ++i) {
-      const u32 s = key_at(i);
-      if (s == 0 || !kept(i, s)) continue;
-      at += weight(s);
-      if (at > goal) {
-        p.tokens[row] = place_of(i);
-        break;
+    in_order([&](const u32(&s)[4], int place) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (at > goal || !kept(s[e], place + e)) continue;
+        at += weight(s[e]);
+        if (at > goal) p.tokens[row] = base + place + e;
       }
-    }
+    });
   }
   if constexpr (C > 1) {  // nobody leaves while another may read its memory
     __syncwarp();
-    if (listed)
-      cluster_wait();
-    else
-      cluster_barrier();
+    cluster_barrier();
   }
 }
 
