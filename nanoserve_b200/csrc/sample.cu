@@ -83,7 +83,8 @@ struct alignas(16) Shared {
   u64 exchange[12];                // what this CTA tells the others, a place per question
   u64 scan[32], scanned[32];
   u64 found[6];
-  u32 list_key[kList], list_at[kList];  // keys and their places in the vocabulary
+  u32 list_key[kList], list_at[kList];  // keys and their places in the vocabulary (or in this CTA's slice)
+  u32 listed;
 };
 
 __device__ __forceinline__ u32 peer_u32(const u32* p, u32 rank) {
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0;
   static_assert(kPowers == kThreads, "a thread per entry");
   sh.power[tid] = exp2(tid / (double)kPowers) * kOne;
-  if (tid == 0) sh.found[0] = 0;
+  if (tid == 0) sh.found[0] = 0, sh.listed = 0;
   const L* src = static_cast<const L*>(p.logits) + row * p.stride + base;
   u32 top = 0;
   constexpr int kVec = 16 / sizeof(L);
@@ -359,18 +360,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       if (cut && front[e] < left && upto[e] >= left) sh.found[0] = b0 + e, sh.found[1] = front[e], sh.found[2] = upto[e];
     if (by_weight) {
       // bins' weights at their near ends, in 2^-36: the true ones are at least e^(-40/2048) of that
-      constexpr double kWidth = (double)kReach / kBins;
-      const double near0 = exp(-kWidth * b0) * 68719476736.0;
+      constexpr float kWidth = kReach / kBins;
       u64 x[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        x[e] = (u64)(near0 * (e ? exp(-kWidth) : 1.0) * (min(upto[e], left) - min(front[e], left))) + 1;
+        x[e] = (u64)(__expf(-kWidth * (b0 + e)) * 68719476736.f * (float)(min(upto[e], left) - min(front[e], left))) + 1;
       u64 total;
       u64 before = block_scan(x[0] + x[1], sh, &total);
       // the border is where the most that the bins can hold reaches top_p of the least, or further, and where the least reaches
-      // top_p of the most, or nearer (1e-4: the steps' rounding)
+      // top_p of the most, or nearer (1e-4: the rounding of steps and weights)
       const double of_all = (double)fmaxf(top_p, 0.f) * (double)total;
-      const double lo = of_all * exp(-kWidth) * 0.9999, hi = fmin((double)total, of_all * exp(kWidth) * 1.0001);
+      const double lo = of_all * exp(-(double)kWidth) * 0.9999, hi = fmin((double)total, of_all * exp((double)kWidth) * 1.0001);
       if (tid == 0 && hi <= 0.0) sh.found[4] = 0, sh.found[5] = upto[0];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -399,21 +399,35 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
         block_scan(mine, sh, &total);
         if (tid == 0) sh.exchange[question] = total;
       }
-      u32 some = 0, mine_n;
-      in_order([&](const u32(&s)[4], int) {
+      // (a thread's first few are kept in registers, so that one pass counts them and has them)
+      constexpr int kFew = 4;
+      u32 some = 0, mine_n, few_key[kFew], few_at[kFew];
+      auto wanted = [&](u32 x) { return x > kf && bin_of(x) <= last_bin; };
+      in_order([&](const u32(&s)[4], int place) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) some += s[e] > kf && bin_of(s[e]) <= last_bin;
+        for (int e = 0; e < 4; ++e)
+          if (wanted(s[e])) {
+#pragma unroll
+            for (int f = 0; f < kFew; ++f)
+              if (some == (u32)f) few_key[f] = s[e], few_at[f] = base + place + e;
+            ++some;
+          }
       });
       u32 at = block_scan(some, sh, &mine_n);
-      if (some)
+      if (some <= kFew) {
+#pragma unroll
+        for (int f = 0; f < kFew; ++f)
+          if ((u32)f < some) sh.list_key[at + f] = few_key[f], sh.list_at[at + f] = few_at[f];
+      } else {
         in_order([&](const u32(&s)[4], int place) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (s[e] > kf && bin_of(s[e]) <= last_bin) {
+            if (wanted(s[e])) {
               sh.list_key[at] = s[e];
               sh.list_at[at++] = base + place + e;
             }
         });
+      }
       if (tid == 0) sh.exchange[question + 1] = mine_n;
       meet();
       if (rank != 0) {
@@ -446,19 +460,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       // sorted: falling keys, equal ones by rising place
       u64* other = reinterpret_cast<u64*>(sh.count);  // [kThreads]
       u64 x = tid < n_list ? (u64)sh.list_key[tid] << 32 | (0xffffffffu - tid) : 0;
-      for (int size = 2; size < 2 * n_list; size *= 2)
-        for (int dist = size / 2; dist > 0; dist /= 2) {
-          u64 y;
-          if (dist < 32) {
-            y = __shfl_xor_sync(0xffffffffu, x, dist);
-          } else {
-            other[tid] = x;
-            __syncthreads();
-            y = other[tid ^ dist];
-            __syncthreads();
+      int sorted = 32;  // threads that take part: the others hold zeros
+      while (sorted < n_list) sorted *= 2;
+      if (tid < sorted)
+        for (int size = 2; size < 2 * n_list; size *= 2)
+          for (int dist = size / 2; dist > 0; dist /= 2) {
+            u64 y;
+            if (dist < 32) {
+              y = __shfl_xor_sync(0xffffffffu, x, dist);
+            } else {
+              other[tid] = x;
+              asm volatile("bar.sync 1, %0;" ::"r"(sorted) : "memory");
+              y = other[tid ^ dist];
+              asm volatile("bar.sync 1, %0;" ::"r"(sorted) : "memory");
+            }
+            x = (((tid & size) == 0) == ((tid & dist) == 0)) == (x > y) ? x : y;
           }
-          x = (((tid & size) == 0) == ((tid & dist) == 0)) == (x > y) ? x : y;
-        }
       const int n_kept = by_count ? min(n_list, k) : n_list;
       u64 w = tid < n_kept ? weight((u32)(x >> 32)) : 0, total;
       const u64 before = block_scan(w, sh, &total);
@@ -491,7 +508,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   // Radix selection, level after level, among the keys from `least` to below `sure` (above kf) in falling order: the key at which the
   // sum of `measure` reaches `goal` (1 or more), the sum in front of it, and the sum of all its equals.  False: it is not reached.
   int level = 0;
-  auto select = [&](auto measure, u32 least, u32 sure, u64 goal, bool wide, u32* key, u64* front, u64* own) {
+  auto select = [&](auto over, auto measure, u32 least, u32 sure, u64 goal, bool wide, u32* key, u64* front, u64* own) {
     u32 prefix = 0;
     u64 above = 0, held = 0;
     const u64 part = rf ? rf * measure(kf) : 0;  // the kept equals of kf are no elements of the histograms
@@ -502,7 +519,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       ++level;
       for (int i = tid; i < 3 * kDigit; i += kThreads) limb[0][i] = 0;
       __syncthreads();
-      each([&](u32 s) {
+      over([&](u32 s) {
         if (s < least || s >= sure || (left < K::kBits && (s >> left) != prefix)) return;
         const u64 v = measure(s);
         const u32 bin = (s >> shift) & (kDigit - 1);
@@ -558,29 +575,61 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   u64 front, own;
   if (cut) {
     const u64 goal = k - front_k;
-    if (select([](u32) -> u64 { return 1; }, first_key(bin_k), bin_k > 0 ? first_key(bin_k - 1) : top + 1, goal, false, &key,
-               &front, &own)) {
+    if (select(each, [](u32) -> u64 { return 1; }, first_key(bin_k), bin_k > 0 ? first_key(bin_k - 1) : top + 1, goal, false,
+               &key, &front, &own)) {
       kf = key;
       rf = (u32)(goal - front);
       equal = (u32)own;
     }
   }
-  if (by_weight) {
-    // the weight of all that is left, and of what is surely in front of the border
-    const u32 least = first_key(bin_hi), sure = bin_lo > 0 ? first_key(bin_lo - 1) : top + 1;
-    u64 mine = 0, mine_sure = 0, total, total_sure, unused;
-    each([&](u32 s) {
-      const u64 v = weight(s);
-      if (s > kf) mine += v;
-      if (s >= sure) mine_sure += v;
-    });
+  // One pass over the weights: all that is left, what is surely kept, a list of what the border decides about.
+  const u32 least = by_weight ? first_key(bin_hi) : 0;
+  const u32 sure = max(kf + 1, by_weight && bin_lo > 0 ? first_key(bin_lo - 1) : by_weight ? top + 1 : 0);
+  const u32 low = max(least, rf ? kf : kf + 1);
+  u32* owned_n = sh.sums;                           // [kThreads], by the thread whose chunk they are in: equals of the border
+  u64* owned = reinterpret_cast<u64*>(sh.count);    // [kThreads] and weights that it keeps
+  owned_n[tid] = 0;
+  owned[tid] = 0;
+  __syncthreads();
+  u64 mine = 0, mine_sure = 0, total, before;
+  in_order([&](const u32(&s)[4], int place) {
+    bool some = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) some |= s[e] >= kf;
+    if (!__any_sync(0xffffffffu, some)) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const u64 v = weight(s[e]);
+      if (s[e] > kf) mine += v;
+      if (s[e] >= sure)
+        mine_sure += v;
+      else if (s[e] >= low) {
+        const u32 at = atomicAdd(&sh.listed, 1u);
+        if (at < kList) sh.list_key[at] = s[e], sh.list_at[at] = place + e;
+      }
+    }
+  });
+  bool listed = true;  // no CTA's list is too short
+  u64 total_sure = 0;
+  if (by_weight || rf) {
     block_scan(mine, sh, &total);
     block_scan(mine_sure, sh, &total_sure);
-    if (tid == 0) sh.exchange[question + 1] = total_sure;
-    total = ask(total, &unused);
-    total_sure = heard(question++, &unused);
+    if (tid == 0) sh.exchange[question + 1] = total_sure, sh.exchange[question + 2] = sh.listed > kList;
+    total = ask(total, &before);
+    total_sure = heard(question++, &before);
+    listed = heard(question++, &before) == 0;
+  }
+  const int n_list = (int)sh.listed;
+  auto over = [&](auto f) {
+    if (listed) {
+      if (tid < n_list) f(sh.list_key[tid]);
+    } else {
+      each(f);
+    }
+  };
+  if (by_weight) {
     const u64 reach = share(total + (rf ? rf * weight(kf) : 0));
-    if (reach > total_sure && select(weight, least, sure, reach - total_sure, true, &key, &front, &own)) {
+    if (reach > total_sure && select(over, weight, least, sure, reach - total_sure, true, &key, &front, &own)) {
       const u64 w = weight(key);
       const u32 some = (u32)((reach - total_sure - front + w - 1) / w), all = (u32)(own / w);
       if (key != kf) equal = all;
@@ -591,17 +640,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   // fewer than all of the border's equals: those up to a place
   int last = 0x7fffffff;
   if (rf != 0 && rf < equal) {
-    u32 mine = 0, total;
-    in_order([&](const u32(&s)[4], int) {
+    u32 equals = 0, sum;
+    if (listed) {
+      if (tid < n_list && sh.list_key[tid] == kf) atomicAdd(&owned_n[sh.list_at[tid] / chunk], 1u);
+      __syncthreads();
+      equals = owned_n[tid];
+    } else {
+      in_order([&](const u32(&s)[4], int) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine += s[e] == kf;
-    });
-    const u32 at = block_scan(mine, sh, &total);
-    u64 before;
-    ask(total, &before);
+        for (int e = 0; e < 4; ++e) equals += s[e] == kf;
+      });
+    }
+    const u32 at = block_scan(equals, sh, &sum);
+    ask(sum, &before);
     if (tid == 0) sh.exchange[question] = 0;
     __syncthreads();
-    if (before + at < rf && before + at + mine >= rf) {
+    if (before + at < rf && before + at + equals >= rf) {
       u32 need = rf - (u32)before - at;
       in_order([&](const u32(&s)[4], int place) {
 #pragma unroll
@@ -615,18 +669,23 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   }
   // the draw, in the order of the vocabulary
   auto kept = [&](u32 s, int place) { return s > kf || (s == kf && rf != 0 && base + place <= last); };
-  u64 mass = 0, total, before;
-  in_order([&](const u32(&s)[4], int place) {
-    bool some = false;
+  u64 mass = mine_sure;
+  if (!by_weight && !rf) {
+  } else if (listed) {
+    if (tid < n_list && kept(sh.list_key[tid], (int)sh.list_at[tid]))
+      atomicAdd(&owned[sh.list_at[tid] / chunk], weight(sh.list_key[tid]));
+    __syncthreads();
+    mass += owned[tid];
+  } else {
+    mass = 0;
+    in_order([&](const u32(&s)[4], int place) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) some |= kept(s[e], place + e);
-    if (!__any_sync(0xffffffffu, some)) return;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const u64 v = weight(s[e]);
-      if (kept(s[e], place + e)) mass += v;
-    }
-  });
+      for (int e = 0; e < 4; ++e) {
+        const u64 v = weight(s[e]);
+        if (kept(s[e], place + e)) mass += v;
+      }
+    });
+  }
   u64 at = block_scan(mass, sh, &total);
   const u64 sum = ask(total, &before);
   at += before;
