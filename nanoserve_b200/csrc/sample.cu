@@ -78,6 +78,7 @@ struct alignas(16) Shared {
   // this CTA's, then (sums) the cluster's up to each bin, within the part of it one CTA adds up
   alignas(8) u32 count[kBins];
   alignas(8) u32 sums[kBins];
+  u32 inside[kBins], insides[kBins];  // the same for how far in their bin the logits lie, in 256ths (each bin for itself)
   u32 limb[2][3][kDigit];          // a selection's bins (counts: the first alone), two in turn: peers may still read the other
   double power[kPowers];           // 2^44 2^(j / kPowers)
   u64 exchange[12];                // what this CTA tells the others, a place per question
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   };
 
   // ---- 1. the row's slice as keys, and the largest
-  for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0;
+  for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0, sh.inside[i] = 0;
   static_assert(kPowers == kThreads, "a thread per entry");
   sh.power[tid] = exp2(tid / (double)kPowers) * kOne;
   if (tid == 0) sh.found[0] = 0, sh.listed = 0;
@@ -296,17 +297,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
 
   const float steps = kBins / (kReach * T);
   // falls with the key (each operation keeps the order); kBins and above: not counted
-  auto bin_of = [&](u32 s) { return s == top ? 0 : (int)fminf((largest - K::logit(s)) * steps, (float)kBins); };
+  auto distance = [&](u32 s) { return s == top ? 0.f : fminf((largest - K::logit(s)) * steps, (float)kBins); };
+  auto bin_of = [&](u32 s) { return (int)distance(s); };
   bool cut = false;  // top_k leaves some out:
   int bin_k = kBins - 1, bin_lo = 0, bin_hi = kBins - 1;  // the bin of the top_k-th, and those that hold the top_p border
   u32 front_k = 0;   // logits in front of bin_k
 
   if (by_count || by_weight) {
     // ---- 2. distances, counted
+    const bool finer = by_weight && !by_count;
     each([&](u32 s) {
       if (s <= kf) return;
-      const int b = bin_of(s);
-      if (b < kBins) atomicAdd(&sh.count[b], 1u);
+      const float x = distance(s);
+      if (x >= (float)kBins) return;
+      const int b = (int)x;
+      atomicAdd(&sh.count[b], 1u);
+      if (finer) atomicAdd(&sh.inside[b], (u32)((x - (float)b) * 256.f));
     });
     meet();
     constexpr int kPart = kBins / C;  // bins this CTA adds up, two to a thread (C = 1), or one
@@ -330,9 +336,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         before += x[e];
+        const int at = rank * kPart + tid * kEach + e;
         if (tid * kEach + e < kPart) {
+          u32 y = 0;
+          if (finer) {
 #pragma unroll
-          for (u32 r = 0; r < (u32)C; ++r) to_peer_u32(&sh.sums[rank * kPart + tid * kEach + e], r, before);
+            for (u32 r = 0; r < (u32)C; ++r) y += peer_u32(&sh.inside[at], r);
+          }
+#pragma unroll
+          for (u32 r = 0; r < (u32)C; ++r) {
+            to_peer_u32(&sh.sums[at], r, before);
+            if (finer) to_peer_u32(&sh.insides[at], r, y);
+          }
         }
       }
     }
@@ -358,26 +373,33 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (cut && front[e] < left && upto[e] >= left) sh.found[0] = b0 + e, sh.found[1] = front[e], sh.found[2] = upto[e];
-    if (by_weight) {
-      // bins' weights at their near ends, in 2^-36: the true ones are at least e^(-40/2048) of that
+    __syncthreads();
+    if (by_weight && !(cut && sh.found[2] <= kList)) {
+      // The most and the least that the bins can weigh, in 2^-36.  A weight is e^(-w (bin + f)), f in [0, 1); with the mean of f
+      // known, the average is at least e^-(w mean) and at most what the chord from f = 0 to 1 gives there: w^2 / 8 apart.
       constexpr float kWidth = kReach / kBins;
-      u64 x[2];
+      u64 most[2], least[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        x[e] = (u64)(__expf(-kWidth * (b0 + e)) * 68719476736.f * (float)(min(upto[e], left) - min(front[e], left))) + 1;
-      u64 total;
-      u64 before = block_scan(x[0] + x[1], sh, &total);
+      for (int e = 0; e < 2; ++e) {
+        const u32 n = min(upto[e], left) - min(front[e], left);
+        const float near = __expf(-kWidth * (b0 + e)) * 68719476736.f * (float)n;
+        const float mean = finer && n > 0 ? (float)sh.insides[b0 + e] / (256.f * (float)n) : 0.f;
+        most[e] = (u64)(near * (1.f - mean * (1.f - __expf(-kWidth)))) + 1;
+        least[e] = (u64)(near * __expf(-kWidth * (finer ? mean + 1.f / 256.f : 1.f)));
+      }
+      u64 total_most, total_least;
+      u64 up = block_scan(most[0] + most[1], sh, &total_most), down = block_scan(least[0] + least[1], sh, &total_least);
       // the border is where the most that the bins can hold reaches top_p of the least, or further, and where the least reaches
-      // top_p of the most, or nearer (1e-4: the rounding of steps and weights)
-      const double of_all = (double)fmaxf(top_p, 0.f) * (double)total;
-      const double lo = of_all * exp(-(double)kWidth) * 0.9999, hi = fmin((double)total, of_all * exp((double)kWidth) * 1.0001);
+      // top_p of the most, or nearer (5e-5: the rounding of distances and weights)
+      const double share_p = (double)fmaxf(top_p, 0.f), lo = share_p * 0.99995 * (double)total_least,
+                   hi = share_p * 1.00005 * (double)total_most;
       if (tid == 0 && hi <= 0.0) sh.found[4] = 0, sh.found[5] = upto[0];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const double with = (double)(before + x[e]);
-        if ((double)before < lo && with >= lo) sh.found[3] = b0 + e;
-        if ((double)before < hi && with >= hi) sh.found[4] = b0 + e, sh.found[5] = upto[e];
-        before += x[e];
+        if ((double)up < lo && (double)(up + most[e]) >= lo) sh.found[3] = b0 + e;
+        if ((double)down < hi && (double)(down + least[e]) >= hi) sh.found[4] = b0 + e, sh.found[5] = upto[e];
+        up += most[e];
+        down += least[e];
       }
     }
     __syncthreads();
