@@ -168,15 +168,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
 
   // ---- 1. the row's slice as keys, and the largest
   for (int i = tid; i < kBins; i += kThreads) sh.count[i] = 0, sh.inside[i] = 0;
-  static_assert(kPowers == kThreads, "a thread per entry");
-  sh.power[tid] = exp2(tid / (double)kPowers) * kOne;
   if (tid == 0) sh.found[0] = 0, sh.listed = 0;
   const L* src = static_cast<const L*>(p.logits) + row * p.stride + base;
   u32 top = 0;
   constexpr int kVec = 16 / sizeof(L);
   const int vectors = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? n / kVec : 0;
-  for (int i = tid; i < vectors; i += kThreads) {
-    const uint4 x = __ldcg(reinterpret_cast<const uint4*>(src) + i);
+  constexpr int kAhead = 4;  // loads of a thread on their way at a time; the table is made while the first are
+  uint4 in[kAhead];
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e)
+    if (tid + e * kThreads < vectors) in[e] = __ldcg(reinterpret_cast<const uint4*>(src) + tid + e * kThreads);
+  static_assert(kPowers == kThreads, "a thread per entry");
+  sh.power[tid] = exp2(tid / (double)kPowers) * kOne;
+  auto take = [&](const uint4& x, int i) {
     const u32 w[4] = {x.x, x.y, x.z, x.w};
     u32 out[4];
 #pragma unroll
@@ -191,6 +195,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       }
     }
     reinterpret_cast<uint4*>(keys)[i] = make_uint4(out[0], out[1], out[2], out[3]);
+  };
+  for (int i0 = tid; i0 < vectors; i0 += kAhead * kThreads) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e)
+      if (i0 + e * kThreads < vectors) take(in[e], i0 + e * kThreads);
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e)
+      if (i0 + (kAhead + e) * kThreads < vectors)
+        in[e] = __ldcg(reinterpret_cast<const uint4*>(src) + i0 + (kAhead + e) * kThreads);
   }
   for (int i = vectors * kVec + tid; i < slice; i += kThreads) {
     const u32 k = i < n ? key_of(K::load(src, i)) : 0;
@@ -228,18 +241,21 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   // The weight of a stored key in multiples of 2^-44.  2^(x / 1024) with x = whole + r, |r| <= 1/2: the whole part's low ten bits
   // from a table, the others into its exponent, and (r ln2 / 1024)^n / n! up to n = 3 (the next term is under 2^-50).  The last
   // product is added to 2^52, which rounds it to a whole number.
-  const double per_T = kPowers * 1.4426950408889634074 / (double)T, offset = -(double)largest * per_T;
+  // For keys that have a weight (from `nothing` on; of others it may be anything).  Where the largest logit is plus infinity only
+  // its equals do.
+  const bool finite = largest < __uint_as_float(0x7f800000u);
+  const double per_T = finite ? kPowers * 1.4426950408889634074 / (double)T : 0.0, high = finite ? (double)largest : 0.0;
   auto weight = [&](u32 s) -> u64 {
     constexpr double a = 0.69314718055994530942 / kPowers;
     // fp32 to fp64 by its bits (a conversion takes as long as four products; numbers under 2^-126 become another such one)
     const u32 bits = __float_as_uint(K::logit(s));
     const double l = __hiloint2double((bits & 0x80000000u) | (((bits & 0x7fffffffu) >> 3) + (896u << 20)), bits << 29);
-    const double x = fma(l, per_T, offset), t = x + kWhole, r = x - (t - kWhole);
+    const double x = (l - high) * per_T, t = x + kWhole, r = x - (t - kWhole);
     const int j = __double2loint(t);
     const double power = sh.power[j & (kPowers - 1)];
     const double scaled = __hiloint2double(__double2hiint(power) + ((j >> 10) << 20), __double2loint(power));
     const double v = fma(fma(fma(fma(a * a * a / 6.0, r, a * a / 2.0), r, a), r, 1.0), scaled, 4503599627370496.0);
-    return s == top ? (u64)kOne : s < nothing ? 0 : (u64)__double_as_longlong(v) & ((1ull << 52) - 1);
+    return (u64)__double_as_longlong(v) & ((1ull << 52) - 1);
   };
 
   // kept: keys above kf, and the first rf (in order of index) of those that equal it
@@ -299,6 +315,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   // falls with the key (each operation keeps the order); kBins and above: not counted
   auto distance = [&](u32 s) { return s == top ? 0.f : fminf((largest - K::logit(s)) * steps, (float)kBins); };
   auto bin_of = [&](u32 s) { return (int)distance(s); };
+  // The smallest key of a bin up to b: a point to a lane.
+  auto first_key = [&](int b) {
+    u32 lo = 1, hi = top;
+    while (lo < hi) {
+      const u32 step = (hi - lo + 30) / 31, at = lo + min((u32)(tid & 31) * step, hi - lo);
+      const int f = __ffs(__ballot_sync(0xffffffffu, bin_of(at) <= b)) - 1;
+      hi = lo + min((u32)f * step, hi - lo);
+      if (f > 0) lo += (f - 1) * step + 1;
+    }
+    return lo;
+  };
   bool cut = false;  // top_k leaves some out:
   int bin_k = kBins - 1, bin_lo = 0, bin_hi = kBins - 1;  // the bin of the top_k-th, and those that hold the top_p border
   u32 front_k = 0;   // logits in front of bin_k
@@ -424,7 +451,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
       // (a thread's first few are kept in registers, so that one pass counts them and has them)
       constexpr int kFew = 4;
       u32 some = 0, mine_n, few_key[kFew], few_at[kFew];
-      auto wanted = [&](u32 x) { return x > kf && bin_of(x) <= last_bin; };
+      const u32 least = max(kf + 1, first_key(last_bin));
+      auto wanted = [&](u32 x) { return x >= least; };
       in_order([&](const u32(&s)[4], int place) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -516,17 +544,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Sampling p, int 
   }
 
   // ---- 4. more logits than that: they stay where they are
-  // The smallest key of a bin up to b: a point to a lane.
-  auto first_key = [&](int b) {
-    u32 lo = 1, hi = top;
-    while (lo < hi) {
-      const u32 step = (hi - lo + 30) / 31, at = lo + min((u32)(tid & 31) * step, hi - lo);
-      const int f = __ffs(__ballot_sync(0xffffffffu, bin_of(at) <= b)) - 1;
-      hi = lo + min((u32)f * step, hi - lo);
-      if (f > 0) lo += (f - 1) * step + 1;
-    }
-    return lo;
-  };
   // Radix selection, level after level, among the keys from `least` to below `sure` (above kf) in falling order: the key at which the
   // sum of `measure` reaches `goal` (1 or more), the sum in front of it, and the sum of all its equals.  False: it is not reached.
   int level = 0;
