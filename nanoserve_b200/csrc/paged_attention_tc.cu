@@ -14,6 +14,9 @@
 // The running maximum moves only when a row's new one is over 2^8 times as much in weight (sums stay far inside fp32's range
 // and the bf16 of a weight is as exact at 2^8 as at 1); O is then rescaled in tensor memory by the softmax warps, between the
 // two products that use it.
+// What bounds it: 128 x 128 scores take the tensor core 1024 cycles (both products) and the 16 exponentials per cycle of an SM
+// as long.  So a quarter of the exponentials are polynomials on the multiply-add pipes, pairs at a time, and the second product
+// starts when half of the weights are there.
 // Every wait is bounded; a time-out is recorded in the device's status word.
 #include <algorithm>
 
@@ -26,7 +29,7 @@ namespace {
 
 constexpr int kKeys = 128;     // keys per block
 constexpr int kThreads = 384;  // three warpgroups: registers are handed over in wholes of them
-constexpr int kRegsSoftmax = 232, kRegsOther = 40;  // 2 * 232 + 40 = 3 * 168, what the launch gives
+constexpr int kRegsSoftmax = 216, kRegsOther = 72;  // 2 * 216 + 72 = 3 * 168, what the launch gives
 constexpr int kPresent = 16;   // blocks whose presence bits are kept
 
 template <int D, bool TWO>
@@ -51,6 +54,27 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t desc_b,
 __device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
   return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>((128 * 128) >> 4) << 16 |
          static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x for x <= 128, two at a time, to 2^-18: x = n + f with |f| <= 1/2 (n + 127 lands in the low bits of a sum with 1.5 * 2^23), a
+// polynomial of fourth degree in f (least largest relative error), times 2^n.  0 from -127 down; not a number stays that.
+__device__ __forceinline__ float2 ex2_pair(float2 x) {
+  constexpr float kMagic = 12582912.f + 127.f;
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
+  auto both = [](float v) { return make_float2(v, v); };
+  const float2 t = add_f32x2(x, both(kMagic)), n = add_f32x2(t, both(-kMagic));
+  const float2 f = fma_f32x2(n, both(-1.f), x);
+  float2 r = fma_f32x2(f, both(0.009570102207362652f), both(0.05591785907745361f));
+  r = fma_f32x2(r, f, both(0.240247443318367f));
+  r = fma_f32x2(r, f, both(0.6931217908859253f));
+  r = fma_f32x2(r, f, both(0.9999992847442627f));
+  return mul_f32x2(r, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 
 // Ones in the bits below x.
@@ -121,8 +145,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* gen = raw + (base - smem_u32(raw));
   const uint32_t ring = base + geo::kQ;
   const uint32_t bar_full = base + geo::kBar, bar_empty = bar_full + 8 * geo::kBufs;
-  const uint32_t bar_s = bar_empty + 8 * geo::kBufs, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_q = bar_o + 16;
-  unsigned char* misc = gen + geo::kBar + 16 * geo::kBufs + 56;
+  // bar_p: [half of the weights][tile]
+  const uint32_t bar_s = bar_empty + 8 * geo::kBufs, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 16;
+  unsigned char* misc = gen + geo::kBar + 16 * geo::kBufs + 72;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 4);
   volatile unsigned* present = reinterpret_cast<volatile unsigned*>(misc + 8);  // [kPresent]
@@ -137,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(bar_s + 8 * t, 1);
       mbar_init(bar_p + 8 * t, 4);
+      mbar_init(bar_p + 16 + 8 * t, 4);
       mbar_init(bar_o + 8 * t, 1);
     }
     mbar_init(bar_q, 8);
@@ -231,11 +257,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     dk + (kk >> 2) * ((128 * 128) >> 4) + 2 * (kk & 3), idesc_s, kk > 0);
       umma_commit(bar_s + 8 * t);
     };
-    auto values = [&](int t, uint32_t buf, bool first) {
+    // (half of the keys)
+    auto values = [&](int t, int half, uint32_t buf, bool first) {
       const uint64_t dv = desc_v(buf);
 #pragma unroll
-      for (int kk = 0; kk < kKeys / 16; ++kk)
+      for (int k4 = 0; k4 < kKeys / 32; ++k4) {
+        const int kk = half * (kKeys / 32) + k4;
         umma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * kk, dv + kk * (2048 >> 4), idesc_o, !first || kk > 0);
+      }
+    };
+    auto weights_of = [&](int t, int half, uint32_t parity) {
+      mbar_wait(bar_p + 16 * half + 8 * t, parity, abort_flag);
+      __syncwarp();
+      tc_fence_after_sync();
     };
     auto loaded = [&] {
       mbar_wait(bar_full + 8 * s, ph, abort_flag);
@@ -282,12 +316,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t buf_k = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          mbar_wait(bar_p + 8 * t, i & 1, abort_flag);
+          weights_of(t, 0, i & 1);
+          if (elect_one()) values(t, 0, buf_v, i == 0);
           __syncwarp();
           if (t == 0 && i + 1 < n) buf_k = loaded();
-          tc_fence_after_sync();
+          weights_of(t, 1, i & 1);
           if (elect_one()) {
-            values(t, buf_v, i == 0);
+            values(t, 1, buf_v, false);
             if (t == 1) umma_commit(bar_empty + 8 * s_v);
             if (i + 1 < n) {
               scores(t, buf_k);
@@ -301,11 +336,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i + 1 < n) step();
       } else {
         const int t = i & 1;
-        mbar_wait(bar_p + 8 * t, (i >> 1) & 1, abort_flag);
+        weights_of(t, 0, (i >> 1) & 1);
+        if (elect_one()) values(t, 0, buf_v, i < 2);
         __syncwarp();
-        tc_fence_after_sync();
+        weights_of(t, 1, (i >> 1) & 1);
         if (elect_one()) {
-          values(t, buf_v, i < 2);
+          values(t, 1, buf_v, false);
           umma_commit(bar_empty + 8 * s_v);
           if (i + 2 >= n) umma_commit(bar_o + 8 * t);
         }
@@ -389,9 +425,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!((keep >> c) & 1)) s[32 * w + c] = -INFINITY;
         }
       }
-      float mx = -INFINITY;
+      float top[4];  // (four chains)
 #pragma unroll
-      for (int c = 0; c < 128; ++c) mx = fmaxf(mx, s[c]);
+      for (int c = 0; c < 4; ++c) top[c] = max3(s[c], s[4 + c], s[8 + c]);
+#pragma unroll
+      for (int c = 12; c < 124; c += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e] = max3(top[e], s[c + e], s[c + 4 + e]);
+      }
+      const float mx = fmaxf(max3(max3(top[0], s[124], s[125]), top[1], s[126]), max3(top[2], top[3], s[127]));
       const bool move = (mx - m) * p.scale_log2 > 8.f;  // (the first maximum that is one: m is -inf)
       const float mn = move ? mx : m;
       if (__any_sync(0xffffffffu, move)) {
@@ -411,26 +453,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         m = mn;
       }
       const float neg = m == -INFINITY ? 0.f : -m * p.scale_log2;
-      float2 sum = make_float2(0.f, 0.f);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int half = 0; half < 2; ++half) {
         uint32_t w[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          float2 x = make_float2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]);
+          float2 x = make_float2(s[64 * half + 2 * e], s[64 * half + 2 * e + 1]);
           x = fma_f32x2(x, make_float2(p.scale_log2, p.scale_log2), make_float2(neg, neg));
-          x = make_float2(ex2(x.x), ex2(x.y));
-          sum = add_f32x2(sum, x);
+          x = e % 4 == 3 ? ex2_pair(x) : make_float2(ex2(x.x), ex2(x.y));
+          sum[e & 1] = add_f32x2(sum[e & 1], x);
           const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
           w[e] = *reinterpret_cast<const uint32_t*>(&y);
         }
-        tmem_st_32x32(t_s + 32 * c, w);
+        tmem_st_32x32(t_s + 32 * half, w);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p + 16 * half + 8 * t);
       }
-      l += sum.x + sum.y;
-      tmem_st_wait();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_p + 8 * t);
+      sum[0] = add_f32x2(sum[0], sum[1]);
+      l += sum[0].x + sum[0].y;
     }
     // ------------------------------------------------------------ results
     if constexpr (TWO) {
