@@ -11,9 +11,10 @@
 // warps 0-3 / 4-7   softmax of the first / second half: one thread per row, 128 scores of it in registers
 // warp 8            loads: a ring of tiles of 128 keys (K, V in the order in which they are used), a page's rows per box
 // warp 9            issues the products (10, 11: nothing)
-// The running maximum moves only when a row's new one is over 2^8 times as much in weight (sums stay far inside fp32's range
-// and the bf16 of a weight is as exact at 2^8 as at 1); O is then rescaled in tensor memory by the softmax warps, between the
-// two products that use it.
+// The reference m of a row's weights is its maximum over the first block that it sees something of.  After that no maximum is
+// taken: weights over 1 are as exact as others, in fp32 and in bf16 alike, and a block whose weights add up to over 2^10 raises m
+// by the sum's exponent, for the next one; O is then rescaled in tensor memory, between the products that use it.  Where half a
+// block adds up to over 2^60 (scores that jump by tens), m is taken anew at once, and that half's weights too.
 // What bounds it: 128 x 128 scores take the tensor core 1024 cycles (both products) and the 16 exponentials per cycle of an SM
 // as long.  So a quarter of the exponentials are polynomials on the multiply-add pipes, pairs at a time, and the second product
 // starts when half of the weights are there.
@@ -30,6 +31,7 @@ namespace {
 constexpr int kKeys = 128;     // keys per block
 constexpr int kThreads = 384;  // three warpgroups: registers are handed over in wholes of them
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;  // 2 * 216 + 72 = 3 * 168, what the launch gives
+constexpr int kEvery = 4;      // every fourth pair of exponentials is a polynomial
 constexpr int kPresent = 16;   // blocks whose presence bits are kept
 
 template <int D, bool TWO>
@@ -80,57 +82,63 @@ __device__ __forceinline__ float2 ex2_pair(float2 x) {
 // Ones in the bits below x.
 __device__ __forceinline__ unsigned below(int x) { return x <= 0 ? 0u : x >= 32 ? ~0u : (1u << x) - 1; }
 
-// The sequence and first row of tile `t` (tiles of `size` rows, sequence after sequence); false: there is none.
-__device__ __forceinline__ bool find_tile(const ManyRows& p, int size, int t, int* b_out, int* r_out) {
-  const int lane = threadIdx.x & 31;
-  if (p.mask.flat) {
-    *b_out = 0;
-    *r_out = t * size;
-    return *r_out < p.mask.flat * p.rep;
-  }
-  int before = 0;
-  for (int b0 = 0; b0 < p.c.B; b0 += 32) {
-    const int b = b0 + lane;
-    int n = 0;
-    if (b < p.c.B) {
-      n = p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - __ldcg(p.cu_tokens + b) : 1;
-      n = (max(0, min(n, p.max_tokens)) * p.rep + size - 1) / size;
-    }
-    int x = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    const unsigned beyond = __ballot_sync(0xffffffffu, before + x > t);
-    if (beyond != 0) {
-      const int l = __ffs(beyond) - 1;
-      *b_out = b0 + l;
-      *r_out = (t - before - __shfl_sync(0xffffffffu, x - n, l)) * size;
-      return true;
-    }
-    before += __shfl_sync(0xffffffffu, x, 31);
-  }
-  return false;
-}
-
-// Rows r0 .. of sequence b as a tile of the kernel: what they see, and how many there are.
+// Tile `t` of `size` rows, sequence after sequence: its rows and what they see.  The whole warp asks.
 struct Tile {
   Visible v;     // rows: of the tile, counted in (token, head)
-  int n_new, p0;  // tokens of the sequence in this call, position of the first
-  __device__ __forceinline__ void set(const ManyRows& p, int b, int r0, int size) {
-    v.first = p.mask.flat ? 0 : p.cu_tokens ? __ldcg(p.cu_tokens + b) : b;
-    n_new = p.mask.flat ? p.mask.flat : p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - v.first : 1;
+  int b, r0;     // sequence, and the tile's first row of it
+  int p0;        // position of the sequence's first token in this call
+  // False: there is no such tile.
+  __device__ __forceinline__ bool find(const ManyRows& p, int size, int t) {
+    const int lane = threadIdx.x & 31;
+    int first = 0, n_new = p.mask.flat, len = 0, all = p.mask.flat * p.rep;
+    if (p.mask.flat) {
+      b = 0;
+      r0 = t * size;
+      len = __ldcg(p.c.lens);
+      if (r0 >= all) return false;
+    } else {
+      int before = 0;
+      b = -1;
+      for (int b0 = 0; b0 < p.c.B && b < 0; b0 += 32) {
+        int rows = 0;
+        if (b0 + lane < p.c.B) {
+          first = p.cu_tokens ? __ldcg(p.cu_tokens + b0 + lane) : b0 + lane;
+          n_new = p.cu_tokens ? __ldcg(p.cu_tokens + b0 + lane + 1) - first : 1;
+          len = __ldcg(p.c.lens + b0 + lane);
+          rows = first < 0 ? 0 : max(0, min(min(n_new, p.max_tokens), p.T - first)) * p.rep;
+        }
+        const int n = (rows + size - 1) / size;
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        const unsigned beyond = __ballot_sync(0xffffffffu, before + x > t);
+        const int l = beyond != 0 ? __ffs(beyond) - 1 : 31;
+        if (beyond != 0) {
+          b = b0 + l;
+          r0 = (t - before - __shfl_sync(0xffffffffu, x - n, l)) * size;
+          first = __shfl_sync(0xffffffffu, first, l);
+          n_new = __shfl_sync(0xffffffffu, n_new, l);
+          len = __shfl_sync(0xffffffffu, len, l);
+          all = __shfl_sync(0xffffffffu, rows, l);
+        }
+        before += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (b < 0) return false;
+    }
+    v.first = first;
     v.rows = n_new;
-    v.set<kKeys>(p.mask, __ldcg(p.c.lens + b), p.c.width << p.c.page_shift);
+    v.set<kKeys>(p.mask, len, p.c.width << p.c.page_shift);
     p0 = v.pmin;
-    const int all = v.first < 0 ? 0 : min(min(n_new, p.max_tokens), p.T - v.first) * p.rep;
-    v.rows = max(0, min(size, all - r0));
+    v.rows = min(size, all - r0);
     if (!p.mask.flat) {
-      v.pmax = p0 + (r0 + max(v.rows, 1) - 1) / p.rep;
+      v.pmax = p0 + (r0 + v.rows - 1) / p.rep;
       v.pmin = p0 + r0 / p.rep;
       v.span<kKeys>(p.mask);
     }
+    return true;
   }
 };
 
@@ -146,8 +154,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t ring = base + geo::kQ;
   const uint32_t bar_full = base + geo::kBar, bar_empty = bar_full + 8 * geo::kBufs;
   // bar_p: [half of the weights][tile]
-  const uint32_t bar_s = bar_empty + 8 * geo::kBufs, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 16;
-  unsigned char* misc = gen + geo::kBar + 16 * geo::kBufs + 72;
+  const uint32_t bar_s = bar_empty + 8 * geo::kBufs, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_h = bar_o + 16,
+                 bar_q = bar_h + 16;
+  unsigned char* misc = gen + geo::kBar + 16 * geo::kBufs + 88;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 4);
   volatile unsigned* present = reinterpret_cast<volatile unsigned*>(misc + 8);  // [kPresent]
@@ -164,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar_p + 8 * t, 4);
       mbar_init(bar_p + 16 + 8 * t, 4);
       mbar_init(bar_o + 8 * t, 1);
+      mbar_init(bar_h + 8 * t, 1);  // the second product's first half is done
     }
     mbar_init(bar_q, 8);
     fence_mbar_init();
@@ -184,12 +194,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the longest tiles of a prompt are its last
   const int z = blockIdx.x % p.splits, h = blockIdx.x / p.splits % p.c.Hk;
   const int tile = gridDim.x / (p.splits * p.c.Hk) - 1 - blockIdx.x / (p.splits * p.c.Hk);
-  int b = 0, r0 = 0;
-  const bool exists = find_tile(p, geo::kRowsPerCta, tile, &b, &r0);
   Tile tl;
+  const bool exists = tl.find(p, geo::kRowsPerCta, tile);
+  const int b = tl.b, r0 = tl.r0;
   int i0 = 0, n = 0;
   if (exists) {
-    tl.set(p, b, r0, geo::kRowsPerCta);
     i0 = (int)((long long)tl.v.count * z / p.splits);
     n = (int)((long long)tl.v.count * (z + 1) / p.splits) - i0;
   }
@@ -265,6 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int kk = half * (kKeys / 32) + k4;
         umma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * kk, dv + kk * (2048 >> 4), idesc_o, !first || kk > 0);
       }
+      if (half == 0) umma_commit(bar_h + 8 * t);
     };
     auto weights_of = [&](int t, int half, uint32_t parity) {
       mbar_wait(bar_p + 16 * half + 8 * t, parity, abort_flag);
@@ -370,13 +380,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int kChunks = TWO ? D / 8 : D / 16;
       const __nv_bfloat16* q = p.q + (long long)(v.first + tok) * p.q_stride + head * D;
       const uint32_t dst = base + (TWO ? t * geo::kTile : 0) + row * 128;
+      uint4 x[kChunks];  // (all on their way before the first is stored)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        x[c] = real ? __ldcg(reinterpret_cast<const uint4*>(q) + (TWO ? c : t * kChunks + c)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         const int cc = TWO ? c : t * kChunks + c;
-        const uint4 x = real ? __ldcg(reinterpret_cast<const uint4*>(q) + cc) : make_uint4(0, 0, 0, 0);
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (cc >> 3) * (128 * 128) +
                                                                       (((cc & 7) ^ (row & 7)) << 4)),
-                     "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                     "r"(x[c].x), "r"(x[c].y), "r"(x[c].z), "r"(x[c].w)
                      : "memory");
       }
       fence_proxy_async_smem();
@@ -395,19 +408,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int box_shift = min(p.c.page_shift, 7);
     const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
     const uint32_t t_s = tmem + lanes + 128 * t, t_o = tmem + lanes + 256 + 128 * t;
-    float m = -INFINITY, l = 0.f;
+    // m: the reference in powers of two (-inf: nothing seen yet); l: the sum; last: what the last block added to it
+    float m = -INFINITY, l = 0.f, last = 0.f;
+    auto rescale = [&](float corr) {
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16];
+        tmem_ld_32x16(t_o + 16 * c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+        tmem_st_32x16(t_o + 16 * c, o);
+      }
+      tmem_st_wait();
+    };
     int k = 0;  // blocks that this half has had
     for (int i = TWO ? 0 : t; i < n; i += TWO ? 1 : 2, ++k) {
       const int j0 = v.block(i0 + i) * kKeys;
+      const bool seen_by_all = wv.all(p.mask, j0, kKeys);
+      // (2^127 or nothing: an exponent that is one)
+      const int up = last > 1024.f && last < INFINITY ? (int)(__float_as_uint(last) >> 23) - 127 : 0;
+      const bool raise = __any_sync(0xffffffffu, up > 0);
       mbar_wait(bar_s + 8 * t, k & 1, abort_flag);
       __syncwarp();
       tc_fence_after_sync();
       float s[128];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-      tmem_ld_wait();
       const unsigned there = present[i % kPresent];
-      if (there != (unsigned)all_present || !wv.all(p.mask, j0, kKeys)) {
+      tmem_ld_wait();
+      if (!seen_by_all || there != (unsigned)all_present) {
         // visible columns: first ones up to `few`, and those from `lo` to `hi`
         const int hi = min(pos, v.end - 1) - j0;
         const int lo = p.mask.window ? pos - p.mask.window + 1 - j0 : 0;
@@ -425,55 +455,69 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!((keep >> c) & 1)) s[32 * w + c] = -INFINITY;
         }
       }
-      float top[4];  // (four chains)
+      auto largest = [&] {
+        float top[4];  // (four chains)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) top[c] = max3(s[c], s[4 + c], s[8 + c]);
+        for (int c = 0; c < 4; ++c) top[c] = max3(s[c], s[4 + c], s[8 + c]);
 #pragma unroll
-      for (int c = 12; c < 124; c += 8) {
+        for (int c = 12; c < 124; c += 8) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top[e] = max3(top[e], s[c + e], s[c + 4 + e]);
-      }
-      const float mx = fmaxf(max3(max3(top[0], s[124], s[125]), top[1], s[126]), max3(top[2], top[3], s[127]));
-      const bool move = (mx - m) * p.scale_log2 > 8.f;  // (the first maximum that is one: m is -inf)
-      const float mn = move ? mx : m;
-      if (__any_sync(0xffffffffu, move)) {
-        const float corr = m == -INFINITY ? 0.f : ex2((m - mn) * p.scale_log2);
-        l *= corr;
-        if (k > 0) {
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld_32x16(t_o + 16 * c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-            tmem_st_32x16(t_o + 16 * c, o);
-          }
+          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], s[c + e], s[c + 4 + e]);
         }
-        m = mn;
+        return p.scale_log2 * fmaxf(max3(max3(top[0], s[124], s[125]), top[1], s[126]), max3(top[2], top[3], s[127]));
+      };
+      if (raise) {  // (k > 0: O is there)
+        const float corr = __uint_as_float((unsigned)(127 - up) << 23);
+        l *= corr;
+        m += (float)up;
+        rescale(corr);
       }
-      const float neg = m == -INFINITY ? 0.f : -m * p.scale_log2;
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      if (__any_sync(0xffffffffu, m == -INFINITY)) {
+        const float mx = largest();
+        if (m == -INFINITY) m = mx;  // (what this row's O and l hold so far is zero)
+      }
+      last = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t w[32];
+        float added;
+        auto weigh = [&] {
+          const float neg = m == -INFINITY ? 0.f : -m;
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float2 x = make_float2(s[64 * half + 2 * e], s[64 * half + 2 * e + 1]);
-          x = fma_f32x2(x, make_float2(p.scale_log2, p.scale_log2), make_float2(neg, neg));
-          x = e % 4 == 3 ? ex2_pair(x) : make_float2(ex2(x.x), ex2(x.y));
-          sum[e & 1] = add_f32x2(sum[e & 1], x);
-          const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
-          w[e] = *reinterpret_cast<const uint32_t*>(&y);
+          for (int e = 0; e < 32; ++e) {
+            float2 x = make_float2(s[64 * half + 2 * e], s[64 * half + 2 * e + 1]);
+            x = fma_f32x2(x, make_float2(p.scale_log2, p.scale_log2), make_float2(neg, neg));
+            x = e % kEvery == kEvery - 1 ? ex2_pair(x) : make_float2(ex2(x.x), ex2(x.y));
+            sum[e & 1] = add_f32x2(sum[e & 1], x);
+            const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
+            w[e] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          sum[0] = add_f32x2(sum[0], sum[1]);
+          added = sum[0].x + sum[0].y;
+        };
+        weigh();
+        if (__any_sync(0xffffffffu, !(added < 1152921504606846976.f))) {  // 2^60, or not a number
+          const float mn = fmaxf(m, largest()), corr = m == mn ? 1.f : ex2(m - mn);
+          if (half == 1) {  // the first half's product has to be done before O is rescaled
+            mbar_wait(bar_h + 8 * t, k & 1, abort_flag);
+            __syncwarp();
+            tc_fence_after_sync();
+          }
+          if (k > 0 || half == 1) rescale(corr);
+          l *= corr;
+          last *= corr;
+          m = mn;
+          weigh();
         }
         tmem_st_32x32(t_s + 32 * half, w);
+        last += added;
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_p + 16 * half + 8 * t);
       }
-      sum[0] = add_f32x2(sum[0], sum[1]);
-      l += sum[0].x + sum[0].y;
+      l += last;
     }
     // ------------------------------------------------------------ results
     if constexpr (TWO) {
@@ -506,15 +550,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float* other = reinterpret_cast<const float*>(gen + geo::kQ);
       if (!TWO && n > 1) {
         const float m1 = other[D * 128 + row], l1 = other[(D + 1) * 128 + row], mn = fmaxf(m, m1);
-        f0 = m == mn ? 1.f : ex2((m - mn) * p.scale_log2);
-        f1 = m1 == mn ? 1.f : ex2((m1 - mn) * p.scale_log2);
+        f0 = m == mn ? 1.f : ex2(m - mn);
+        f1 = m1 == mn ? 1.f : ex2(m1 - mn);
         l = f0 * l + f1 * l1;
         m = mn;
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const long long slot = (((long long)h * p.slots + (TWO ? 2 * tile + t : tile)) * p.splits + z) * 128 + row;
       __nv_bfloat16* out = p.out + (long long)(v.first + tok) * p.out_stride + head * D;
-      if (p.part != nullptr && real) p.stat[slot] = make_float2(m * p.scale_log2, l);
+      if (p.part != nullptr && real) p.stat[slot] = make_float2(m, l);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -560,11 +604,9 @@ __global__ void __launch_bounds__(128) join_many_kernel(const ManyRows p) {
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   const int size = p.two ? 256 : 128;
-  int b, r0;
-  if (!find_tile(p, size, p.two ? slot >> 1 : slot, &b, &r0)) return;
   Tile tl;
-  tl.set(p, b, r0, size);
-  const int off = p.two ? 128 * (slot & 1) : 0, row = blockIdx.y * 4 + (threadIdx.x >> 5), r = r0 + off + row;
+  if (!tl.find(p, size, p.two ? slot >> 1 : slot)) return;
+  const int off = p.two ? 128 * (slot & 1) : 0, row = blockIdx.y * 4 + (threadIdx.x >> 5), r = tl.r0 + off + row;
   if (off + row >= tl.v.rows) return;
   const long long at = ((long long)h * p.slots + slot) * p.splits * 128 + row;
   float m = -INFINITY, l = 0.f, o[E] = {};
