@@ -8,33 +8,32 @@
 // the other's softmax runs:
 //   two tiles (TWO)  two neighbouring row tiles share every block of keys
 //   one tile         up to 128 rows: the two halves take blocks of keys in turn, and are joined at the end
-// warps 0-7 / 8-15  softmax of the first / second tile: two threads per row, 64 scores of it each.  (One thread per row, half as
-//                   many warps, left the schedulers waiting for the one warp's results: 412 us for 8192 tokens of 28 / 4 heads of
-//                   128 with a window of 4096, against XX)
-// warp 16           loads: a ring of tiles of 128 keys (K, V in the order in which they are used), a page's rows per box
-// warp 17           issues the products (18, 19: nothing)
-// A row's reference m moves only when its maximum is over 2^8 times as much in weight (sums stay far inside fp32's range and the
-// bf16 of a weight is as exact at 2^8 as at 1); O is then rescaled in tensor memory by the softmax warps, between the two products
-// that use it.
+// warps 0-3 / 4-7   softmax of the first / second tile: one thread per row, 128 scores of it in registers
+// warp 8            loads: a ring of tiles of 128 keys (K, V in the order in which they are used), a page's rows per box
+// warp 9            issues the products (10, 11: nothing)
+// The reference m of a row's weights is its maximum over the first block that it sees something of.  After that no maximum is
+// taken: weights over 1 are as exact as others, in fp32 and in bf16 alike, and a block whose weights add up to over 2^10 raises m
+// by the sum's exponent, for the next one; O is then rescaled in tensor memory, between the products that use it.  Where half a
+// block adds up to over 2^60 (scores that jump by tens), m is taken anew at once, and that half's weights too.
 // What bounds it: 128 x 128 scores take the tensor core 1024 cycles (both products) and the 16 exponentials per cycle of an SM
-// as long.  So a quarter of the exponentials are polynomials on the multiply-add pipes, pairs at a time, and the second product
+// as long.  So an eighth of the exponentials are polynomials on the multiply-add pipes, pairs at a time, and the second product
 // starts when half of the weights are there.
 // Every wait is bounded; a time-out is recorded in the device's status word.
 #include <algorithm>
 
 #include "paged_attention.cuh"
 #include "ptx.cuh"
+#include "w4_common.cuh"
 #include "w4_internal.h"
 
 namespace b2 {
 namespace {
 
 constexpr int kKeys = 128;     // keys per block
-constexpr int kLoadWarp = 16, kMmaWarp = 17;
-constexpr int kThreads = 640;  // five warpgroups: registers are handed over in wholes of them
-constexpr int kRegsSoftmax = 104, kRegsOther = 64;  // 4 * 104 + 64 = 5 * 96, what the launch gives
-constexpr float kRaise = 8.f;  // powers of two by which a maximum has to exceed a row's reference to become it
-constexpr int kEvery = 4;      // every fourth pair of exponentials is a polynomial
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 384;  // three warpgroups: registers are handed over in wholes of them
+constexpr int kRegsSoftmax = 216, kRegsOther = 72;  // 2 * 216 + 72 = 3 * 168, what the launch gives
+constexpr int kEvery = 8;      // every eighth pair of exponentials is a polynomial
 constexpr int kPresent = 16;   // blocks whose presence bits are kept
 
 template <int D, bool TWO>
@@ -80,20 +79,6 @@ __device__ __forceinline__ float2 ex2_pair(float2 x) {
   r = fma_f32x2(r, f, both(0.6931217908859253f));
   r = fma_f32x2(r, f, both(0.9999992847442627f));
   return mul_f32x2(r, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
-}
-
-// Whether `yes` holds in any of the 256 threads that meet at barrier `id`.
-__device__ __forceinline__ bool any_of_256(int id, bool yes) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred q, r;\n\t"
-      "setp.ne.u32 q, %2, 0;\n\t"
-      "bar.red.or.pred r, %1, 256, q;\n\t"
-      "selp.u32 %0, 1, 0, r;\n\t}"
-      : "=r"(any)
-      : "r"(id), "r"((uint32_t)yes)
-      : "memory");
-  return any != 0;
 }
 
 // Ones in the bits below x.
@@ -171,8 +156,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t ring = base + geo::kQ;
   const uint32_t bar_full = base + geo::kBar, bar_empty = bar_full + 8 * geo::kBufs;
   // bar_p: [half of the weights][tile]
-  const uint32_t bar_s = bar_empty + 8 * geo::kBufs, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 16;
-  unsigned char* misc = gen + geo::kBar + 16 * geo::kBufs + 72;
+  const uint32_t bar_s = bar_empty + 8 * geo::kBufs, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_h = bar_o + 16,
+                 bar_q = bar_h + 16;
+  unsigned char* misc = gen + geo::kBar + 16 * geo::kBufs + 88;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 4);
   volatile unsigned* present = reinterpret_cast<volatile unsigned*>(misc + 8);  // [kPresent]
@@ -189,8 +175,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar_p + 8 * t, 4);
       mbar_init(bar_p + 16 + 8 * t, 4);
       mbar_init(bar_o + 8 * t, 1);
+      mbar_init(bar_h + 8 * t, 1);  // the second product's first half is done
     }
-    mbar_init(bar_q, 16);
+    mbar_init(bar_q, 8);
     fence_mbar_init();
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
@@ -289,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int kk = half * (kKeys / 32) + k4;
         umma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * kk, dv + kk * (2048 >> 4), idesc_o, !first || kk > 0);
       }
+      if (half == 0) umma_commit(bar_h + 8 * t);
     };
     auto weights_of = [&](int t, int half, uint32_t parity) {
       mbar_wait(bar_p + 16 * half + 8 * t, parity, abort_flag);
@@ -385,168 +373,178 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     if (exists) {
-      // ------------------------------------------------------------ softmax: a row, and half of its columns, per thread
-      const int t = warp >> 3, hf = (warp >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
+      // ------------------------------------------------------------ softmax: a row per thread
+      const int t = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
       const int r = r0 + (TWO ? 128 * t : 0) + row, tok = r / p.rep, head = h * p.rep + r - tok * p.rep;
       const unsigned real = __ballot_sync(0xffffffffu, (TWO ? 128 * t : 0) + row < v.rows);  // of the warp's rows
-      // Sixteen bytes to a lane, the lanes of half a row beside one another: rows of global memory in whole sectors.
-      constexpr int kPieces = D / 16, kRowsAtOnce = 32 / kPieces;  // of half a row of bf16; rows per instruction
+      // Sixteen bytes to a lane, the lanes of a row beside one another: rows of global memory in whole sectors.
+      constexpr int kPieces = D / 8, kRowsAtOnce = 32 / kPieces;  // of a row of bf16; rows per instruction
       const int piece = lane % kPieces, sub = lane / kPieces;
       {
-        // Q: chunk c of sixteen bytes of row r lies at c ^ (r & 7)
+        // Q (one tile: each half of the warps half of its rows); chunk c of sixteen bytes of row r lies at c ^ (r & 7)
         constexpr int kLoads = (TWO ? 32 : 16) / kRowsAtOnce;
         const long long off = (long long)(v.first + tok) * p.q_stride + head * D;
-        const int cc = hf * kPieces + piece;
         uint4 x[kLoads];  // (all on their way before the first is stored)
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
           const int rr = (TWO ? 0 : 16 * t) + i * kRowsAtOnce + sub;
           const long long at = __shfl_sync(0xffffffffu, off, rr);
-          x[i] = (real >> rr) & 1 ? __ldcg(reinterpret_cast<const uint4*>(p.q + at) + cc) : make_uint4(0, 0, 0, 0);
+          x[i] = (real >> rr) & 1 ? __ldcg(reinterpret_cast<const uint4*>(p.q + at) + piece) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
           const int qrow = quad * 32 + (TWO ? 0 : 16 * t) + i * kRowsAtOnce + sub;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (TWO ? t * geo::kTile : 0) + (cc >> 3) * (128 * 128) +
-                                                                        qrow * 128 + (((cc & 7) ^ (qrow & 7)) << 4)),
-                       "r"(x[i].x), "r"(x[i].y), "r"(x[i].z), "r"(x[i].w)
-                       : "memory");
+          sts128(base + (TWO ? t * geo::kTile : 0) + (piece >> 3) * (128 * 128) + qrow * 128 + (((piece & 7) ^ (qrow & 7)) << 4), x[i]);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_q);
       }
       const int pos = p.mask.flat ? v.pmax : tl.p0 + tok;
-      // positions of this warp's rows
-      const int w0 = r0 + (TWO ? 128 * t : 0) + quad * 32;
-      Visible wv = v;
-      if (!p.mask.flat) {
-        wv.pmin = tl.p0 + w0 / p.rep;
-        wv.pmax = tl.p0 + (w0 + 31) / p.rep;
+      // The blocks that every row of this warp sees whole, as far as positions go: [whole0, whole1) of those behind the first tokens'.
+      int whole0 = 0, whole1 = 0;
+      {
+        const int w0 = r0 + (TWO ? 128 * t : 0) + quad * 32;
+        const int first = p.mask.flat ? v.pmin : tl.p0 + w0 / p.rep, last = p.mask.flat ? v.pmax : tl.p0 + (w0 + 31) / p.rep;
+        const int lo = p.mask.window ? max(0, last - p.mask.window + 1) : 0;
+        const int skip = v.n_sink - v.from - i0;  // block b of the keys is this CTA's i = b + skip
+        whole0 = max(v.n_sink - i0, (lo + kKeys - 1) / kKeys + skip);
+        whole1 = max(0, min(v.end, first + 1)) / kKeys + skip;
       }
       const int all_present = (1 << (kKeys / min(p.c.page, kKeys))) - 1;
-      const int box_shift = min(p.c.page_shift, 7);
       const uint32_t lanes = (uint32_t)quad * 32 << 16;
-      const uint32_t t_s = tmem + lanes + 128 * t, t_o = tmem + lanes + 256 + 128 * t + hf * (D / 2);
-      // a number of this thread's for the other one of its row, through columns of S that nothing else uses then
-      auto swapped = [&](float mine) {
-        tmem_st_32x1(t_s + 64 + hf, __float_as_uint(mine));
+      const uint32_t t_s = tmem + lanes + 128 * t, t_o = tmem + lanes + 256 + 128 * t;
+      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+      // m: the reference in powers of two (-inf: nothing seen yet); l: the sum; up: powers by which the last block asks m to rise
+      float m = -INFINITY, l = 0.f;
+      int up = 0;
+      auto rescale = [&](float corr) {
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld_32x16(t_o + 16 * c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+          tmem_st_32x16(t_o + 16 * c, o);
+        }
         tmem_st_wait();
-        tc_fence_before_sync();
-        asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
-        tc_fence_after_sync();
-        const uint32_t x = tmem_ld_32x1(t_s + 65 - hf);
-        tmem_ld_wait();
-        return __uint_as_float(x);
       };
-      float m = -INFINITY, l = 0.f;  // the row's reference in powers of two (-inf: nothing seen yet), and this half's sum
-      int k = 0;                     // blocks that this tile has had
-      for (int i = TWO ? 0 : t; i < n; i += TWO ? 1 : 2, ++k) {
-        const int j0 = v.block(i0 + i) * kKeys;
-        const bool seen_by_all = wv.all(p.mask, j0, kKeys);
-        mbar_wait(bar_s + 8 * t, k & 1, abort_flag);
+      uint32_t parity = 0;  // of the tile's block
+      for (int i = TWO ? 0 : t; i < n; i += TWO ? 1 : 2, parity ^= 1) {
+        const bool whole = i >= whole0 && i < whole1;
+        const bool some = __any_sync(0xffffffffu, up > 0 || m == -INFINITY);
+        mbar_wait(bar_s + 8 * t, parity, abort_flag);
         __syncwarp();
         tc_fence_after_sync();
-        float s[64];
+        float s[128];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          tmem_ld_32x32(t_s + 64 * hf + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
         const unsigned there = present[i % kPresent];
         tmem_ld_wait();
-        if (!seen_by_all || there != (unsigned)all_present) {
+        if (!whole || there != (unsigned)all_present) {
           // visible columns: first ones up to `few`, and those from `lo` to `hi`
+          const int j0 = v.block(i0 + i) * kKeys, box_shift = min(p.c.page_shift, 7);
           const int hi = min(pos, v.end - 1) - j0;
           const int lo = p.mask.window ? pos - p.mask.window + 1 - j0 : 0;
           const int few = p.mask.window ? min(p.mask.sinks - j0, hi + 1) : 0;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int at = 64 * hf + 32 * c;
-            unsigned keep = (below(hi + 1 - at) & ~below(lo - at)) | below(few - at);
-            keep &= ((there >> (at >> box_shift)) & 1 ? 0xffffu : 0u) | ((there >> ((at + 16) >> box_shift)) & 1 ? 0xffff0000u : 0u);
+          for (int c = 0; c < 4; ++c) {
+            unsigned keep = (below(hi + 1 - 32 * c) & ~below(lo - 32 * c)) | below(few - 32 * c);
+            keep &= ((there >> (32 * c >> box_shift)) & 1 ? 0xffffu : 0u) | ((there >> ((32 * c + 16) >> box_shift)) & 1 ? 0xffff0000u : 0u);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!((keep >> e) & 1)) s[32 * c + e] = -INFINITY;
           }
         }
-        float top[4];  // (four chains)
+        auto largest = [&] {
+          float top[4];  // (four chains)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top[e] = max3(s[e], s[4 + e], s[8 + e]);
+          for (int c = 0; c < 4; ++c) top[c] = max3(s[c], s[4 + c], s[8 + c]);
 #pragma unroll
-        for (int c = 12; c < 60; c += 8) {
+          for (int c = 12; c < 124; c += 8) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], s[c + e], s[c + 4 + e]);
-        }
-        const float mx = p.scale_log2 * fmaxf(max3(max3(top[0], s[60], s[61]), top[1], s[62]), max3(top[2], top[3], s[63]));
-        // (also: the other half of the row has been read, part of which this one's weights will lie on)
-        tc_fence_before_sync();
-        const bool raise = any_of_256(1 + t, mx - m > kRaise);  // (-inf from -inf is no number, and no raise)
-        tc_fence_after_sync();
-        if (raise) {
-          const float both = fmaxf(mx, swapped(mx)), mn = both - m > kRaise ? both : m;
-          const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
-          l *= corr;
-          m = mn;
-          if (k > 0) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[16];
-              tmem_ld_32x16(t_o + 16 * c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-              tmem_st_32x16(t_o + 16 * c, o);
-            }
+            for (int e = 0; e < 4; ++e) top[e] = max3(top[e], s[c + e], s[c + 4 + e]);
           }
+          return p.scale_log2 * fmaxf(max3(max3(top[0], s[124], s[125]), top[1], s[126]), max3(top[2], top[3], s[127]));
+        };
+        const bool first = i < (TWO ? 1 : 2);
+        if (some) {
+          if (!first && __any_sync(0xffffffffu, up > 0)) {
+            const float corr = __uint_as_float((unsigned)(127 - up) << 23);
+            l *= corr;
+            m += (float)up;
+            rescale(corr);
+          }
+          const float mx = largest();
+          if (m == -INFINITY) m = mx;  // (what this row's O and l hold so far is zero)
         }
-        const float neg = m == -INFINITY ? 0.f : -m;
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t w[32];
+        float added = 0.f;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float2 x = make_float2(s[2 * e], s[2 * e + 1]);
-          x = fma_f32x2(x, make_float2(p.scale_log2, p.scale_log2), make_float2(neg, neg));
-          x = e % kEvery == kEvery - 1 ? ex2_pair(x) : make_float2(ex2(x.x), ex2(x.y));
-          sum[e & 1] = add_f32x2(sum[e & 1], x);
-          const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
-          w[e] = *reinterpret_cast<const uint32_t*>(&y);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[32];
+          float mine;
+          auto weigh = [&] {
+            const float neg = m == -INFINITY ? 0.f : -m;
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float2 x = fma_f32x2(make_float2(s[64 * half + 2 * e], s[64 * half + 2 * e + 1]), scale2, make_float2(neg, neg));
+              x = e % kEvery == kEvery - 1 ? ex2_pair(x) : make_float2(ex2(x.x), ex2(x.y));
+              sum[e & 1] = add_f32x2(sum[e & 1], x);
+              const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
+              w[e] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+            tmem_st_32x32(t_s + 32 * half, w);
+            sum[0] = add_f32x2(sum[0], sum[1]);
+            mine = sum[0].x + sum[0].y;
+          };
+          weigh();
+          if (__any_sync(0xffffffffu, !(mine < 1152921504606846976.f))) {  // 2^60, or not a number
+            const float mn = fmaxf(m, largest()), corr = m == mn ? 1.f : ex2(m - mn);
+            if (half == 1) {  // the first half's product has to be done before O is rescaled
+              mbar_wait(bar_h + 8 * t, parity, abort_flag);
+              __syncwarp();
+              tc_fence_after_sync();
+            }
+            if (!first || half == 1) rescale(corr);
+            l *= corr;
+            added *= corr;
+            m = mn;
+            weigh();
+          }
+          added += mine;
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p + 16 * half + 8 * t);
         }
-        tmem_st_32x32(t_s + 32 * hf, w);
-        sum[0] = add_f32x2(sum[0], sum[1]);
-        l += sum[0].x + sum[0].y;
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p + 16 * hf + 8 * t);
+        l += added;
+        up = added > 1024.f && added < INFINITY ? (int)(__float_as_uint(added) >> 23) - 127 : 0;
       }
       // ------------------------------------------------------------ results
-      if (n > (TWO ? 0 : t)) {
-        mbar_wait(bar_o + 8 * t, 0, abort_flag);
-        __syncwarp();
-        tc_fence_after_sync();
-        l += swapped(l);
-      } else if (TWO) {
-        any_of_256(1 + t, false);  // (nobody stores Q any more where rows will leave)
-      }
+      if (n > (TWO ? 0 : t)) mbar_wait(bar_o + 8 * t, 0, abort_flag);
+      __syncwarp();
+      tc_fence_after_sync();
       float* other = reinterpret_cast<float*>(gen + geo::kQ);  // one tile: the second half's, [D + 2][128], where the ring was
       if constexpr (!TWO) {
-        if (t == 0 && n > 1) mbar_wait(bar_o + 8, 0, abort_flag);  // (and both halves' products have left the ring)
+        if (n > 1) mbar_wait(bar_o + 8 * (1 - t), 0, abort_flag);  // (both halves' products have left Q and the ring)
+        __syncwarp();
         if (t == 1 && n > 1) {
-          mbar_wait(bar_o, 0, abort_flag);
-          __syncwarp();
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
             tmem_ld_32x16(t_o + 16 * c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) other[(hf * (D / 2) + 16 * c + e) * 128 + row] = __uint_as_float(o[e]);
+            for (int e = 0; e < 16; ++e) other[(16 * c + e) * 128 + row] = __uint_as_float(o[e]);
           }
-          if (hf == 0) {
-            other[D * 128 + row] = m;
-            other[(D + 1) * 128 + row] = l;
-          }
+          other[D * 128 + row] = m;
+          other[(D + 1) * 128 + row] = l;
         }
-        asm volatile("bar.sync 3, 512;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      } else if (n == 0) {
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");  // (nobody stores Q any more where rows will leave)
       }
       if (TWO || t == 0) {
         float f0 = 1.f, f1 = 0.f;
@@ -561,32 +559,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const long long slot = (((long long)h * p.slots + (TWO ? 2 * tile + t : tile)) * p.splits + z) * 128 + row;
         const bool parts = p.part != nullptr;
-        if (parts && hf == 0 && (real >> lane) & 1) p.stat[slot] = make_float2(m, l);
-        // rows leave through the place where Q was, D bytes of a row at a time, to be stored in whole sectors
-        const uint32_t stage = base + (TWO ? t * geo::kTile : 0) + hf * (geo::kTile / 2) + quad * 32 * D;
+        if (parts && (real >> lane) & 1) p.stat[slot] = make_float2(m, l);
+        // rows leave through the place where Q was, 2 D bytes of a row at a time, to be stored in whole sectors
+        constexpr int kBytes = 2 * D;
+        const uint32_t stage = base + (TWO ? t * geo::kTile : 0) + quad * 32 * kBytes;
         const long long off = parts ? slot * D : (long long)(v.first + tok) * p.out_stride + head * D;
-        auto staged = [&](int at, const uint32_t(&x)[4]) {
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * D + ((at ^ (lane & (kPieces - 1))) << 4)),
-                       "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
-                       : "memory");
+        auto staged = [&](int at, uint32_t a, uint32_t bb, uint32_t c, uint32_t d) {
+          sts128(stage + lane * kBytes + ((at ^ (lane & (kPieces - 1))) << 4), make_uint4(a, bb, c, d));
         };
-        auto store = [&](char* to, int elem, int first_elem) {  // this half's D bytes of every row
+        auto store = [&](char* to, int elem, int first_elem) {  // 2 D bytes of every row
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
             const int rr = i * kRowsAtOnce + sub;
-            uint4 x;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                         : "r"(stage + rr * D + ((piece ^ (rr & (kPieces - 1))) << 4))
-                         : "memory");
+            const uint4 x = lds128(stage + rr * kBytes + ((piece ^ (rr & (kPieces - 1))) << 4));
             const long long at = __shfl_sync(0xffffffffu, off, rr);
             if ((real >> rr) & 1) *reinterpret_cast<uint4*>(to + (at + first_elem) * elem + piece * 16) = x;
           }
           __syncwarp();
         };
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {  // sixteen columns
+        for (int c = 0; c < D / 16; ++c) {  // sixteen columns
           uint32_t o[16];
           __syncwarp();
           if (n > 0) {
@@ -597,29 +590,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             x[e] = n > 0 ? __uint_as_float(o[e]) : 0.f;
-            if (two_parts) x[e] = f0 * x[e] + f1 * other[(hf * (D / 2) + 16 * c + e) * 128 + row];
+            if (two_parts) x[e] = f0 * x[e] + f1 * other[(16 * c + e) * 128 + row];
           }
           if (parts) {
-            constexpr int kAtOnce = D / 64;  // sixteens of columns that D bytes hold in fp32
+            constexpr int kAtOnce = D / 32;  // sixteens of columns that 2 D bytes hold in fp32
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              staged((c % kAtOnce) * 4 + q, {__float_as_uint(x[4 * q]), __float_as_uint(x[4 * q + 1]),
-                                             __float_as_uint(x[4 * q + 2]), __float_as_uint(x[4 * q + 3])});
-            if (c % kAtOnce == kAtOnce - 1)
-              store(reinterpret_cast<char*>(p.part), 4, hf * (D / 2) + 16 * (c - kAtOnce + 1));
+              staged((c % kAtOnce) * 4 + q, __float_as_uint(x[4 * q]), __float_as_uint(x[4 * q + 1]), __float_as_uint(x[4 * q + 2]),
+                     __float_as_uint(x[4 * q + 3]));
+            if (c % kAtOnce == kAtOnce - 1) store(reinterpret_cast<char*>(p.part), 4, 16 * (c - kAtOnce + 1));
           } else {
+            uint32_t y[8];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t y[4];
-#pragma unroll
-              for (int a = 0; a < 4; ++a) {
-                const float u0 = x[8 * q + 2 * a], u1 = x[8 * q + 2 * a + 1];
-                const __nv_bfloat162 b2v = __floats2bfloat162_rn(inv == 0.f ? 0.f : u0 * inv, inv == 0.f ? 0.f : u1 * inv);
-                y[a] = *reinterpret_cast<const uint32_t*>(&b2v);
-              }
-              staged(2 * c + q, y);
+            for (int e = 0; e < 8; ++e) {
+              const __nv_bfloat162 pair =
+                  __floats2bfloat162_rn(inv == 0.f ? 0.f : x[2 * e] * inv, inv == 0.f ? 0.f : x[2 * e + 1] * inv);
+              y[e] = *reinterpret_cast<const uint32_t*>(&pair);
             }
-            if (c == D / 32 - 1) store(reinterpret_cast<char*>(p.out), 2, hf * (D / 2));
+            staged(2 * c, y[0], y[1], y[2], y[3]);
+            staged(2 * c + 1, y[4], y[5], y[6], y[7]);
+            if (c == D / 16 - 1) store(reinterpret_cast<char*>(p.out), 2, 0);
           }
         }
       }
