@@ -36,10 +36,13 @@ template <int D>
 struct Geo {
   static constexpr int kTile = kKeys * D * 2;                 // K (or V) of a block
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kStages = D == 128 ? 6 : 12;
+  static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kJoin = kStages * kStage;              // the warps' 16 x D sums, joined here
   static constexpr int kPitch = D + 4;                        // floats from row to row there: rows start in different banks
-  static constexpr int kBar = kJoin + kWarps * kRows * kPitch * 4;
+  static constexpr int kQ = kJoin + kWarps * kRows * kPitch * 4;  // two tiles of sixteen rows of q
+  static constexpr int kQPitch = 2 * D + 16;                  // bytes, for the same reason
+  static constexpr int kQTile = kRows * kQPitch;
+  static constexpr int kBar = kQ + 2 * kQTile;
   static constexpr int kSmem = kBar + 1024 + 1024;            // barriers, statistics; room to align to 1024
 };
 
@@ -71,33 +74,42 @@ __device__ __forceinline__ Visible sequence_rows(const FewRows& p, const Told& t
   v.first = t.first;
   v.rows = t.rows;
   v.set<kKeys>(p.mask, t.len, p.c.width << p.c.page_shift);
-  v.rows = v.first < 0 ? 0 : max(0, min(min(v.rows, min(p.max_tokens, kRows / p.rep)), p.T - v.first));
+  v.rows = v.first < 0 ? 0 : max(0, min(min(v.rows, p.max_tokens), p.T - v.first));
   v.count = v.rows == 0 ? 0 : max(1, v.count);
   return v;
 }
 // The first query head of tile h of a sequence, and its rows.
-__device__ __forceinline__ int first_head(const FewRows& p, int h) { return h / p.groups * p.rep_all + h % p.groups * kRows; }
+__device__ __forceinline__ int kv_head(const FewRows& p, int h) { return p.groups == 1 ? h : h / p.groups; }
+__device__ __forceinline__ int group(const FewRows& p, int h) { return p.groups == 1 ? 0 : h % p.groups; }
+__device__ __forceinline__ int first_head(const FewRows& p, int h) { return kv_head(p, h) * p.rep_all + group(p, h) * kRows; }
 __device__ __forceinline__ int tile_rows(const FewRows& p, const Visible& v, int h) {
-  return v.rows * min(p.rep, p.rep_all - h % p.groups * kRows);
+  return v.rows * min(p.rep, p.rep_all - group(p, h) * kRows);
 }
-// The sequences as a warp sees them, 32 at a time, one to a lane; the first 32 are kept.  The whole warp asks.
+__device__ __forceinline__ int token_of(const FewRows& p, int row) { return p.max_tokens == 1 ? 0 : row / p.rep; }
+// The sequences as a warp sees them, 32 at a time, one to a lane.  What the device says of the first 32 is kept, and the blocks of
+// the first 128.  The whole warp asks.
 struct Sequences {
+  static constexpr int kKept = 4;
   Told kept;
-  int kept_n;  // this lane's blocks of a KV head
-  unsigned total;  // blocks of all sequences and KV heads
+  unsigned kept_n[kKept];  // this lane's blocks of a KV head
+  unsigned total;          // blocks of all sequences and KV heads
   __device__ __forceinline__ Sequences(const FewRows& p) {
     const int lane = threadIdx.x & 31;
+    Told t[kKept];
+#pragma unroll
+    for (int c = 0; c < kKept; ++c)  // (all on their way before the first is looked at)
+      if (32 * c + lane < p.c.B) t[c] = told(p, 32 * c + lane);
     unsigned sum = 0;
-    for (int b0 = 0; b0 < p.c.B; b0 += 32) {
-      Told t{};
-      int n = 0;
-      if (b0 + lane < p.c.B) {
-        t = told(p, b0 + lane);
-        n = sequence_rows(p, t).count;
-      }
-      if (b0 == 0) kept = t, kept_n = n;
-      sum += __reduce_add_sync(0xffffffffu, (unsigned)n);
+#pragma unroll
+    for (int c = 0; c < kKept; ++c) {
+      kept_n[c] = 0;
+      if (32 * c >= p.c.B) continue;
+      if (32 * c + lane < p.c.B) kept_n[c] = sequence_rows(p, t[c]).count;
+      sum += __reduce_add_sync(0xffffffffu, kept_n[c]);
     }
+    kept = t[0];
+    for (int b0 = 32 * kKept; b0 < p.c.B; b0 += 32)
+      sum += __reduce_add_sync(0xffffffffu, b0 + lane < p.c.B ? (unsigned)sequence_rows(p, told(p, b0 + lane)).count : 0u);
     total = sum * p.heads;
   }
   __device__ __forceinline__ Visible rows(const FewRows& p, int b) const {
@@ -116,10 +128,10 @@ struct Sequences {
   __device__ __forceinline__ int add_up(const FewRows& p, unsigned stop, int upto, unsigned* before) const {
     const int lane = threadIdx.x & 31;
     unsigned sum = 0;
-    for (int b0 = 0; b0 < upto; b0 += 32) {
-      const int b = b0 + lane;
-      const unsigned n = b >= upto ? 0 : b0 == 0 ? kept_n : sequence_rows(p, told(p, b)).count;
-      unsigned x = n;
+    int found = -1;
+    auto chunk = [&](int b0, unsigned n) {
+      unsigned x = b0 + lane < upto ? n : 0;
+      n = x;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
@@ -128,13 +140,19 @@ struct Sequences {
       const unsigned beyond = __ballot_sync(0xffffffffu, (sum + x) * p.heads > stop);
       if (beyond != 0) {
         const int l = __ffs(beyond) - 1;
-        *before = sum + __shfl_sync(0xffffffffu, x - n, l);
-        return b0 + l;
+        sum += __shfl_sync(0xffffffffu, x - n, l);
+        found = b0 + l;
+      } else {
+        sum += __shfl_sync(0xffffffffu, x, 31);
       }
-      sum += __shfl_sync(0xffffffffu, x, 31);
-    }
+    };
+#pragma unroll
+    for (int c = 0; c < kKept; ++c)
+      if (found < 0 && 32 * c < upto) chunk(32 * c, kept_n[c]);
+    for (int b0 = 32 * kKept; b0 < upto && found < 0; b0 += 32)
+      chunk(b0, b0 + lane < upto ? sequence_rows(p, told(p, b0 + lane)).count : 0);
     *before = sum;
-    return upto;
+    return found < 0 ? upto : found;
   }
 };
 
@@ -182,8 +200,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   unsigned char* gen = raw + (base - smem_u32(raw));
   const uint32_t bar_full = base + geo::kBar, bar_empty = bar_full + 8 * geo::kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + geo::kBar + 16 * geo::kStages);
-  volatile unsigned* present = reinterpret_cast<volatile unsigned*>(gen + geo::kBar + 16 * geo::kStages + 8);  // [kStages]
+  const uint32_t bar_q = bar_empty + 8 * geo::kStages;  // [2] there, [2] free
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + geo::kBar + 16 * geo::kStages + 32);
+  volatile unsigned* present = reinterpret_cast<volatile unsigned*>(gen + geo::kBar + 16 * geo::kStages + 40);  // [kStages]
   float* s_m = reinterpret_cast<float*>(gen + geo::kBar + 256 + 4 * 16);  // [kWarps][kRows] maxima, then sums
   float* s_l = s_m + kWarps * kRows;
   float* s_o = reinterpret_cast<float*>(gen + geo::kJoin);                // [kWarps][kRows][kPitch]
@@ -194,6 +213,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < geo::kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, kWarps);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar_q + 8 * s, 1);
+      mbar_init(bar_q + 16 + 8 * s, kWarps);
     }
     fence_mbar_init();
     tma_prefetch_desc(&tmap_k);
@@ -224,13 +247,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       return page_at(p.c, p.c.table + w.b * p.c.table_stride, p.c.width, key >> p.c.page_shift);
     };
     int page = page_of(w), s = 0;
-    uint32_t ph = 0;
+    uint32_t ph = 0, items = 0;
+    bool fresh = true;  // the run's, or a tile's, first block: its rows of q are brought too, one to a lane
     for (unsigned u = u0; u < u1; ++u) {
       Walk next = w;
       int page_next = 0;
       if (u + 1 < u1) {  // (the next block's table entries are on their way while this one's slot is waited for)
         next.next(p, all);
         page_next = page_of(next);
+      }
+      if (fresh) {
+        const uint32_t slot = items & 1;
+        const int rows = tile_rows(p, w.v, w.h), tok = token_of(p, lane);
+        mbar_wait(bar_q + 16 + 8 * slot, ((items >> 1) & 1) ^ 1, abort_flag);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(bar_q + 8 * slot, rows * 2 * D);
+        __syncwarp();
+        if (lane < rows)
+          bulk_g2s(base + geo::kQ + slot * geo::kQTile + lane * geo::kQPitch,
+                   p.q + (long long)(w.v.first + tok) * p.q_stride + (first_head(p, w.h) + lane - tok * p.rep) * D, 2 * D,
+                   bar_q + 8 * slot);
+        ++items;
       }
       mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
       __syncwarp();
@@ -244,9 +281,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int key = w.v.block(w.i) * kKeys + bx * box_rows;
         // (a page that is not there: a coordinate behind the last one, for which the load brings zeros)
         tma_load_4d(base + s * geo::kStage + which * geo::kTile + half * (kKeys * 128) + bx * box_rows * 128,
-                    which ? &tmap_v : &tmap_k, half * 64, key & (p.c.page - 1), w.h / p.groups, page < 0 ? p.c.n_pages : page,
+                    which ? &tmap_v : &tmap_k, half * 64, key & (p.c.page - 1), kv_head(p, w.h), page < 0 ? p.c.n_pages : page,
                     bar_full + 8 * s);
       }
+      fresh = next.b != w.b || next.h != w.h;
       w = next;
       page = page_next;
       if (++s == geo::kStages) { s = 0; ph ^= 1; }
@@ -260,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int key_lane = 16 * warp + (lane >> 4) * 8 + (lane & 7);      // K: this lane's row for ldmatrix, chunk (lane >> 3) & 1
   const int val_lane = 16 * warp + ((lane >> 3) & 1) * 8 + (lane & 7);  // V, transposed: row; chunk lane >> 4
   int s = 0;
-  uint32_t ph = 0;
+  uint32_t ph = 0, items = 0;
   unsigned u = u0;
   while (u < u1) {
     // ---- one sequence and KV head, or what of them this run holds
@@ -271,15 +309,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t qf[D / 16][4];
     int pos[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + 8 * r, tok = row / p.rep;
-      pos[r] = min(v.pmin + tok, v.pmax);
-      const __nv_bfloat16* q = p.q + (long long)(v.first + tok) * p.q_stride + (head0 + row - tok * p.rep) * D + 2 * quad;
+    for (int r = 0; r < 2; ++r) pos[r] = min(v.pmin + token_of(p, g + 8 * r), v.pmax);
+    {
+      const uint32_t slot = items & 1, tile = base + geo::kQ + slot * geo::kQTile;
+      mbar_wait(bar_q + 8 * slot, (items >> 1) & 1, abort_flag);
+      __syncwarp();
+      // (rows that do not exist hold anything: a row of the product has nothing of the others)
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        qf[kk][r] = row < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + 16 * kk)) : 0;
-        qf[kk][2 + r] = row < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + 16 * kk + 8)) : 0;
-      }
+      for (int kk = 0; kk < D / 16; ++kk)
+        ldmatrix4(tile + ((lane & 7) + ((lane >> 3) & 1) * 8) * geo::kQPitch + 32 * kk + (lane >> 4) * 16, qf[kk]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q + 16 + 8 * slot);
+      ++items;
     }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
 #pragma unroll
@@ -412,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         acc.w += f * t.w;
       }
       if (final) {
-        const int tok = row / p.rep;
+        const int tok = token_of(p, row);
         const float inv = ll == 0.f ? 0.f : 1.f / ll;  // 0: the row sees nothing
         *reinterpret_cast<uint2*>(p.out + (long long)(v.first + tok) * p.out_stride + (head0 + row - tok * p.rep) * D + d) =
             make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
@@ -432,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- joining parts
-// One CTA per row and KV head of a sequence; D threads.  The parts are taken in the order of their keys.
+// One CTA per tile of a sequence, a warp to a row.
 struct JoinArgs {
   FewRows own;                    // the sequences' own keys
   int prefix_kind;                // 0: none, 1: the same kernel over the prefix, 2: the kernel for many rows
@@ -465,87 +506,41 @@ struct FewParts {
   }
 };
 
-constexpr int kMostParts = 1024;  // a tile's: one from each CTA that shares it, of the prefix and of its own keys
-
 template <int D>
-__global__ void __launch_bounds__(D) join_kernel(const JoinArgs a) {
-  __shared__ float s_w[kMostParts];
-  __shared__ float s_x[2][D / 32];
+__global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
   const FewRows& p = a.own;
-  const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, row = blockIdx.y, d = threadIdx.x;
+  const int b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads, lane = threadIdx.x & 31;
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   const Sequences all(p);
   const Visible v = all.rows(p, b);
-  if (row >= tile_rows(p, v, h)) return;
+  const int rows = tile_rows(p, v, h);
+  if (rows == 0) return;
   const FewParts own(p, all, v, b, h);
   if (own.n == 1 && a.prefix_kind == 0) return;  // written by its one CTA
   // the prefix's parts in front, then its own: which rows of which arrays
-  int n_pre = 0, pre_rows = 1;
-  long long pre0 = 0;
-  const float2* pre_stat = nullptr;
-  const float* pre_part = nullptr;
+  int n_pre = 0;
   FewParts pre = own;
   if (a.prefix_kind == 1) {
     const Sequences one(a.prefix);
     pre = FewParts(a.prefix, one, one.rows(a.prefix, 0), 0, h);
     n_pre = pre.n;
-    pre_rows = kRows;
-    pre0 = b * p.rep + row;
-    pre_stat = a.prefix.stat;
-    pre_part = a.prefix.part;
   } else if (a.prefix_kind == 2) {
-    const int r = b * p.rep_all + (h % p.groups) * kRows + row;
     n_pre = a.many_splits;
-    pre_rows = 128;
-    pre0 = ((long long)(h / p.groups) * a.many_tiles + r / 128) * a.many_splits * 128 + r % 128;
-    pre_stat = a.many_stat;
-    pre_part = a.many_part;
   }
-  const int n = n_pre + own.n;
-  auto at = [&](int i) { return i < n_pre ? pre0 + (a.prefix_kind == 1 ? pre.slot(i) : i) * pre_rows : own.slot(i - n_pre) * kRows + row; };
-  // ---- every part's weight, a thread to a part
-  float m = -INFINITY;
-  for (int i = d; i < n; i += D) {
-    const float2 st = __ldcg((i < n_pre ? pre_stat : p.stat) + at(i));
-    m = fmaxf(m, st.x);
+  for (int row = threadIdx.x >> 5; row < rows; row += 8) {
+    const int r = b * p.rep_all + group(p, h) * kRows + row;  // of the prefix's rows
+    const long long pre0 = ((long long)kv_head(p, h) * a.many_tiles + r / 128) * a.many_splits * 128 + r % 128;
+    Row<D> out;
+    out.join(
+        n_pre + own.n, lane, [&](int i) {
+          return i >= n_pre            ? Part{p.stat, p.part, own.slot(i - n_pre) * kRows + row}
+                 : a.prefix_kind == 1 ? Part{a.prefix.stat, a.prefix.part, pre.slot(i) * kRows + r}
+                                      : Part{a.many_stat, a.many_part, pre0 + i * 128};
+        });
+    const int tok = token_of(p, row);
+    out.store(p.out + (long long)(v.first + tok) * p.out_stride + (first_head(p, h) + row - tok * p.rep) * D, lane);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((d & 31) == 0) s_x[0][d >> 5] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < D / 32; ++w) m = fmaxf(m, s_x[0][w]);
-  float l = 0.f;
-  for (int i = d; i < n; i += D) {
-    const float2 st = __ldcg((i < n_pre ? pre_stat : p.stat) + at(i));
-    const float f = st.y == 0.f ? 0.f : st.x == m ? 1.f : ex2(st.x - m);
-    s_w[i] = f;
-    l += f * st.y;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  if ((d & 31) == 0) s_x[1][d >> 5] = l;
-  __syncthreads();
-  l = 0.f;
-#pragma unroll
-  for (int w = 0; w < D / 32; ++w) l += s_x[1][w];
-  // ---- the parts' rows, sixteen on their way at a time, added up in their order
-  float o = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 16) {
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      x[i] = i0 + i < n ? __ldcg((i0 + i < n_pre ? pre_part : p.part) + at(i0 + i) * D + d) : 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float f = i0 + i < n ? s_w[i0 + i] : 0.f;
-      if (f != 0.f) o += f * x[i];
-    }
-  }
-  const int tok = row / p.rep;
-  p.out[(long long)(v.first + tok) * p.out_stride + (first_head(p, h) + row - tok * p.rep) * D + d] =
-      __float2bfloat16(l == 0.f ? 0.f : o / l);
 }
 
 // ---------------------------------------------------------------- host
@@ -567,7 +562,7 @@ FewRows few_rows(const void* q, long long q_stride, const PagedCache& c, const i
                  void* out, long long out_stride, void* parts, long long slots, int n_cta, int T, int max_tokens) {
   FewRows p{};
   p.T = T;
-  p.max_tokens = max_tokens;
+  p.max_tokens = std::min(max_tokens, std::max(1, kRows / rep));
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_stride = q_stride;
   p.out = static_cast<__nv_bfloat16*>(out);
@@ -587,8 +582,8 @@ FewRows few_rows(const void* q, long long q_stride, const PagedCache& c, const i
 }
 
 int join(const JoinArgs& a, int rows, cudaStream_t s) {
-  const dim3 grid((unsigned)(a.own.c.B * a.own.heads), (unsigned)std::min(rows, kRows));
-  return a.own.c.D == 64 ? launch_pdl(join_kernel<64>, grid, 64, 0, s, a) : launch_pdl(join_kernel<128>, grid, 128, 0, s, a);
+  return launch_pdl(a.own.c.D == 64 ? join_kernel<64> : join_kernel<128>, dim3((unsigned)(a.own.c.B * a.own.heads)),
+                    32 * std::min(rows, 8), 0, s, a);
 }
 
 int check_rows(const void* q, long long q_stride, const PagedCache& c, int T, int Hq, float scale, const void* out,
@@ -615,7 +610,7 @@ bool paged_tensor_maps(const PagedCache& c, int block, CUtensorMap* k, CUtensorM
 namespace {
 
 // How the kernel for many rows cuts a call up: tiles of 128 rows, two to a CTA where sequences have more; CTAs that would leave
-// SMs idle share the keys of a tile, down to four blocks of 128 each.
+// SMs idle share the keys of a tile, down to two blocks of 128 each.
 struct ManyPlan {
   int two, slots, splits;
 };
@@ -626,7 +621,7 @@ ManyPlan many_plan(long long rows, int B, long long most_rows, int Hk, long long
   const long long tiles = std::min(rows / size + B, B * ((most_rows + size - 1) / size));  // no fewer than there are
   const long long likely = std::max<long long>(1, std::max((rows + size - 1) / size, tiles - B / 2));
   m.slots = (int)(m.two ? 2 * tiles : tiles);
-  m.splits = (int)std::max<long long>(1, std::min<long long>(sm_count / (likely * Hk), most_keys / 512));
+  m.splits = (int)std::max<long long>(1, std::min<long long>(sm_count / (likely * Hk), most_keys / 256));
   return m;
 }
 size_t many_bytes(const ManyPlan& m, int Hk, int D) { return part_bytes((long long)m.slots * Hk * m.splits, 128, D); }

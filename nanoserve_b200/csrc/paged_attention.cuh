@@ -90,6 +90,70 @@ int launch_pdl(void (*kernel)(Args...), dim3 grid, int block, size_t smem, cudaS
   return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Parts of a row joined by a warp, in the order of their keys: a lane holds D / 32 columns of the row.
+struct Part {
+  const float2* stat;  // maximum (in powers of two) and sum
+  const float* sums;   // D to a row
+  long long at;        // row
+};
+template <int D>
+struct Row {
+  static constexpr int E = D / 32;
+  float l = 0.f, o[E] = {};
+  template <typename F>
+  __device__ __forceinline__ void join(int n, int lane, F part) {
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) {
+      const Part x = part(i);
+      m = fmaxf(m, __ldcg(x.stat + x.at).x);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float2 st = make_float2(-INFINITY, 0.f);
+      if (i0 + lane < n) {
+        const Part x = part(i0 + lane);
+        st = __ldcg(x.stat + x.at);
+      }
+      const float f = st.y == 0.f ? 0.f : st.x == m ? 1.f : ex2(st.x - m);
+      l += f * st.y;
+      const int here = min(32, n - i0);
+      for (int i1 = 0; i1 < here; i1 += 8) {  // eight on their way at a time
+        float x[8][E];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const Part y = part(i0 + min(i1 + i, here - 1));
+          const float* src = y.sums + y.at * D + lane * E;
+          if constexpr (E == 4) {
+            const float4 z = __ldcg(reinterpret_cast<const float4*>(src));
+            x[i][0] = z.x, x[i][1] = z.y, x[i][2] = z.z, x[i][3] = z.w;
+          } else {
+            const float2 z = __ldcg(reinterpret_cast<const float2*>(src));
+            x[i][0] = z.x, x[i][1] = z.y;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float g = __shfl_sync(0xffffffffu, f, (i1 + i) & 31);
+          if (i1 + i < here && g != 0.f) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += g * x[i][e];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* to, int lane) const {  // a sum of 0: the row sees nothing
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      *reinterpret_cast<__nv_bfloat162*>(to + lane * E + e) =
+          __floats2bfloat162_rn(inv == 0.f ? 0.f : o[e] * inv, inv == 0.f ? 0.f : o[e + 1] * inv);
+  }
+};
+
 // Tensor maps of K and V: boxes of 64 elements of min(page, block) tokens of one head of one page.
 bool paged_tensor_maps(const PagedCache& c, int block, CUtensorMap* k, CUtensorMap* v);
 

@@ -621,60 +621,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0 && *abort_flag && p.status) atomicCAS(p.status, 0, kStatusGemmTimeout);
 }
 
-// Splits of the keys joined, in their order: a warp per row of a tile of 128, a lane per split and then per D / 32 columns.
+// Splits of the keys joined: sixteen rows of a tile of 128 to a CTA, four to a warp.
 template <int D>
 __global__ void __launch_bounds__(128) join_many_kernel(const ManyRows p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, h = blockIdx.x / p.slots, slot = blockIdx.x % p.slots;
+  const int lane = threadIdx.x & 31, h = blockIdx.x / p.slots, slot = blockIdx.x - h * p.slots;
   pdl_wait_prior_grid();
   pdl_launch_dependents();
-  const int size = p.two ? 256 : 128;
+  const int size = p.two ? 256 : 128, off = p.two ? 128 * (slot & 1) : 0, row0 = blockIdx.y * 16 + (threadIdx.x >> 5) * 4;
   Tile tl;
   if (!tl.find(p, size, p.two ? slot >> 1 : slot)) return;
-  const int off = p.two ? 128 * (slot & 1) : 0, row = blockIdx.y * 4 + (threadIdx.x >> 5), r = tl.r0 + off + row;
-  if (off + row >= tl.v.rows) return;
-  const long long at = ((long long)h * p.slots + slot) * p.splits * 128 + row;
-  float m = -INFINITY, l = 0.f, o[E] = {};
-  for (int z = lane; z < p.splits; z += 32) m = fmaxf(m, __ldcg(&p.stat[at + z * 128].x));
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  for (int z0 = 0; z0 < p.splits; z0 += 32) {
-    const float2 st = z0 + lane < p.splits ? __ldcg(&p.stat[at + (z0 + lane) * 128]) : make_float2(-INFINITY, 0.f);
-    const float f = st.y == 0.f ? 0.f : st.x == m ? 1.f : ex2(st.x - m);
-    l += f * st.y;
-    const int n = min(32, p.splits - z0);
-    for (int z1 = 0; z1 < n; z1 += 8) {
-      float x[8][E];
-#pragma unroll
-      for (int z = 0; z < 8; ++z) {
-        const float* src = p.part + (at + (z0 + min(z1 + z, n - 1)) * 128) * D + lane * E;
-        if constexpr (E == 4) {
-          const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
-          x[z][0] = y.x, x[z][1] = y.y, x[z][2] = y.z, x[z][3] = y.w;
-        } else {
-          const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
-          x[z][0] = y.x, x[z][1] = y.y;
-        }
-      }
-#pragma unroll
-      for (int z = 0; z < 8; ++z) {
-        const float g = __shfl_sync(0xffffffffu, f, (z1 + z) & 31);
-        if (z1 + z < n && g != 0.f) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += g * x[z][e];
-        }
-      }
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int row = row0 + i, r = tl.r0 + off + row;
+    if (off + row >= tl.v.rows) return;
+    const long long at = ((long long)h * p.slots + slot) * p.splits * 128 + row;
+    Row<D> out;
+    out.join(p.splits, lane, [&](int z) { return Part{p.stat, p.part, at + z * 128}; });
+    const int tok = r / p.rep;
+    out.store(p.out + (long long)(tl.v.first + tok) * p.out_stride + (h * p.rep + r - tok * p.rep) * D, lane);
   }
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int tok = r / p.rep;
-  __nv_bfloat162* out = reinterpret_cast<__nv_bfloat162*>(p.out + (long long)(tl.v.first + tok) * p.out_stride +
-                                                          (h * p.rep + r - tok * p.rep) * D + lane * E);
-#pragma unroll
-  for (int e = 0; e < E; e += 2)
-    out[e / 2] = inv == 0.f ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(o[e] * inv, o[e + 1] * inv);
 }
 
 template <int D, bool TWO>
@@ -695,7 +660,7 @@ int many_rows_launch(const ManyRows& p, cudaStream_t s) {
   return p.two ? launch<128, true>(p, s) : launch<128, false>(p, s);
 }
 int join_many_launch(const ManyRows& p, cudaStream_t s) {
-  const dim3 grid((unsigned)(p.slots * p.c.Hk), 32);
+  const dim3 grid((unsigned)(p.slots * p.c.Hk), 8);
   return launch_pdl(p.c.D == 64 ? join_many_kernel<64> : join_many_kernel<128>, grid, 128, 0, s, p);
 }
 
