@@ -17,6 +17,7 @@
 // end of a run.
 #include <algorithm>
 #include <cfloat>
+#include <cmath>
 
 #include "paged_attention.cuh"
 #include "paged_rows.cuh"
@@ -610,18 +611,25 @@ bool paged_tensor_maps(const PagedCache& c, int block, CUtensorMap* k, CUtensorM
 namespace {
 
 // How the kernel for many rows cuts a call up: tiles of 128 rows, two to a CTA where sequences have more; CTAs that would leave
-// SMs idle share the keys of a tile, down to two blocks of 128 each.
+// SMs idle share the keys of a tile, down to two blocks of 128 each.  Where single tiles just fill the SMs, or over half of them,
+// they are a CTA's each: it then works on two blocks of keys at a time, which two CTAs would have to join (three chunks of
+// 150 to 517 tokens, 16 / 2 heads of 64: XX us against YY).
 struct ManyPlan {
   int two, slots, splits;
 };
 ManyPlan many_plan(long long rows, int B, long long most_rows, int Hk, long long most_keys, int sm_count) {
   ManyPlan m;
-  m.two = most_rows > 128;
-  const int size = m.two ? 256 : 128;
-  const long long tiles = std::min(rows / size + B, B * ((most_rows + size - 1) / size));  // no fewer than there are
-  const long long likely = std::max<long long>(1, std::max((rows + size - 1) / size, tiles - B / 2));
+  long long tiles = 0, likely = 0;
+  for (m.two = 0;; m.two = 1) {
+    const int size = m.two ? 256 : 128;
+    tiles = std::min(rows / size + B, B * ((most_rows + size - 1) / size));  // no fewer than there are
+    likely = std::max<long long>(1, std::max((rows + size - 1) / size, tiles - B / 2));
+    if (m.two || most_rows <= 128 || (likely * Hk <= sm_count && 2 * likely * Hk > sm_count)) break;
+  }
   m.slots = (int)(m.two ? 2 * tiles : tiles);
-  m.splits = (int)std::max<long long>(1, std::min<long long>(sm_count / (likely * Hk), most_keys / 256));
+  // (a step over a tile's blocks takes some 1.9 us, a part 0.15 us in the join: the sum is least where steps and parts balance)
+  const long long balance = (long long)std::sqrt((m.two ? 12.0 : 6.0) * (double)(most_keys / 128));
+  m.splits = (int)std::max<long long>(1, std::min({sm_count / (likely * Hk), most_keys / 256, balance}));
   return m;
 }
 size_t many_bytes(const ManyPlan& m, int Hk, int D) { return part_bytes((long long)m.slots * Hk * m.splits, 128, D); }

@@ -103,17 +103,30 @@ struct Row {
   template <typename F>
   __device__ __forceinline__ void join(int n, int lane, F part) {
     float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) {
+    float2 kept[2];  // of the first 64 parts
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      kept[c] = make_float2(-INFINITY, 0.f);
+      if (32 * c + lane < n) {
+        const Part x = part(32 * c + lane);
+        kept[c] = __ldcg(x.stat + x.at);
+      }
+    }
+    for (int i = 64 + lane; i < n; i += 32) {
       const Part x = part(i);
       m = fmaxf(m, __ldcg(x.stat + x.at).x);
     }
+    m = fmaxf(m, fmaxf(kept[0].x, kept[1].x));
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
     for (int i0 = 0; i0 < n; i0 += 32) {
-      float2 st = make_float2(-INFINITY, 0.f);
-      if (i0 + lane < n) {
-        const Part x = part(i0 + lane);
-        st = __ldcg(x.stat + x.at);
+      float2 st = i0 == 0 ? kept[0] : kept[1];
+      if (i0 >= 64) {
+        st = make_float2(-INFINITY, 0.f);
+        if (i0 + lane < n) {
+          const Part x = part(i0 + lane);
+          st = __ldcg(x.stat + x.at);
+        }
       }
       const float f = st.y == 0.f ? 0.f : st.x == m ? 1.f : ex2(st.x - m);
       l += f * st.y;
