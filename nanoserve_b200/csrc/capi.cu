@@ -404,8 +404,10 @@ int b2_paged_kv_append(const void* qkv, long long qkv_stride, const void* bias, 
                        long long q_stride, const b2_paged_cache* cache, const void* cu_tokens, int T, int Hq, void* stream) {
   b2::PagedCache c;
   if (const int bad = to_paged(cache, &c)) return bad;
+  int rc = 0;
+  const int sms = sm_count_of_device(&rc);  // (what is wrong with the arguments comes before what is wrong with the device)
   return b2::paged_append_launch(qkv, qkv_stride, bias, inv_freq, q_out, q_stride, c, static_cast<const int*>(cu_tokens), T,
-                                 Hq, static_cast<cudaStream_t>(stream));
+                                 Hq, rc ? -rc : sms, static_cast<cudaStream_t>(stream));
 }
 
 size_t b2_paged_attention_workspace_bytes(int T, int n_seqs, int max_tokens, int Hq, int Hk, int D) {
@@ -421,7 +423,7 @@ int b2_paged_attention(const void* q, long long q_stride, const b2_paged_cache* 
   b2::PagedCache c;
   if (const int bad = to_paged(cache, &c)) return bad;
   int rc = 0;
-  const int sms = sm_count_of_device(&rc);  // (what is wrong with the arguments comes before what is wrong with the device)
+  const int sms = sm_count_of_device(&rc);
   return b2::paged_attention_launch(q, q_stride, c, static_cast<const int*>(cu_tokens), T, max_tokens, Hq, window, sinks,
                                     scale, out, out_stride, workspace, workspace_bytes, rc ? -rc : sms, static_cast<cudaStream_t>(stream));
 }

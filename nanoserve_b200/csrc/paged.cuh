@@ -9,42 +9,36 @@ namespace b2 {
 
 inline bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
-// Everything that another kernel of the stream may have written is read through L2: under a programmatic launch the L1 may
-// hold an older line.
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
-  const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
-  uint4 u;
-  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-  *reinterpret_cast<uint4*>(p) = u;
-}
+// (Everything that another kernel of the stream may have written is read through L2, __ldcg: under a programmatic launch the L1 may
+// hold an older line.)
 
-// The sequence that row t belongs to and its first row (the whole warp asks, with one t); -1 behind the last sequence.
-// Without cu_tokens every sequence has one row.
-__device__ __forceinline__ int sequence_of(const int* cu_tokens, int B, int t, int* first) {
-  *first = t;
-  if (cu_tokens == nullptr) return t < B ? t : -1;
-  const int lane = threadIdx.x & 31;
-  int before = 0, start = 0;  // sequences that end at or before row t, and the end of the last of them
-  for (int b0 = 0; b0 < B; b0 += 32) {
-    const int end = b0 + lane < B ? __ldcg(cu_tokens + b0 + lane + 1) : 0x7fffffff;
-    const unsigned done = __ballot_sync(0xffffffffu, end <= t);
-    if (done != 0) start = __shfl_sync(0xffffffffu, end, 31 - __clz(done));
-    before += __popc(done);
-    if (done != 0xffffffffu) break;
+// The sequence that row t belongs to, its first row, its rows and its length (the whole warp asks, with one t); -1 behind the last
+// sequence or in front of the first.  Without cu_tokens every sequence has one row.
+__device__ __forceinline__ int sequence_of(const int* cu_tokens, const PagedCache& c, int t, int* first, int* n_new, int* len) {
+  if (cu_tokens == nullptr) {
+    *first = t;
+    *n_new = 1;
+    *len = t < c.B ? __ldcg(c.lens + t) : 0;
+    return t < c.B ? t : -1;
   }
-  if (before >= B) return -1;
-  *first = before == 0 ? __ldcg(cu_tokens) : start;
-  return t < *first ? -1 : before;
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < c.B; b0 += 32) {
+    int begin = 0, end = -1, n = 0;
+    if (b0 + lane < c.B) {
+      begin = __ldcg(cu_tokens + b0 + lane);
+      end = __ldcg(cu_tokens + b0 + lane + 1);
+      n = __ldcg(c.lens + b0 + lane);
+    }
+    const unsigned has = __ballot_sync(0xffffffffu, begin <= t && t < end);
+    if (has != 0) {
+      const int l = __ffs(has) - 1;
+      *first = __shfl_sync(0xffffffffu, begin, l);
+      *n_new = __shfl_sync(0xffffffffu, end, l) - *first;
+      *len = __shfl_sync(0xffffffffu, n, l);
+      return b0 + l;
+    }
+  }
+  return -1;
 }
 
 // The page that holds token `col` * page of a table's sequence, -1 where there is none.

@@ -32,9 +32,10 @@ struct Sampling {
   long long* tokens;
 };
 
-int paged_append_launch(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq, void* q_out,
-                        long long q_stride, const PagedCache& c, const int* cu_tokens, int T, int Hq, cudaStream_t s);
 // sm_count below 1: minus the error that the device gave, returned once the arguments are found right.
+int paged_append_launch(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq, void* q_out,
+                        long long q_stride, const PagedCache& c, const int* cu_tokens, int T, int Hq, int sm_count,
+                        cudaStream_t s);
 int paged_attention_launch(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int T,
                            int max_tokens, int Hq, int window, int sinks, float scale, void* out, long long out_stride,
                            void* workspace, size_t workspace_bytes, int sm_count, cudaStream_t s);

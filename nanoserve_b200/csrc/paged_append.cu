@@ -5,81 +5,157 @@
 //
 // in 32 bits with one rounding to bf16 at the store.  The angle is formed and reduced to [-pi, pi] in 64 bits: in 32 bits the
 // product alone is off by 2^-24 of itself, 0.004 radians at position 65536.
-#include "paged.h"
-#include "paged.cuh"
+//
+// Bound by memory.  A thread moves eight (i, i + D/2) pairs of one head, two rows at a time, for rows the grid's length apart: while
+// its loads are on their way, a thread makes an angle of the next rows and a warp finds where the rows behind those belong, so that
+// nothing waits for the chain of row, sequence, page and angle (8065 rows of 28 / 4 heads of 128: 41 us with a CTA to a row and
+// its loads behind the chain, 30 us so).
+#include <algorithm>
+
+#include "paged_attention.cuh"
+#include "ptx.cuh"
 #include "w4_internal.h"
 
 namespace b2 {
 namespace {
 
 constexpr int kMaxHalf = 128;  // D / 2
+constexpr int kMostThreads = 320;  // three CTAs to an SM at up to 64 registers
 
-// One CTA per row.  Bound by memory; one thread moves eight (i, i + D/2) pairs of a head.
-__global__ void __launch_bounds__(256) paged_append_kernel(const __nv_bfloat16* qkv, long long qkv_stride,
-                                                           const __nv_bfloat16* bias, const float* inv_freq,
-                                                           __nv_bfloat16* q_out, long long q_stride, PagedCache c,
-                                                           const int* cu_tokens, int Hq) {
-  __shared__ float s_cos[kMaxHalf], s_sin[kMaxHalf];
-  const int t = blockIdx.x, D = c.D, heads = Hq + 2 * c.Hk;
-  int first;
-  const int b = sequence_of(cu_tokens, c.B, t, &first);
-  if (b < 0) return;
-  const int n_new = cu_tokens ? __ldcg(cu_tokens + b + 1) - first : 1;
-  const int pos = __ldcg(c.lens + b) - n_new + (t - first);
-  if (pos < 0) return;  // the sequence has no place for this row
-  for (int i = threadIdx.x; i < D / 2; i += blockDim.x) rotation(pos, __ldcg(inv_freq + i), &s_sin[i], &s_cos[i]);
-  const int col = pos >> c.page_shift;
-  const int page = col < c.width ? __ldcg(c.table + b * c.table_stride + col) : -1;
-  const bool stored = page >= 0 && page < c.n_pages;
-  const long long at = (long long)page * c.page_stride + (long long)(pos & (c.page - 1)) * c.token_stride;
-  __syncthreads();
-  const int per_head = D / 16;
-  for (int u = threadIdx.x; u < heads * per_head; u += blockDim.x) {
-    const int h = u / per_head, e0 = (u - h * per_head) * 8;
-    if (h >= Hq && !stored) continue;
-    const __nv_bfloat16* src = qkv + t * qkv_stride + (long long)h * D;
-    float lo[8], hi[8], f[8];
-    load8(src + e0, lo);
-    load8(src + D / 2 + e0, hi);
-    if (bias != nullptr) {
-      load8(bias + h * D + e0, f);
+struct Place {
+  int pos;       // of the row in its sequence; negative: there is none, and nothing of the row is written
+  int stored;    // its page is there
+  long long at;  // where in the caches, without the head
+};
+
+__device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+__device__ __forceinline__ float2 pair_of(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t pack_pair(float2 x) {
+  const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+template <int R>
+__global__ void __launch_bounds__(kMostThreads, 3) paged_append_kernel(const __nv_bfloat16* qkv, long long qkv_stride,
+                                                                    const __nv_bfloat16* bias, const float* inv_freq,
+                                                                    __nv_bfloat16* q_out, long long q_stride, PagedCache c,
+                                                                    const int* cu_tokens, int T, int Hq) {
+  __shared__ alignas(8) float s_cos[2][R][kMaxHalf], s_sin[2][R][kMaxHalf];
+  __shared__ Place s_place[3][R];
+  const int D = c.D, half = D / 2, per_head = D / 16, units = (Hq + 2 * c.Hk) * per_head, groups = (T + R - 1) / R;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int u = blockIdx.y * blockDim.x + threadIdx.x, h = u / per_head, e0 = (u - h * per_head) * 8;
+  pdl_wait_prior_grid();
+  pdl_launch_dependents();
+  const float freq0 = (int)threadIdx.x < R * half ? __ldcg(inv_freq + threadIdx.x % half) : 0.f;  // of this thread's first angle
+  auto load = [&](int g, uint4 (&x)[R][2]) {
+    if (u >= units || g >= groups) return;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] += f[e];
-      load8(bias + h * D + D / 2 + e0, f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) hi[e] += f[e];
+    for (int r = 0; r < R; ++r) {
+      const __nv_bfloat16* src = qkv + (long long)min(g * R + r, T - 1) * qkv_stride + (long long)h * D + e0;
+      x[r][0] = __ldcg(reinterpret_cast<const uint4*>(src));
+      x[r][1] = __ldcg(reinterpret_cast<const uint4*>(src + half));
     }
-    if (h < Hq + c.Hk) {
+  };
+  auto find = [&](int g, int r, Place* to) {
+    const int t = g * R + r;
+    int first = 0, n_new = 1, len = 0;
+    const int b = t < T ? sequence_of(cu_tokens, c, t, &first, &n_new, &len) : -1;
+    Place at{-1, 0, 0};
+    if (b >= 0) {
+      at.pos = len - n_new + (t - first);
+      const int page = at.pos < 0 ? -1 : page_at(c, c.table + b * c.table_stride, c.width, at.pos >> c.page_shift);
+      at.stored = page >= 0;
+      at.at = (long long)page * c.page_stride + (long long)(at.pos & (c.page - 1)) * c.token_stride;
+    }
+    if (lane == 0) to[r] = at;
+  };
+  auto turn = [&](const Place* of, int to) {
+    for (int i = threadIdx.x; i < R * half; i += blockDim.x) {
+      const int r = i / half, f = i - r * half;
+      const float freq = i == (int)threadIdx.x ? freq0 : __ldcg(inv_freq + f);
+      if (of[r].pos >= 0) rotation(of[r].pos, freq, &s_sin[to][r][f], &s_cos[to][r][f]);
+    }
+  };
+  const int g0 = blockIdx.x, step = gridDim.x;
+  uint4 x[R][2], add[2] = {};
+  load(g0, x);
+  if (bias != nullptr && u < units) {
+    add[0] = __ldcg(reinterpret_cast<const uint4*>(bias + h * D + e0));
+    add[1] = __ldcg(reinterpret_cast<const uint4*>(bias + h * D + half + e0));
+  }
+  if (warp < R) find(g0, warp, s_place[0]);
+  if (warp >= R && warp < 2 * R) find(g0 + step, warp - R, s_place[1]);
+  __syncthreads();
+  turn(s_place[0], 0);
+  __syncthreads();
+  int now = 0, place = 0;
+  for (int g = g0; g < groups; g += step) {
+    if (g != g0) load(g, x);
+    const int place1 = place == 2 ? 0 : place + 1, place2 = place1 == 2 ? 0 : place1 + 1;
+    if (g + step < groups) {
+      turn(s_place[place1], now ^ 1);
+      const int last = (int)(blockDim.x >> 5) - 1 - warp;  // (the warps that are not the first to make angles)
+      if (last < R) find(g + 2 * step, last, s_place[place2]);
+    }
+    if (u < units) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = lo[e], bb = hi[e], cs = s_cos[e0 + e], sn = s_sin[e0 + e];
-        lo[e] = a * cs - bb * sn;
-        hi[e] = bb * cs + a * sn;
+      for (int r = 0; r < R; ++r) {
+        const Place at = s_place[place][r];
+        if (at.pos < 0 || (h >= Hq && !at.stored)) continue;
+        const bool turned = h < Hq + c.Hk;
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {  // two pairs at a time
+          float2 a = pair_of(word(x[r][0], w)), b = pair_of(word(x[r][1], w));
+          a = add_f32x2(a, pair_of(word(add[0], w)));
+          b = add_f32x2(b, pair_of(word(add[1], w)));
+          if (turned) {
+            const float2 cs = *reinterpret_cast<const float2*>(&s_cos[now][r][e0 + 2 * w]);
+            const float2 sn = *reinterpret_cast<const float2*>(&s_sin[now][r][e0 + 2 * w]);
+            const float2 y = make_float2(a.x * cs.x - b.x * sn.x, a.y * cs.y - b.y * sn.y);
+            b = make_float2(b.x * cs.x + a.x * sn.x, b.y * cs.y + a.y * sn.y);
+            a = y;
+          }
+          lo[w] = pack_pair(a);
+          hi[w] = pack_pair(b);
+        }
+        __nv_bfloat16* dst = h < Hq          ? q_out + (long long)(g * R + r) * q_stride + (long long)h * D
+                             : h < Hq + c.Hk ? c.k + at.at + (h - Hq) * c.head_stride
+                                             : c.v + at.at + (h - Hq - c.Hk) * c.head_stride;
+        *reinterpret_cast<uint4*>(dst + e0) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4*>(dst + half + e0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       }
     }
-    __nv_bfloat16* dst = h < Hq          ? q_out + t * q_stride + (long long)h * D
-                         : h < Hq + c.Hk ? c.k + at + (h - Hq) * c.head_stride
-                                         : c.v + at + (h - Hq - c.Hk) * c.head_stride;
-    store8(dst + e0, lo);
-    store8(dst + D / 2 + e0, hi);
+    __syncthreads();
+    now ^= 1;
+    place = place1;
   }
 }
 
 }  // namespace
 
 int paged_append_launch(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq, void* q_out,
-                        long long q_stride, const PagedCache& c, const int* cu_tokens, int T, int Hq, cudaStream_t s) {
-  const int heads = Hq + 2 * c.Hk;
+                        long long q_stride, const PagedCache& c, const int* cu_tokens, int T, int Hq, int sm_count,
+                        cudaStream_t s) {
+  const long long heads = (long long)Hq + 2 * c.Hk;
   if (T < 1 || Hq < 1 || (!cu_tokens && T != c.B)) return kErrBadShape;
-  if (qkv_stride < (long long)heads * c.D || qkv_stride % 8 || q_stride < (long long)Hq * c.D || q_stride % 8)
-    return kErrBadShape;
+  if (qkv_stride < heads * c.D || qkv_stride % 8 || q_stride < (long long)Hq * c.D || q_stride % 8) return kErrBadShape;
   if (!qkv || !inv_freq || !q_out || misaligned(qkv, 16) || misaligned(bias, 16) || misaligned(q_out, 16) ||
       misaligned(inv_freq, 4) || misaligned(cu_tokens, 4))
     return kErrBadPointer;
-  paged_append_kernel<<<T, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(qkv), qkv_stride,
-                                        static_cast<const __nv_bfloat16*>(bias), static_cast<const float*>(inv_freq),
-                                        static_cast<__nv_bfloat16*>(q_out), q_stride, c, cu_tokens, Hq);
-  return (int)cudaGetLastError();
+  if (heads * c.D > (1 << 24)) return kErrTooLarge;
+  if (sm_count < 1) return -sm_count;
+  // a unit to a thread; where there are more, they are cut into as few and as equal parts as fit
+  const int units = (int)heads * (c.D / 16), parts = (units + kMostThreads - 1) / kMostThreads;
+  const int threads = std::max(128, ((units + parts - 1) / parts + 31) / 32 * 32);
+  const bool two = T >= 2 * sm_count;
+  const int groups = two ? (T + 1) / 2 : T, resident = std::max(1, sm_count * std::max(1, 3 * kMostThreads / threads) / parts);
+  return launch_pdl(two ? paged_append_kernel<2> : paged_append_kernel<1>, dim3(std::min(groups, resident), parts), threads, 0, s,
+                    static_cast<const __nv_bfloat16*>(qkv), qkv_stride, static_cast<const __nv_bfloat16*>(bias),
+                    static_cast<const float*>(inv_freq), static_cast<__nv_bfloat16*>(q_out), q_stride, c, cu_tokens, T, Hq);
 }
 
 }  // namespace b2

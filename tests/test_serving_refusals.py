@@ -167,4 +167,4 @@ def test_no_page_number_is_used_unseen():
             found += 1
             after = text[m.start():m.start() + 400]
             assert re.search(r"page < c\.n_pages|page >= c\.n_pages|< \(unsigned\)\w*\.?\w*n_pages|valid_page\(", after), (f, after[:120])
-    assert found >= 2
+    assert found >= 1
