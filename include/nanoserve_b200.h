@@ -351,10 +351,13 @@ int b2_tp_wait(const void* wait_sig, const void* epoch, unsigned wait_per_epoch,
  *     qkv is not modified.  A row whose position is negative is left out.  head_dim % 16 == 0, at most 256.
  *   b2_paged_attention: out [T, Hq D] = softmax(scale q K^T) V; the row at position i sees the keys j <= i of its sequence and, with
  *     window > 0, of those only j > i - window and the first `sinks`.  A row that sees no key is zero.  head_dim 64 or 128,
- *     Hq % Hk == 0, 0 < scale < infinity.  max_tokens: no sequence has more rows than that (rows beyond it are left as they are).
+ *     Hq % Hk == 0, 0 < scale < 2^127.  max_tokens: no sequence has more rows than that (rows beyond it are left as they are).
  *   b2_shared_prefix_attention: one row per sequence, which sees the first *prefix_len (int32, on the device) tokens of the pages
  *     prefix_table [prefix_width], and all seq_lens[b] tokens (which may be none) of its own pages.  The prefix's keys and values
  *     are read once for all sequences.
+ *   Both: what no row of a call sees (slots behind a sequence's end, keys in front of every row's window) may hold anything.  A value
+ *   (of v) that is infinite or not a number reaches the rows that see its key and, with several rows per sequence, may reach others
+ *   of the same sequence.  T * Hq < 2^30, and (n_seqs + blocks of 64 keys that the tables hold) * Hq < 2^31.
  *   Both take device scratch of the caller's, 16-byte aligned, of at least the bytes that the two size calls give, contents
  *   undefined before and after; calls that may overlap in time need scratch of their own.
  *

@@ -65,12 +65,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x for x <= 128, two at a time, to 2^-18: x = n + f with |f| <= 1/2 (n + 127 lands in the low bits of a sum with 1.5 * 2^23), a
-// polynomial of fourth degree in f (least largest relative error), times 2^n.  0 from -127 down; not a number stays that.
+// 2^x, two at a time, to 2^-18: x = n + f with |f| <= 1/2 (n + 127 lands in the low bits of a sum with 1.5 * 2^23), a
+// polynomial of fourth degree in f (least largest relative error), times 2^n.  0 from -127 down, infinity from 128 up; not a number
+// stays that.
 __device__ __forceinline__ float2 ex2_pair(float2 x) {
   constexpr float kMagic = 12582912.f + 127.f;
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;\n\tmin.NaN.f32 %0, %0, %2;" : "+f"(x.x) : "f"(-127.f), "f"(128.f));
+  asm("max.NaN.f32 %0, %0, %1;\n\tmin.NaN.f32 %0, %0, %2;" : "+f"(x.y) : "f"(-127.f), "f"(128.f));
   auto both = [](float v) { return make_float2(v, v); };
   const float2 t = add_f32x2(x, both(kMagic)), n = add_f32x2(t, both(-kMagic));
   const float2 f = fma_f32x2(n, both(-1.f), x);
@@ -500,8 +501,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             mine = sum[0].x + sum[0].y;
           };
           weigh();
-          if (__any_sync(0xffffffffu, !(mine < 1152921504606846976.f))) {  // 2^60, or not a number
-            const float mn = fmaxf(m, largest()), corr = m == mn ? 1.f : ex2(m - mn);
+          const bool large = !(mine < 1152921504606846976.f);  // 2^60, or not a number
+          if (__any_sync(0xffffffffu, large)) {  // (rows that are not large keep their reference, and with it their bits)
+            const float mx = largest(), mn = large ? fmaxf(m, mx) : m, corr = m == mn ? 1.f : ex2(m - mn);
             if (half == 1) {  // the first half's product has to be done before O is rescaled
               mbar_wait(bar_h + 8 * t, parity, abort_flag);
               __syncwarp();

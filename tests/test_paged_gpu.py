@@ -166,6 +166,25 @@ def test_attention_large_scores_and_scale(kernels):
             check(attend(kernels, b, cu_tokens=b.cu, window=128, sinks=2, scale=scale), ref, tol)
 
 
+@pytest.mark.parametrize("new", [[1, 1], [64, 200]])
+def test_one_key_far_above_the_others(kernels, new):
+    """One key, at every place of a block in turn, whose scores are hundreds of powers of two above all others: it takes all."""
+    b = Batch(new, [400, 600], 2, 1, 64, 128, seed=14)
+    q = torch.zeros_like(b.q.view(b.T, 2, 64))
+    q[..., 0] = 30.0  # rows score the keys' first column alone
+    b.q = q.view(b.T, -1)
+    plain_k = b.cache_k.clone()
+    for j in list(range(130, 258)):
+        b.cache_k = plain_k.clone()
+        for i in range(2):
+            b.cache_k[int(b.table[i, j // 128]), :, j % 128, 0] = 20.0
+        out = attend(kernels, b, cu_tokens=b.cu, scale=1.0).view(b.T, 2, 64)
+        for i in range(2):
+            v = b.cache_v[int(b.table[i, j // 128]), 0, j % 128]
+            rows = slice(b.starts[i], b.starts[i] + new[i])
+            assert ((out[rows].float() - v.float()).abs() <= BF16_STEP * v.float().abs()).all(), (j, i)
+
+
 def test_attention_strided_rows(kernels):
     """q as a view of the projection's rows, out as a view of a wider buffer."""
     for new in ([1, 1, 1], [30, 1, 100]):
@@ -178,6 +197,70 @@ def test_attention_strided_rows(kernels):
         ref, tol = paged_reference(b)
         check(out[:, :1024], ref, tol)
         assert (out[:, 1024:] == 7.0).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 40, 200]])
+def test_attention_of_rows_that_are_not_numbers(kernels, new):
+    """A row of q that holds a nan, or an infinity against finite keys, is not a number; no other row notices."""
+    b = Batch(new, [100, 300, 500], 14, 2, 128, 32, seed=8)
+    want = attend(kernels, b, cu_tokens=b.cu)
+    row = new[0] + new[1] - 1  # the second sequence's last
+    b.q[row, 5 * 128 + 3] = float("nan")
+    b.q[row, 9 * 128 + 7] = float("inf")
+    got = attend(kernels, b, cu_tokens=b.cu).view(b.T, 14, 128)
+    hit = torch.zeros(b.T, 14, dtype=torch.bool, device="cuda")
+    hit[row, 5] = hit[row, 9] = True
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], want.view(b.T, 14, 128)[~hit])
+
+
+@pytest.mark.parametrize("new,most", [([2, 1, 2], 1), ([5, 300, 20], 16), ([300, 20, 700], 130)])
+def test_rows_in_front_of_the_first_and_beyond_max_tokens(kernels, new, most):
+    b = Batch(new, [400, 700, 900], 7, 1, 64, 64, seed=10, extra_rows=1)
+    ref, tol = paged_reference(b)
+    start = 4  # rows in front of the first sequence
+    b.q = torch.cat([b.q.new_full((start, 7 * 64), 5.0), b.q])
+    b.cu, b.T = b.cu + start, b.T + start
+    out = attend(kernels, b, cu_tokens=b.cu, max_tokens=most)
+    kept = torch.zeros(b.T, dtype=torch.bool, device="cuda")
+    for n, s in zip(new, b.starts):
+        kept[start + s:start + s + min(n, most)] = True
+    check(out[kept], ref[kept[start:]], tol[kept[start:]])
+    assert (out[~kept] == 7.0).all()
+    q_out = torch.full((b.T, 7 * 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    kernels.paged_kv_append(torch.ones(b.T, 9 * 64, dtype=torch.bfloat16, device="cuda"), None, torch.zeros(32, device="cuda"),
+                            b.cache_k, b.cache_v, b.table, b.seq_lens, 7, 1, 64, cu_tokens=b.cu, q_out=q_out)
+    assert (q_out[:start] == 7.0).all() and (q_out[start:-1] == 1.0).all() and (q_out[-1:] == 7.0).all()
+
+
+def test_long_sequences_split_over_many_ctas(kernels):
+    """One sequence whose keys all SMs share, for few rows and for many; a short chunk behind a long context."""
+    for new, window in ((1, 0), (2, 0), (64, 0), (64, 30000)):
+        b = Batch([new], [70001], 4, 1, 64, 256, seed=12)
+        ref, tol = paged_reference(b, window, 5)
+        check(attend(kernels, b, cu_tokens=b.cu, window=window, sinks=5), ref, tol)
+
+
+def test_many_sequences(kernels):
+    """More sequences than a warp has lanes, than lengths are kept, empty ones among them."""
+    for B in (33, 129, 300):
+        g = torch.Generator().manual_seed(B)
+        lens = torch.randint(0, 200, (B,), generator=g).tolist()
+        b = Batch([1] * B, lens, 4, 2, 64, 16, seed=B)
+        ref, tol = paged_reference(b)
+        check(attend(kernels, b), ref, tol)
+        new = torch.randint(0, 12, (B,), generator=g).tolist()
+        b = Batch(new, [n + x for n, x in zip(new, lens)], 4, 2, 64, 16, seed=B)
+        ref, tol = paged_reference(b)
+        check(attend(kernels, b, cu_tokens=b.cu), ref, tol)
+        check(attend(kernels, b, cu_tokens=b.cu, max_tokens=12), ref, tol)
+
+
+def test_output_in_place_of_q(kernels):
+    for new in ([1, 1], [70, 300]):
+        b = Batch(new, [500, 600], 8, 2, 128, 64, seed=13)
+        want = attend(kernels, b, cu_tokens=b.cu)
+        got = kernels.paged_attention(b.q, b.cache_k, b.cache_v, b.table, b.seq_lens, *b.heads, cu_tokens=b.cu, out=b.q)
+        assert torch.equal(got, want)
 
 
 # ---------------------------------------------------------------- shared prefix

@@ -91,6 +91,18 @@ def test_prefix(lib, kw, code):
     assert prefix(lib, cache(), **kw) == code
 
 
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("nan"), float("inf"), 3e38])
+def test_scales(lib, scale):
+    c = cache()
+    assert lib.b2_paged_attention(A, 28 * 128, c, None, 2, 1, 28, 0, 0, scale, A, 28 * 128, A, 1 << 40, None) == BAD_SHAPE
+    assert lib.b2_shared_prefix_attention(A, 28 * 128, c, A, 3, A, 28, scale, A, 28 * 128, A, 1 << 40, None) == BAD_SHAPE
+
+
+def test_sizes_beyond_31_bits(lib):
+    assert attend(lib, cache(n_seqs=1 << 26, table_stride=8), T=1 << 26) == TOO_LARGE
+    assert attend(lib, cache(n_seqs=1 << 20, table_width=1 << 14, table_stride=1 << 14), T=1 << 20) == TOO_LARGE
+
+
 def test_head_dims(lib):
     for D, both in ((96, BAD_SHAPE), (256, BAD_SHAPE), (80, BAD_SHAPE)):
         c = dict(head_dim=D, token_stride=D, head_stride=16 * D, page_stride=64 * D)
