@@ -732,6 +732,7 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
   pre.lens = prefix_len;
   pre.B = 1;
   JoinArgs a{};
+  int own_ctas = sm_count;
   if (c.B * rep <= kRows) {
     a.prefix_kind = 1;
     a.prefix = few_rows(q, q_stride, pre, nullptr, rep, scale_log2, out, out_stride, prefix_parts, 2LL * sm_count + c.Hk,
@@ -750,8 +751,12 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
     a.many_stat = p.stat;
     a.many_splits = m.splits;
     a.many_tiles = m.slots;
+    // Where the prefix leaves a third of the SMs or more, the own keys' kernel runs beside it, on those alone (8192 tokens, 16
+    // sequences of up to 512: XX us against YY with CTAs for all SMs, half of which waited for the prefix's to end).
+    const int left = sm_count - (m.two ? m.slots / 2 : m.slots) * c.Hk * m.splits;
+    if (left * 3 >= sm_count) own_ctas = left;
   }
-  a.own = few_rows(q, q_stride, c, nullptr, rep, scale_log2, out, out_stride, workspace, own_slots, sm_count, c.B, 1);
+  a.own = few_rows(q, q_stride, c, nullptr, rep, scale_log2, out, out_stride, workspace, own_slots, own_ctas, c.B, 1);
   a.own.mask = Mask{0, 0, 0};
   a.own.parts_only = 1;
   a.own.late_wait = 1;
