@@ -14,7 +14,7 @@
 // The reference m of a row's weights is its maximum over the first block that it sees something of.  After that no maximum is
 // taken: weights over 1 are as exact as others, in fp32 and in bf16 alike, and a block whose weights add up to over 2^10 raises m
 // by the sum's exponent, for the next one; O is then rescaled in tensor memory, between the products that use it.  Where half a
-// block adds up to over 2^60 (scores that jump by tens), m is taken anew at once, and that half's weights too.
+// block adds up to over 2^24 (scores that jump), m is taken anew at once, and that half's weights too: O stays under 2^25 |v|.
 // What bounds it: 128 x 128 scores take the tensor core 1024 cycles (both products) and the 16 exponentials per cycle of an SM
 // as long.  So an eighth of the exponentials are polynomials on the multiply-add pipes, pairs at a time, and the second product
 // starts when half of the weights are there.
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mine = sum[0].x + sum[0].y;
           };
           weigh();
-          const bool large = !(mine < 1152921504606846976.f);  // 2^60, or not a number
+          const bool large = !(mine < 16777216.f);  // 2^24, or not a number
           if (__any_sync(0xffffffffu, large)) {  // (rows that are not large keep their reference, and with it their bits)
             const float mx = largest(), mn = large ? fmaxf(m, mx) : m, corr = m == mn ? 1.f : ex2(m - mn);
             if (half == 1) {  // the first half's product has to be done before O is rescaled

@@ -410,3 +410,18 @@ def test_offsets_beyond_32_bits(kernels):
                                 cu_tokens=b.cu)
         assert torch.equal(cache_v[1, :, 119 - 64], qkv[-1].view(-1, D)[Hq + Hk:])
         assert torch.equal(cache_k[0, :, 59], qkv[new[0] - 1].view(-1, D)[Hq:Hq + Hk])
+
+
+@pytest.mark.parametrize("new", [[1, 1], [64, 200]])
+def test_large_values_under_a_jump_of_the_scores(kernels, new):
+    """Values of 2^85 and a key, behind the first blocks, whose weight is some 2^50 times theirs: the sums stay finite."""
+    b = Batch(new, [400, 600], 4, 2, 64, 64, seed=15)
+    q = torch.zeros(b.T, 4, 64, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 4.0  # rows score the keys' first column alone: up to some 4 * 4, and 12 * 4 at that key
+    b.q = q.view(b.T, -1)
+    for i in range(2):
+        b.cache_k[int(b.table[i, 200 // 64]), :, 200 % 64, 0] = 12.0
+    b.cache_v *= 2.0 ** 85
+    ref, tol = paged_reference(b, scale=1.0)
+    out = attend(kernels, b, cu_tokens=b.cu, scale=1.0)
+    check(out, ref, tol)
