@@ -32,6 +32,7 @@ class Batch:
         self.prefix_len = torch.zeros(1, dtype=torch.int32, device=dev)
         self.lens = torch.zeros(n_seqs, dtype=torch.int32, device=dev)
         self.step_no = torch.zeros(1, dtype=torch.int64, device=dev)
+        self.left = 0  # steps that there is room for
         self.tokens = torch.zeros(max_own, n_seqs, dtype=torch.int64, device=dev)
         self.last = torch.zeros(n_seqs, dtype=torch.int64, device=dev)
         self.u = torch.zeros(max_own, n_seqs, device=dev)
@@ -85,6 +86,7 @@ class Batch:
             self.table = torch.cat([self.prefix_table[None].expand(self.B, -1), self.own_table], 1).contiguous()
         self.lens.copy_(torch.tensor([shared + x for x in n], dtype=torch.int32))
         self.step_no.zero_()
+        self.left = min(self.max_own - 1, self.own_table.shape[1] * self.page - max(n))
         ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
         if shared:
             cu, lens, table = ints(0, shared), ints(shared), self.prefix_table[None]
@@ -105,7 +107,11 @@ class Batch:
 
     @torch.no_grad()
     def step(self):
-        """The next token of every sequence (nothing of it on the host: it can be captured)."""
+        """The next token of every sequence (nothing of it on the host: it can be captured).  A row without a token (-1: its logits
+        were not numbers) goes on from token 0."""
+        if self.left < 1:
+            raise ValueError("no prefill, or no room for another token")
+        self.left -= 1
         self.lens += 1
         first = self.shared // self.page
         own_lens = self.lens - self.prefix_len
@@ -116,7 +122,7 @@ class Batch:
                 return self.k.paged_attention(q, self.cache_k[li], self.cache_v[li], self.table, self.lens, *self.heads)
             return self.k.shared_prefix_attention(q, self.cache_k[li], self.cache_v[li], self.prefix_table, self.prefix_len,
                                                   self.table[:, first:], own_lens, *self.heads)
-        self._pick(self._layers(F.embedding(self.last, self.r.embed), attend))
+        self._pick(self._layers(F.embedding(self.last.clamp(min=0), self.r.embed), attend))
 
     def generate(self, prefix: torch.Tensor, prompts: Sequence[torch.Tensor], n_new: int, temperature: float = 1.0, top_k: int = 0,
                  top_p: float = 1.0, min_p: float = 0.0, u: Optional[torch.Tensor] = None, seed: int = 0,
@@ -140,18 +146,20 @@ class Batch:
             self.u[:n_new].copy_(u)
             self.prefill(prefix, prompts)
             if use_graph and self.graph is None and n_new > 1:
-                lens, step_no, last = self.lens.clone(), self.step_no.clone(), self.last.clone()
+                lens, step_no, last, left = self.lens.clone(), self.step_no.clone(), self.last.clone(), self.left
                 self.step()  # (warms what the capture needs; its token is drawn again)
                 torch.cuda.synchronize()
                 graph = torch.cuda.CUDAGraph()
+                self.left = left
                 with torch.cuda.graph(graph, stream=stream):
                     self.step()
-                self.graph = graph
+                self.graph, self.left = graph, left
                 self.lens.copy_(lens)
                 self.step_no.copy_(step_no)
                 self.last.copy_(last)
             for _ in range(n_new - 1):
                 if use_graph:
+                    self.left -= 1
                     self.graph.replay()
                 else:
                     self.step()

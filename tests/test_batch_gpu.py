@@ -147,3 +147,39 @@ def test_refusals(runner):
         b.generate(ids(10, 1), [ids(120, 2)] * 2, 20)
     with pytest.raises(ValueError):
         b.generate(ids(0, 1), [ids(1, 2), ids(0, 3)], 2)
+
+
+def test_rows_without_a_token_go_on(runner):
+    """-1 (a row whose logits were not numbers) is no row of the embedding: such a sequence goes on from token 0."""
+    b = Batch(runner, 3, 64, 8, page=16)
+    b.u.fill_(0.5)
+    b.prefill(ids(40, 1), [ids(3, 2 + i) for i in range(3)])
+    lens, step_no = b.lens.clone(), b.step_no.clone()
+    b.last[1] = 0
+    b.step()
+    want = b.tokens[1].tolist()
+    b.lens.copy_(lens)
+    b.step_no.copy_(step_no)
+    b.last.copy_(b.tokens[0])
+    b.last[1] = -1
+    b.step()
+    assert b.tokens[1].tolist() == want
+    torch.cuda.synchronize()
+
+
+def test_steps_end_with_the_room(runner):
+    b = Batch(runner, 2, 64, 4, page=16)
+    with pytest.raises(ValueError):
+        b.step()
+    b.prefill(ids(40, 1), [ids(3, 2), ids(1, 3)])
+    for _ in range(3):
+        b.step()
+    with pytest.raises(ValueError):  # (four tokens are drawn)
+        b.step()
+    b.prefill(ids(33, 1), [ids(18, 2), ids(1, 3)])  # 19 of a sequence's 32 slots are taken, one token is drawn
+    assert b.left == 3
+    b.generate(ids(40, 1), [ids(3, 2), ids(1, 3)], 4)
+    assert b.left == 0
+    b.prefill(ids(33, 1), [ids(31, 2), ids(1, 3)])  # (32 of 32)
+    with pytest.raises(ValueError):
+        b.step()
