@@ -1,6 +1,7 @@
-// The host side of ops.Kernels.w4_linear and w4_quantize, and of the operators of batched serving, as one native call each.  Through ctypes an eager one-token call spent
-// more time in Python (argument conversion, torch.empty with keywords, the tensors' properties) than its launch takes; here the
-// same steps run on the tensors' C++ objects (512 x 3584 at one token 8.6 -> 4.8 us a call).
+// The host side of ops.Kernels.w4_linear and w4_quantize, and of the operators of batched serving, as one native call each.
+// Through ctypes an eager one-token call spent more time in Python (argument conversion, torch.empty with keywords, the tensors'
+// properties) than its launch takes; here the same steps run on the tensors' C++ objects (512 x 3584 at one token 8.6 -> 4.8 us a
+// call).
 //
 // w4_linear(fn, x, Wq, S, group, flags, out): `fn` is the address of b2_w4_linear in whatever library the caller has loaded.
 // w4_quantize(fn, W, group): likewise of ns_w4_quantize.  paged_kv_append, paged_attention, shared_prefix_attention and sample
@@ -271,7 +272,7 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NOTIMPLEMENTED;
   const at::Tensor &q = tensor(a[2]), &table = tensor(a[5]), &len = tensor(a[6]);
   const int64_t width = (int64_t)Hq * D;
-  if (!is_rows(q, c.n_seqs, width) || table.dim() != 1 || table.size(0) > INT32_MAX || !is_vector(table, at::kInt, table.size(0)) ||
+  if (c.n_seqs < 1 || !is_rows(q, c.n_seqs, width) || table.dim() != 1 || table.size(0) > INT32_MAX || !is_vector(table, at::kInt, table.size(0)) ||
       len.scalar_type() != at::kInt || len.numel() != 1 || (a[13] != Py_None && !is_rows(tensor(a[13]), c.n_seqs, width)))
     Py_RETURN_NOTIMPLEMENTED;
   const auto fn = reinterpret_cast<decltype(&b2_shared_prefix_attention)>(PyLong_AsVoidPtr(a[0]));

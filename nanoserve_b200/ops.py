@@ -522,6 +522,8 @@ class Kernels:
             out = torch.empty((q.shape[0], n_heads * head_dim), dtype=q.dtype, device=q.device)
         else:
             self._rows(what, out, n_heads * head_dim, None, c.n_seqs)
+        if not c.n_seqs:
+            return out
         n = self.lib.b2_shared_prefix_workspace_bytes(c.n_seqs, n_heads, n_kv_heads, head_dim)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         rc = self.lib.b2_shared_prefix_attention(q.data_ptr(), q.stride(0), ctypes.byref(c), prefix_table.data_ptr(),

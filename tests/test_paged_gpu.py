@@ -425,3 +425,67 @@ def test_large_values_under_a_jump_of_the_scores(kernels, new):
     ref, tol = paged_reference(b, scale=1.0)
     out = attend(kernels, b, cu_tokens=b.cu, scale=1.0)
     check(out, ref, tol)
+
+
+def test_no_sequence(kernels):
+    """A call without sequences answers with nothing."""
+    b = Batch([1, 1], [20, 30], 4, 2, 64, 16, seed=16)
+    none = lambda t: t[:0]
+    plen = torch.tensor([16], dtype=torch.int32, device="cuda")
+    args = (b.cache_k, b.cache_v, b.table[0], plen, none(b.table), none(b.seq_lens), *b.heads)
+    assert kernels.shared_prefix_attention(none(b.q), *args).shape == (0, 4 * 64)
+    args = (b.cache_k, b.cache_v, none(b.table), none(b.seq_lens), *b.heads)
+    assert kernels.paged_attention(none(b.q), *args).shape == (0, 4 * 64)
+    qkv = torch.zeros(0, 8 * 64, dtype=torch.bfloat16, device="cuda")
+    assert kernels.paged_kv_append(qkv, None, torch.zeros(32, device="cuda"), *args).shape == (0, 4 * 64)
+
+
+def test_many_rows_and_prefixes_on_streams_and_in_graphs(kernels):
+    """Prompts, split prompts and shared prefixes: two streams that overlap, and two graphs of each, replayed in turn on two
+    streams with other lengths than at their capture, give the bits of single calls."""
+    prompts = [Batch([300, 1, 64], [300, 900 + i, 5000], 28, 4, 128, 64, seed=30 + i) for i in range(2)]
+    tails = [Batch([0] + [1] * 20, [4000 + 64 * i] + [30 + i] * 20, 28, 4, 128, 64, seed=40 + i) for i in range(2)]
+    few = [Batch([0] + [1] * 2, [3000 + 64 * i] + [300, 20 + i], 14, 2, 64, 64, seed=50 + i) for i in range(2)]
+
+    def prompt(b):
+        return attend(kernels, b, cu_tokens=b.cu)
+
+    def prefix(b):
+        return kernels.shared_prefix_attention(b.q, b.cache_k, b.cache_v, b.table[0], b.seq_lens[:1], b.table[1:], b.seq_lens[1:],
+                                               *b.heads)
+
+    runs = [lambda i, f=f, bs=bs: f(bs[i]) for f, bs in ((prompt, prompts), (prefix, tails), (prefix, few))]
+    want = [[run(i) for i in range(2)] for run in runs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        for r, run in enumerate(runs):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got.append((r, i, run(i)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[r][i]) for r, i, o in got)
+    # captured with shorter lengths
+    batches, lens = [prompts, tails, few], [[b.seq_lens.clone() for b in bs] for bs in (prompts, tails, few)]
+    for bs in batches:
+        for b in bs:
+            b.seq_lens.copy_((b.seq_lens - 7).clamp(min=1))
+    graphs = []
+    torch.cuda.synchronize()
+    for r, run in enumerate(runs):
+        for i, s in enumerate(streams):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                out = run(i)
+            graphs.append((r, i, g, out))
+    for bs, ls in zip(batches, lens):
+        for b, n in zip(bs, ls):
+            b.seq_lens.copy_(n)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for r, i, g, _ in graphs:
+            with torch.cuda.stream(streams[i]):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[r][i]) for r, i, _, out in graphs)

@@ -1,6 +1,6 @@
-"""GPU tests of sampling against the definition in 64 bits: tokens are whole numbers and have to be equal.  A draw or a border
-closer to u (top_p) than the sums' precision could fall either way: the reference says how near the next border is, and rows
-where that is under 2^-30 of the total are drawn again (none are met here; weights are held to 2^-45)."""
+"""GPU tests of sampling against the definition in 64 bits: tokens are whole numbers and have to be equal.  (A draw or a border
+nearer to u or top_p of the sum than the weights' precision, 2^-44 of the largest each, could fall either way; the reference's own
+sums in 64 bits are no finer.  No row here comes that near.)"""
 import numpy as np
 import pytest
 import torch
@@ -142,3 +142,31 @@ def test_captured(kernels):
         g.replay()
         torch.cuda.synchronize()
         assert got.tolist() == both(kernels, x, v, 1.0, 50, 0.9).tolist()
+
+
+def test_streams_and_settings_that_are_no_numbers(kernels):
+    """Calls that overlap on two streams draw what single calls draw; settings that are not numbers, or infinite, are answered:
+    a temperature that is no positive number takes the largest logit, an infinite one draws evenly, other nans filter as 0."""
+    x = [rows(9, 50000, torch.bfloat16, seed=60 + i) for i in range(2)]
+    draw = lambda i, **kw: kernels.sample(*x[i], **kw)
+    ways = [dict(temperature=0.8), dict(top_k=50, top_p=0.9), dict(top_p=0.9, temperature=3.0)]
+    want = [[draw(i, **kw) for i in range(2)] for kw in ways]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        for w, kw in enumerate(ways):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got.append((w, i, draw(i, **kw)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want[w][i]) for w, i, t in got)
+    inf, nan = float("inf"), float("nan")
+    greedy = draw(0, temperature=0.0)
+    for kw in (dict(temperature=nan), dict(temperature=-1.0), dict(temperature=-inf), dict(top_p=nan), dict(top_p=-1.0)):
+        assert torch.equal(draw(0, **kw), greedy), kw
+    assert torch.equal(draw(0, min_p=nan), draw(0))
+    logits, u = rows(4, 1000, torch.float32, seed=70)
+    assert torch.equal(kernels.sample(logits, u, temperature=1e-45), logits.argmax(-1))  # (no two are equal)
+    logits[:, ::2] = -inf
+    assert torch.equal(kernels.sample(logits, u, temperature=inf), 2 * (u.double() * 500).long() + 1)
