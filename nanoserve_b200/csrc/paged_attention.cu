@@ -12,9 +12,14 @@
 // Few rows: the up to sixteen (token, query head) rows of a sequence that share a KV head are the M side of m16n8k16 products.
 // Work is counted in blocks of 64 keys over all sequences and KV heads, and every CTA takes an equal run of them, wherever
 // sequences begin and end: a batch of ragged lengths leaves no SM waiting for its longest member.  The lengths are on the
-// device, so every CTA adds them up for itself.  One warp keeps TMA loads of the pages' rows in flight (a ring of up to
-// 192 KB per SM); each of four warps takes sixteen keys of a block, with a maximum, sum and 16 x D of its own, joined at the
-// end of a run.
+// device, so every CTA adds them up for itself.  One warp keeps TMA loads of the pages' rows in flight (a ring of 160 KB per SM);
+// each of four warps takes sixteen keys of a block, with a maximum, sum and 16 x D of its own, joined at the end of a run.  Parts
+// of rows whose keys several CTAs shared go through device memory to join_kernel.
+//
+// Bound by the start and the end of a launch, then by memory: a block of 64 keys of 128 takes an SM 1240 cycles from shared memory
+// (at HBM's pace 32 KB take 1455), a launch some 7000 before the first block (lengths, tables, the first loads) and the join 2 to
+// 4 us behind it.  28 / 4 heads of 128: 16 sequences of 500 to 32767 tokens in a window of 4096, 22 us for 89 MB, 4.1 TB/s; the own
+// keys of 64 sequences behind a prefix, 34 us for 143 MB, 4.2 TB/s.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -613,7 +618,7 @@ namespace {
 // How the kernel for many rows cuts a call up: tiles of 128 rows, two to a CTA where sequences have more; CTAs that would leave
 // SMs idle share the keys of a tile, down to two blocks of 128 each.  Where single tiles just fill the SMs, or over half of them,
 // they are a CTA's each: it then works on two blocks of keys at a time, which two CTAs would have to join (three chunks of
-// 150 to 517 tokens, 16 / 2 heads of 64: XX us against YY).
+// 150 to 517 tokens, 16 / 2 heads of 64: 22 us against 30).
 struct ManyPlan {
   int two, slots, splits;
 };
@@ -752,7 +757,7 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
     a.many_splits = m.splits;
     a.many_tiles = m.slots;
     // Where the prefix leaves a third of the SMs or more, the own keys' kernel runs beside it, on those alone (8192 tokens, 16
-    // sequences of up to 512: XX us against YY with CTAs for all SMs, half of which waited for the prefix's to end).
+    // sequences of up to 512: 23 us against 27.5 with CTAs for all SMs, half of which waited for the prefix's to end).
     const int left = sm_count - (m.two ? m.slots / 2 : m.slots) * c.Hk * m.splits;
     if (left * 3 >= sm_count) own_ctas = left;
   }

@@ -15,9 +15,13 @@
 // taken: weights over 1 are as exact as others, in fp32 and in bf16 alike, and a block whose weights add up to over 2^10 raises m
 // by the sum's exponent, for the next one; O is then rescaled in tensor memory, between the products that use it.  Where half a
 // block adds up to over 2^24 (scores that jump), m is taken anew at once, and that half's weights too: O stays under 2^25 |v|.
-// What bounds it: 128 x 128 scores take the tensor core 1024 cycles (both products) and the 16 exponentials per cycle of an SM
-// as long.  So an eighth of the exponentials are polynomials on the multiply-add pipes, pairs at a time, and the second product
-// starts when half of the weights are there.
+// What bounds it: 128 x 128 scores of heads of 128 take the tensor core 1024 cycles (both products), and the 16 exponentials per
+// cycle of an SM as long.  An eighth of the exponentials are therefore polynomials on the multiply-add pipes, pairs at a time, and
+// the second product starts when half of the weights are there.  256 rows x 128 keys take 3300 cycles where the products alone would
+// take 2048: a tile's softmax waits some 1000 for its scores (behind the other tile's products), spends 1350 on the exponentials and
+// the rest on reading, masking and storing.  8192 new tokens in a window of 4096, 28 / 4 heads of 128: 353 us, 1020 TFLOP/s (a bf16
+// GEMM here: 1670), at the board's power limit.  Tried there: two threads to a row 388 us, so that rows of half the length leave room in registers;
+// every second, third or fourth pair a polynomial 413, 358 and 357 us.
 // Every wait is bounded; a time-out is recorded in the device's status word.
 #include <algorithm>
 
