@@ -10,7 +10,7 @@
 //   one tile         up to 128 rows: the two halves take blocks of keys in turn, and are joined at the end
 // warps 0-3 / 4-7   softmax of the first / second tile: one thread per row, 128 scores of it in registers
 // warp 8            loads: a ring of tiles of 128 keys (K, V in the order in which they are used), a page's rows per box
-// warp 9            issues the products (10, 11: nothing)
+// warp 9            issues the products; warps 10, 11 zero the values that no row sees
 // The reference m of a row's weights is its maximum over the first block that it sees something of.  After that no maximum is
 // taken: weights over 1 are as exact as others, in fp32 and in bf16 alike, and a block whose weights add up to over 2^10 raises m
 // by the sum's exponent, for the next one; O is then rescaled in tensor memory, between the products that use it.  Where half a
@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t bar_full = base + geo::kBar, bar_empty = bar_full + 8 * geo::kBufs;
   // bar_p: [half of the weights][tile]
   const uint32_t bar_s = bar_empty + 8 * geo::kBufs, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_h = bar_o + 16,
-                 bar_q = bar_h + 16;
-  unsigned char* misc = gen + geo::kBar + 16 * geo::kBufs + 88;
+                 bar_q = bar_h + 16, bar_z = bar_q + 8, bar_y = bar_z + 8 * geo::kBufs;
+  unsigned char* misc = gen + geo::kBar + 32 * geo::kBufs + 88;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 4);
   volatile unsigned* present = reinterpret_cast<volatile unsigned*>(misc + 8);  // [kPresent]
@@ -174,6 +174,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < geo::kBufs; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
+      mbar_init(bar_y + 8 * s, 1);  // values with some that no row sees are on their way
+      mbar_init(bar_z + 8 * s, 2);  // those are zeros
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(bar_s + 8 * t, 1);
@@ -210,170 +212,181 @@ __global__ void __launch_bounds__(kThreads, 1)
     n = (int)((long long)tl.v.count * (z + 1) / p.splits) - i0;
   }
   const Visible& v = tl.v;
+  // Whether some row sees each of a block's keys: blocks [seen0, seen1), and [0, sink1) of the first tokens'.
+  const int skip = v.n_sink - v.from - i0;  // block b of the keys is this CTA's i = b + skip
+  const int seen0 = max(v.n_sink - i0, (p.mask.window ? max(0, v.pmin - p.mask.window + kKeys) / kKeys : 0) + skip);
+  const int seen1 = max(0, min(v.end, v.pmax + 1)) / kKeys + skip;
+  const int sink1 = min(v.n_sink, p.mask.sinks / kKeys) - i0;
+  auto whole_block = [&](int i) { return (i >= seen0 && i < seen1) || i < sink1; };
 
   if (warp >= kLoadWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (exists && warp == kLoadWarp) {
-    // ------------------------------------------------------------ loads
-    const int box_rows = min(p.c.page, kKeys), boxes = kKeys / box_rows;
-    const int bx = lane % boxes, half = lane / boxes;
-    const int* table = p.c.table + b * p.c.table_stride;
-    // loads 0 .. kAhead - 1: K of these blocks; then V of block i, K of block i + kAhead, in turn
-    const int ahead = min(kAhead, n), total = 2 * n;
-    auto what = [&](int x, int* block) {
-      if (x < ahead) {
-        *block = x;
-        return 0;
-      }
-      const int y = x - ahead;
-      if (y < 2 * (n - ahead)) {
-        *block = (y >> 1) + ((y & 1) ? ahead : 0);
-        return (y & 1) ? 0 : 1;
-      }
-      *block = n - ahead + (y - 2 * (n - ahead));  // V of the last blocks
-      return 1;
-    };
-    auto page_of = [&](int x) {
-      int block;
-      what(x, &block);
-      return page_at(p.c, table, p.c.width, (v.block(i0 + block) * kKeys + bx * box_rows) >> p.c.page_shift);
-    };
-    int page = total > 0 ? page_of(0) : 0, s = 0;
-    uint32_t ph = 0;
-    for (int x = 0; x < total; ++x) {
-      const int page_next = x + 1 < total ? page_of(x + 1) : 0;
-      int block;
-      const int is_v = what(x, &block);
-      mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
-      __syncwarp();
-      const unsigned there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << boxes) - 1);
-      if (lane == 0) {
-        if (!is_v) present[block % kPresent] = there;
-        mbar_arrive_expect_tx(bar_full + 8 * s, geo::kTile);
-      }
-      __syncwarp();
-      if (half < kHalves)
-        tma_load_4d(ring + s * geo::kTile + half * (128 * 128) + bx * box_rows * 128, is_v ? &tmap_v : &tmap_k, half * 64,
-                    (v.block(i0 + block) * kKeys + bx * box_rows) & (p.c.page - 1), h, page < 0 ? p.c.n_pages : page,
-                    bar_full + 8 * s);
-      page = page_next;
-      if (++s == geo::kBufs) { s = 0; ph ^= 1; }
-    }
-  } else if (exists && warp == kMmaWarp) {
-    // ------------------------------------------------------------ products
-    constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128);
-    constexpr uint32_t idesc_o = umma_idesc_bf16(128, D) | (1u << 16);  // B along N as it lies
-    int s = 0;
-    uint32_t ph = 0;
-    auto scores = [&](int t, uint32_t buf) {
-      const uint64_t dq = umma_desc_k128(base + (TWO ? t * geo::kTile : 0)), dk = umma_desc_k128(buf);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        umma_f16_ss(tmem + 128 * t, dq + (kk >> 2) * ((128 * 128) >> 4) + 2 * (kk & 3),
-                    dk + (kk >> 2) * ((128 * 128) >> 4) + 2 * (kk & 3), idesc_s, kk > 0);
-      umma_commit(bar_s + 8 * t);
-    };
-    // (half of the keys)
-    auto values = [&](int t, int half, uint32_t buf, bool first) {
-      const uint64_t dv = desc_v(buf);
-#pragma unroll
-      for (int k4 = 0; k4 < kKeys / 32; ++k4) {
-        const int kk = half * (kKeys / 32) + k4;
-        umma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * kk, dv + kk * (2048 >> 4), idesc_o, !first || kk > 0);
-      }
-      if (half == 0) umma_commit(bar_h + 8 * t);
-    };
-    auto weights_of = [&](int t, int half, uint32_t parity) {
-      mbar_wait(bar_p + 16 * half + 8 * t, parity, abort_flag);
-      __syncwarp();
-      tc_fence_after_sync();
-    };
-    auto loaded = [&] {
-      mbar_wait(bar_full + 8 * s, ph, abort_flag);
-      __syncwarp();
-      tc_fence_after_sync();
-      return ring + s * geo::kTile;
-    };
-    auto used = [&] {  // (the elected lane): the buffer is free once what was issued is done
-      umma_commit(bar_empty + 8 * s);
-    };
-    auto step = [&] {
-      if (++s == geo::kBufs) { s = 0; ph ^= 1; }
-    };
-    if (n > 0) mbar_wait(bar_q, 0, abort_flag);
-    for (int i = 0; i < min(kAhead, n); ++i) {
-      const uint32_t buf = loaded();
-      if (elect_one()) {
-        scores(TWO ? 0 : i, buf);
-        if (TWO) scores(1, buf);
-        used();
-      }
-      __syncwarp();
-      step();
-    }
-    for (int i = 0; i < n; ++i) {
-      const uint32_t buf_v = loaded();
-      const int j0 = v.block(i0 + i) * kKeys;
-      // keys that no row sees may hold anything, and 0 times an infinity is none: their values become zeros
-      if (!(v.any(p.mask, j0) && v.any(p.mask, j0 + kKeys - 1) &&
-            (p.mask.window == 0 || j0 > v.pmin - p.mask.window || j0 + kKeys <= p.mask.sinks))) {
-        for (int x = lane; x < kKeys * kHalves * 8; x += 32) {
-          const int key = x / (kHalves * 8), half = x / 8 % kHalves;
-          if (!v.any(p.mask, j0 + key))
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(buf_v + half * (128 * 128) + key * 128 + (x & 7) * 16),
-                         "r"(0)
-                         : "memory");
+      // ------------------------------------------------------------ loads
+      const int box_rows = min(p.c.page, kKeys), boxes = kKeys / box_rows;
+      const int bx = lane % boxes, half = lane / boxes;
+      const int* table = p.c.table + b * p.c.table_stride;
+      // loads 0 .. kAhead - 1: K of these blocks; then V of block i, K of block i + kAhead, in turn
+      const int ahead = min(kAhead, n), total = 2 * n;
+      auto what = [&](int x, int* block) {
+        if (x < ahead) {
+          *block = x;
+          return 0;
         }
-        fence_proxy_async_smem();
+        const int y = x - ahead;
+        if (y < 2 * (n - ahead)) {
+          *block = (y >> 1) + ((y & 1) ? ahead : 0);
+          return (y & 1) ? 0 : 1;
+        }
+        *block = n - ahead + (y - 2 * (n - ahead));  // V of the last blocks
+        return 1;
+      };
+      auto page_of = [&](int x) {
+        int block;
+        what(x, &block);
+        return page_at(p.c, table, p.c.width, (v.block(i0 + block) * kKeys + bx * box_rows) >> p.c.page_shift);
+      };
+      int page = total > 0 ? page_of(0) : 0, s = 0;
+      uint32_t ph = 0;
+      for (int x = 0; x < total; ++x) {
+        const int page_next = x + 1 < total ? page_of(x + 1) : 0;
+        int block;
+        const int is_v = what(x, &block);
+        mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
         __syncwarp();
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << boxes) - 1);
+        if (lane == 0) {
+          if (!is_v) present[block % kPresent] = there;
+          if (is_v && !whole_block(block)) mbar_arrive(bar_y + 8 * s);
+          mbar_arrive_expect_tx(bar_full + 8 * s, geo::kTile);
+        }
+        __syncwarp();
+        if (half < kHalves)
+          tma_load_4d(ring + s * geo::kTile + half * (128 * 128) + bx * box_rows * 128, is_v ? &tmap_v : &tmap_k, half * 64,
+                      (v.block(i0 + block) * kKeys + bx * box_rows) & (p.c.page - 1), h, page < 0 ? p.c.n_pages : page,
+                      bar_full + 8 * s);
+        page = page_next;
+        if (++s == geo::kBufs) { s = 0; ph ^= 1; }
       }
-      const int s_v = s;
-      step();
-      if constexpr (TWO) {
-        uint32_t buf_k = 0;
+    } else if (exists && warp == kMmaWarp) {
+      // ------------------------------------------------------------ products (one thread)
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(128, D) | (1u << 16);  // B along N as it lies
+      if (elect_one()) {
+        int s = 0;
+        uint32_t ph = 0, ph_z = 0;
+        auto scores = [&](int t, uint32_t buf) {
+          const uint64_t dq = umma_desc_k128(base + (TWO ? t * geo::kTile : 0)), dk = umma_desc_k128(buf);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          weights_of(t, 0, i & 1);
-          if (elect_one()) values(t, 0, buf_v, i == 0);
-          __syncwarp();
-          if (t == 0 && i + 1 < n) buf_k = loaded();
-          weights_of(t, 1, i & 1);
-          if (elect_one()) {
-            values(t, 1, buf_v, false);
-            if (t == 1) umma_commit(bar_empty + 8 * s_v);
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_f16_ss(tmem + 128 * t, dq + (kk >> 2) * ((128 * 128) >> 4) + 2 * (kk & 3),
+                        dk + (kk >> 2) * ((128 * 128) >> 4) + 2 * (kk & 3), idesc_s, kk > 0);
+          umma_commit(bar_s + 8 * t);
+        };
+        // (half of the keys)
+        auto values = [&](int t, int half, uint32_t buf, bool first) {
+          const uint64_t dv = desc_v(buf);
+#pragma unroll
+          for (int k4 = 0; k4 < kKeys / 32; ++k4) {
+            const int kk = half * (kKeys / 32) + k4;
+            umma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * kk, dv + kk * (2048 >> 4), idesc_o, !first || kk > 0);
+          }
+          if (half == 0) umma_commit(bar_h + 8 * t);
+        };
+        auto weights_of = [&](int t, int half, uint32_t parity) {
+          mbar_wait(bar_p + 16 * half + 8 * t, parity, abort_flag);
+          tc_fence_after_sync();
+        };
+        auto loaded = [&] {
+          mbar_wait(bar_full + 8 * s, ph, abort_flag);
+          tc_fence_after_sync();
+          return ring + s * geo::kTile;
+        };
+        auto step = [&] {
+          if (++s == geo::kBufs) { s = 0; ph ^= 1; }
+        };
+        // (a commit to bar_empty: the buffer is free once what was issued is done)
+        if (n > 0) mbar_wait(bar_q, 0, abort_flag);
+        for (int i = 0; i < min(kAhead, n); ++i) {
+          const uint32_t buf = loaded();
+          scores(TWO ? 0 : i, buf);
+          if (TWO) scores(1, buf);
+          umma_commit(bar_empty + 8 * s);
+          step();
+        }
+        for (int i = 0; i < n; ++i) {
+          const uint32_t buf_v = loaded();
+          if (!whole_block(i)) {
+            mbar_wait(bar_z + 8 * s, (ph_z >> s) & 1, abort_flag);
+            ph_z ^= 1u << s;
+          }
+          const int s_v = s;
+          step();
+          if constexpr (TWO) {
+            uint32_t buf_k = 0;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              weights_of(t, 0, i & 1);
+              values(t, 0, buf_v, i == 0);
+              if (t == 0 && i + 1 < n) buf_k = loaded();
+              weights_of(t, 1, i & 1);
+              values(t, 1, buf_v, false);
+              if (t == 1) umma_commit(bar_empty + 8 * s_v);
+              if (i + 1 < n)
+                scores(t, buf_k);
+              else
+                umma_commit(bar_o + 8 * t);
+            }
             if (i + 1 < n) {
+              umma_commit(bar_empty + 8 * s);
+              step();
+            }
+          } else {
+            const int t = i & 1;
+            weights_of(t, 0, (i >> 1) & 1);
+            values(t, 0, buf_v, i < 2);
+            uint32_t buf_k = 0;
+            if (i + 2 < n) buf_k = loaded();
+            weights_of(t, 1, (i >> 1) & 1);
+            values(t, 1, buf_v, false);
+            umma_commit(bar_empty + 8 * s_v);
+            if (i + 2 < n) {
               scores(t, buf_k);
-              if (t == 1) used();
+              umma_commit(bar_empty + 8 * s);
+              step();
             } else {
               umma_commit(bar_o + 8 * t);
             }
           }
-          __syncwarp();
-        }
-        if (i + 1 < n) step();
-      } else {
-        const int t = i & 1;
-        weights_of(t, 0, (i >> 1) & 1);
-        if (elect_one()) values(t, 0, buf_v, i < 2);
-        __syncwarp();
-        weights_of(t, 1, (i >> 1) & 1);
-        if (elect_one()) {
-          values(t, 1, buf_v, false);
-          umma_commit(bar_empty + 8 * s_v);
-          if (i + 2 >= n) umma_commit(bar_o + 8 * t);
-        }
-        __syncwarp();
-        if (i + 2 < n) {
-          const uint32_t buf_k = loaded();
-          if (elect_one()) {
-            scores(t, buf_k);
-            used();
-          }
-          __syncwarp();
-          step();
         }
       }
-    }
+      __syncwarp();
+    } else if (exists) {
+      // ------------------------------------------------------------ zeros
+      // Keys that no row sees may hold anything, and 0 times an infinity is none: their values become zeros.
+      // (bar_y first: of a phase of bar_full that is further off than the next, a wait would not know.)
+      uint32_t ph_y = 0;
+      for (int i = 0; i < n; ++i) {
+        if (whole_block(i)) continue;
+        const int at = i < n - kAhead ? min(kAhead, n) + 2 * i : n + i, slot = at % geo::kBufs;  // of the loads (see there)
+        mbar_wait(bar_y + 8 * slot, (ph_y >> slot) & 1, abort_flag);
+        ph_y ^= 1u << slot;
+        mbar_wait(bar_full + 8 * slot, (at / geo::kBufs) & 1, abort_flag);
+        __syncwarp();
+        const int j0 = v.block(i0 + i) * kKeys, thread = 32 * (warp - kMmaWarp - 1) + lane;
+        auto clear = [&](int from, int to) {
+          for (int x = from * (kHalves * 8) + thread; x < to * (kHalves * 8); x += 64)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             ring + slot * geo::kTile + x / 8 % kHalves * (128 * 128) + x / (kHalves * 8) * 128 + (x & 7) * 16),
+                         "r"(0)
+                         : "memory");
+        };
+        clear(max(0, min(v.end, v.pmax + 1) - j0), kKeys);
+        if (p.mask.window) clear(max(0, p.mask.sinks - j0), min(kKeys, v.pmin - p.mask.window + 1 - j0));
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_z + 8 * slot);
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
