@@ -241,17 +241,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         *block = n - ahead + (y - 2 * (n - ahead));  // V of the last blocks
         return 1;
       };
-      auto page_of = [&](int x) {
-        int block;
-        what(x, &block);
-        return page_at(p.c, table, p.c.width, (v.block(i0 + block) * kKeys + bx * box_rows) >> p.c.page_shift);
+      // The pages of 32 / boxes blocks at a time, one to a lane: those of the values' block, of the next ones (the keys are up to two
+      // blocks ahead), and the ones behind on their way.
+      const int per = 32 / boxes;
+      auto pages_of = [&](int group) {
+        const int block = group * per + half;
+        return block < n ? page_at(p.c, table, p.c.width, (v.block(i0 + block) * kKeys + bx * box_rows) >> p.c.page_shift) : -1;
       };
-      int page = total > 0 ? page_of(0) : 0, s = 0;
+      int group = 0, pages = pages_of(0), pages1 = pages_of(1), pages2 = pages_of(2), s = 0;
       uint32_t ph = 0;
       for (int x = 0; x < total; ++x) {
-        const int page_next = x + 1 < total ? page_of(x + 1) : 0;
         int block;
         const int is_v = what(x, &block);
+        if (is_v && block / per > group) {
+          ++group;
+          pages = pages1, pages1 = pages2, pages2 = pages_of(group + 2);
+        }
+        const int page = __shfl_sync(0xffffffffu, block / per == group ? pages : pages1, block % per * boxes + bx);
         mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
         __syncwarp();
         const unsigned there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << boxes) - 1);
@@ -265,7 +271,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_4d(ring + s * geo::kTile + half * (128 * 128) + bx * box_rows * 128, is_v ? &tmap_v : &tmap_k, half * 64,
                       (v.block(i0 + block) * kKeys + bx * box_rows) & (p.c.page - 1), h, page < 0 ? p.c.n_pages : page,
                       bar_full + 8 * s);
-        page = page_next;
         if (++s == geo::kBufs) { s = 0; ph ^= 1; }
       }
     } else if (exists && warp == kMmaWarp) {
