@@ -634,7 +634,7 @@ ManyPlan many_plan(long long rows, int B, long long most_rows, int Hk, long long
   m.slots = (int)(m.two ? 2 * tiles : tiles);
   // (a step over a tile's blocks takes some 1.9 us, a part 0.15 us in the join: the sum is least where steps and parts balance)
   const long long balance = (long long)std::sqrt((m.two ? 12.0 : 6.0) * (double)(most_keys / 128));
-  m.splits = (int)std::max<long long>(1, std::min({sm_count / (likely * Hk), most_keys / 256, balance}));
+  m.splits = (int)std::max<long long>(1, std::min({sm_count / (likely * Hk), (most_keys + 255) / 256, balance}));
   return m;
 }
 size_t many_bytes(const ManyPlan& m, int Hk, int D) { return part_bytes((long long)m.slots * Hk * m.splits, 128, D); }

@@ -602,37 +602,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         auto store = [&](char* to, int elem, int first_elem) {  // 2 D bytes of every row
           __syncwarp();
+          constexpr int kBatch = 8;  // (reads first, then what waits for them)
 #pragma unroll
-          for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
-            const int rr = i * kRowsAtOnce + sub;
-            const uint4 x = lds128(stage + rr * kBytes + ((piece ^ (rr & (kPieces - 1))) << 4));
-            const long long at = __shfl_sync(0xffffffffu, off, rr);
-            if ((real >> rr) & 1) *reinterpret_cast<uint4*>(to + (at + first_elem) * elem + piece * 16) = x;
+          for (int i0 = 0; i0 < 32 / kRowsAtOnce; i0 += kBatch) {
+            uint4 x[kBatch];
+            long long at[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              const int rr = (i0 + i) * kRowsAtOnce + sub;
+              x[i] = lds128(stage + rr * kBytes + ((piece ^ (rr & (kPieces - 1))) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) at[i] = __shfl_sync(0xffffffffu, off, (i0 + i) * kRowsAtOnce + sub);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+              if ((real >> ((i0 + i) * kRowsAtOnce + sub)) & 1)
+                *reinterpret_cast<uint4*>(to + (at[i] + first_elem) * elem + piece * 16) = x[i];
           }
           __syncwarp();
         };
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {  // sixteen columns
+        auto columns = [&](int c, float (&x)[16]) {  // sixteen of them
           uint32_t o[16];
           __syncwarp();
           if (n > 0) {
             tmem_ld_32x16(t_o + 16 * c, o);
             tmem_ld_wait();
           }
-          float x[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             x[e] = n > 0 ? __uint_as_float(o[e]) : 0.f;
             if (two_parts) x[e] = f0 * x[e] + f1 * other[(16 * c + e) * 128 + row];
           }
-          if (parts) {
-            constexpr int kAtOnce = D / 32;  // sixteens of columns that 2 D bytes hold in fp32
+        };
+        if (parts) {
+          constexpr int kAtOnce = D / 32;  // sixteens of columns that 2 D bytes hold in fp32
+#pragma unroll 1
+          for (int c0 = 0; c0 < D / 16; c0 += kAtOnce) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              staged((c % kAtOnce) * 4 + q, __float_as_uint(x[4 * q]), __float_as_uint(x[4 * q + 1]), __float_as_uint(x[4 * q + 2]),
-                     __float_as_uint(x[4 * q + 3]));
-            if (c % kAtOnce == kAtOnce - 1) store(reinterpret_cast<char*>(p.part), 4, 16 * (c - kAtOnce + 1));
-          } else {
+            for (int c = 0; c < kAtOnce; ++c) {
+              float x[16];
+              columns(c0 + c, x);
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                staged(c * 4 + q, __float_as_uint(x[4 * q]), __float_as_uint(x[4 * q + 1]), __float_as_uint(x[4 * q + 2]),
+                       __float_as_uint(x[4 * q + 3]));
+            }
+            store(reinterpret_cast<char*>(p.part), 4, 16 * c0);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            float x[16];
+            columns(c, x);
             uint32_t y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -642,8 +663,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             staged(2 * c, y[0], y[1], y[2], y[3]);
             staged(2 * c + 1, y[4], y[5], y[6], y[7]);
-            if (c == D / 16 - 1) store(reinterpret_cast<char*>(p.out), 2, 0);
           }
+          store(reinterpret_cast<char*>(p.out), 2, 0);
         }
       }
     }
