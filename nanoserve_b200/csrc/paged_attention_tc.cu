@@ -17,11 +17,13 @@
 // block adds up to over 2^24 (scores that jump), m is taken anew at once, and that half's weights too: O stays under 2^25 |v|.
 // What bounds it: 128 x 128 scores of heads of 128 take the tensor core 1024 cycles (both products), and the 16 exponentials per
 // cycle of an SM as long.  An eighth of the exponentials are therefore polynomials on the multiply-add pipes, pairs at a time, and
-// the second product starts when half of the weights are there.  256 rows x 128 keys take 3300 cycles where the products alone would
-// take 2048: a tile's softmax waits some 1000 for its scores (behind the other tile's products), spends 1350 on the exponentials and
-// the rest on reading, masking and storing.  8192 new tokens in a window of 4096, 28 / 4 heads of 128: 353 us, 1020 TFLOP/s (a bf16
-// GEMM here: 1670), at the board's power limit.  Tried there: two threads to a row 388 us, so that rows of half the length leave room in registers;
-// every second, third or fourth pair a polynomial 413, 358 and 357 us.
+// the second product starts when half of the weights are there.  The products are issued by one thread without a branch between
+// them: with a choice of the lane and a barrier of the warp around each group that warp alone took 2900 cycles per 256 rows x 128
+// keys, where the products take 2048.  8192 new tokens in a window of 4096, 28 / 4 heads of 128: 333 us, 1080 TFLOP/s (a bf16 GEMM
+// here: 1670), at the board's power limit; with nothing done between the products 242 us.  Tried there: two threads to a row, so
+// that rows of half the length leave room in registers, 388 us where one took 353; every second, third or fourth pair a
+// polynomial 413, 358 and 357; the next block's scores in halves, beside the weights, 375 where 353 (products of 64 columns read
+// their operands twice); weights handed over as 96 and 32 keys 339 where 338.
 // Every wait is bounded; a time-out is recorded in the device's status word.
 #include <algorithm>
 
