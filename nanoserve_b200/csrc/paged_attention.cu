@@ -69,9 +69,9 @@ struct Told {
 };
 __device__ __forceinline__ Told told(const FewRows& p, int b) {
   Told t;
-  t.first = p.mask.flat ? 0 : p.cu_tokens ? __ldcg(p.cu_tokens + b) : b;
+  t.first = p.mask.flat ? b * p.mask.flat : p.cu_tokens ? __ldcg(p.cu_tokens + b) : b;
   t.rows = p.mask.flat ? p.mask.flat : p.cu_tokens ? __ldcg(p.cu_tokens + b + 1) - t.first : 1;
-  t.len = __ldcg(p.c.lens + b);
+  t.len = __ldcg(p.c.lens + (p.mask.flat ? 0 : b));
   return t;
 }
 // A sequence's rows and what they see; at least one block, so that somebody writes the rows that see nothing.
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // One CTA per tile of a sequence, a warp to a row.
 struct JoinArgs {
   FewRows own;                    // the sequences' own keys
-  int prefix_kind;                // 0: none, 1: the same kernel over the prefix, 2: the kernel for many rows
+  int prefix_kind;                // 0: none, 1 and 3: the same kernel over the prefix, one tile or several, 2: the kernel for many rows
   FewRows prefix;
   const float* many_part;         // [tile, split][128][D]
   const float2* many_stat;        // [tile, split][128]
@@ -512,7 +512,8 @@ struct FewParts {
   }
 };
 
-template <int D>
+// KIND: prefix_kind.  (Its own code for each: a launch this short takes as long as its instructions take to come.)
+template <int D, int KIND>
 __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
   const FewRows& p = a.own;
   const int b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads, lane = threadIdx.x & 31;
@@ -523,26 +524,28 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
   const int rows = tile_rows(p, v, h);
   if (rows == 0) return;
   const FewParts own(p, all, v, b, h);
-  if (own.n == 1 && a.prefix_kind == 0) return;  // written by its one CTA
+  if (KIND == 0 && own.n == 1) return;  // written by its one CTA
   // the prefix's parts in front, then its own: which rows of which arrays
   int n_pre = 0;
   FewParts pre = own;
-  if (a.prefix_kind == 1) {
-    const Sequences one(a.prefix);
-    pre = FewParts(a.prefix, one, one.rows(a.prefix, 0), 0, h);
+  if constexpr (KIND == 1 || KIND == 3) {
+    const Sequences parts(a.prefix);
+    const int g = KIND == 3 ? b / a.prefix.mask.flat : 0;
+    pre = FewParts(a.prefix, parts, parts.rows(a.prefix, g), g, h);
     n_pre = pre.n;
-  } else if (a.prefix_kind == 2) {
+  } else if constexpr (KIND == 2) {
     n_pre = a.many_splits;
   }
   for (int row = threadIdx.x >> 5; row < rows; row += 8) {
-    const int r = b * p.rep_all + group(p, h) * kRows + row;  // of the prefix's rows
+    // of the prefix's rows, or of those of a tile of them
+    const int r = (KIND == 3 ? b % a.prefix.mask.flat : b) * p.rep_all + group(p, h) * kRows + row;
     const long long pre0 = ((long long)kv_head(p, h) * a.many_tiles + r / 128) * a.many_splits * 128 + r % 128;
     Row<D> out;
     out.join(
         n_pre + own.n, lane, [&](int i) {
-          return i >= n_pre            ? Part{p.stat, p.part, own.slot(i - n_pre) * kRows + row}
-                 : a.prefix_kind == 1 ? Part{a.prefix.stat, a.prefix.part, pre.slot(i) * kRows + r}
-                                      : Part{a.many_stat, a.many_part, pre0 + i * 128};
+          return KIND == 0 || i >= n_pre ? Part{p.stat, p.part, own.slot(i - n_pre) * kRows + row}
+                 : KIND == 2             ? Part{a.many_stat, a.many_part, pre0 + i * 128}
+                                         : Part{a.prefix.stat, a.prefix.part, pre.slot(i) * kRows + r};
         });
     const int tok = token_of(p, row);
     out.store(p.out + (long long)(v.first + tok) * p.out_stride + (first_head(p, h) + row - tok * p.rep) * D, lane);
@@ -588,8 +591,9 @@ FewRows few_rows(const void* q, long long q_stride, const PagedCache& c, const i
 }
 
 int join(const JoinArgs& a, int rows, cudaStream_t s) {
-  return launch_pdl(a.own.c.D == 64 ? join_kernel<64> : join_kernel<128>, dim3((unsigned)(a.own.c.B * a.own.heads)),
-                    32 * std::min(rows, 8), 0, s, a);
+  static void (*const kernels[2][4])(JoinArgs) = {{join_kernel<64, 0>, join_kernel<64, 1>, join_kernel<64, 2>, join_kernel<64, 3>},
+                                                  {join_kernel<128, 0>, join_kernel<128, 1>, join_kernel<128, 2>, join_kernel<128, 3>}};
+  return launch_pdl(kernels[a.own.c.D == 128][a.prefix_kind], dim3((unsigned)(a.own.c.B * a.own.heads)), 32 * std::min(rows, 8), 0, s, a);
 }
 
 int check_rows(const void* q, long long q_stride, const PagedCache& c, int T, int Hq, float scale, const void* out,
@@ -679,11 +683,16 @@ size_t paged_attention_workspace(int T, int B, int max_tokens, int Hq, int Hk, i
   const ManyPlan m = many_plan((long long)T * rep, B, (long long)max_tokens * rep, Hk, kMostKeys, sm_count);
   return std::max<size_t>(256, m.splits > 1 ? many_bytes(m, Hk, D) : 0);
 }
+// The prefix through the kernel for few rows: sixteen rows' worth of whole sequences to a tile.  0: a sequence's rows do not fit.
+long long prefix_tiles(int B, int rep) { return rep > kRows ? 0 : (B + kRows / rep - 1) / (kRows / rep); }
+
 size_t shared_prefix_workspace(int B, int Hq, int Hk, int D, int sm_count) {
   const int rep = Hq / Hk;
   const size_t own = part_bytes(2LL * sm_count + (long long)B * Hk * ((rep + kRows - 1) / kRows), kRows, D);
-  if ((long long)B * rep <= kRows) return own + part_bytes(2LL * sm_count + Hk, kRows, D);
-  return own + many_bytes(many_plan((long long)B * rep, 1, (long long)B * rep, Hk, kMostKeys, sm_count), Hk, D);
+  const long long tiles = prefix_tiles(B, rep);
+  const size_t few = tiles ? part_bytes(2LL * sm_count + tiles * Hk, kRows, D) : 0;  // (which it will be, the prefix's length says)
+  if (tiles == 1) return own + few;
+  return own + std::max(few, many_bytes(many_plan((long long)B * rep, 1, (long long)B * rep, Hk, kMostKeys, sm_count), Hk, D));
 }
 
 int paged_attention_launch(const void* q, long long q_stride, const PagedCache& c, const int* cu_tokens, int T,
@@ -738,11 +747,27 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
   pre.B = 1;
   JoinArgs a{};
   int own_ctas = sm_count;
-  if (c.B * rep <= kRows) {
-    a.prefix_kind = 1;
-    a.prefix = few_rows(q, q_stride, pre, nullptr, rep, scale_log2, out, out_stride, prefix_parts, 2LL * sm_count + c.Hk,
-                        sm_count, c.B, c.B);
-    a.prefix.mask = Mask{0, 0, c.B};
+  // A tile reads all of the prefix, which several of them do where it is short and the sequences' own tables are: up to two blocks of
+  // 64 keys to an SM in all, up to 128 rows, up to four blocks to an SM of own keys.  The kernel for many rows takes 13 us for whatever
+  // it does (777 tokens, three sequences of 28 / 4 heads of 128: 13.2 us the three launches, 18.9 through that one; 500 tokens, 16
+  // sequences of 300 and of 2000: 15.8 and 29.4 against 18.4 and 26.4).  Where both tables hold more blocks than there are SMs, the two
+  // kernels divide these in that ratio, up to eight blocks to a CTA of the prefix's; else idle CTAs make room by themselves.
+  const long long tiles = prefix_tiles(c.B, rep), blocks = tiles * c.Hk * (((long long)prefix_width * c.page + kKeys - 1) / kKeys);
+  const long long own_blocks = (long long)c.B * c.Hk * (((long long)c.width * c.page + kKeys - 1) / kKeys);
+  const bool little = blocks <= 2LL * sm_count;
+  if (tiles == 1 || (tiles > 1 && little && c.B * rep <= 128 && own_blocks <= 4LL * sm_count)) {
+    a.prefix_kind = tiles == 1 ? 1 : 3;
+    pre.B = (int)tiles;
+    pre.table_stride = 0;
+    int ctas = sm_count;
+    if (little && blocks + own_blocks > sm_count) {
+      const long long share = std::max(sm_count * blocks / (blocks + own_blocks), (blocks + 7) / 8);
+      ctas = (int)std::max<long long>(1, std::min({share, blocks, sm_count - (sm_count + 7LL) / 8}));
+      own_ctas = std::max(1, sm_count - ctas);
+    }
+    a.prefix = few_rows(q, q_stride, pre, nullptr, rep, scale_log2, out, out_stride, prefix_parts, 2LL * sm_count + tiles * c.Hk,
+                        ctas, c.B, c.B);
+    a.prefix.mask = Mask{0, 0, std::min(c.B, kRows / rep)};
     a.prefix.parts_only = 1;
     if (const int rc = launch_few(a.prefix, s)) return rc;
   } else {

@@ -489,3 +489,26 @@ def test_many_rows_and_prefixes_on_streams_and_in_graphs(kernels):
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(out, want[r][i]) for r, i, _, out in graphs)
+
+
+@pytest.mark.parametrize("B,prefix,own,Hq,Hk,D,page,spare", [
+    (3, 200, [1, 64, 65], 9, 1, 128, 16, 0),       # a sequence to a tile
+    (5, 300, [0, 2, 70, 5, 1], 16, 1, 64, 32, 0),
+    (18, 190, [3] * 18, 28, 4, 128, 16, 0),        # 126 rows; 19 sequences: 133
+    (19, 190, [3] * 19, 28, 4, 128, 16, 0),
+    (33, 100, [7, 0, 130] * 11, 2, 2, 64, 16, 0),  # sixteen sequences to a tile
+    (4, 500, [700, 1, 90, 5], 64, 8, 128, 64, 0),  # both kernels beside one another
+    (3, 777, [20, 30, 1], 28, 4, 128, 16, 400),    # wide tables, short sequences
+    (3, 0, [20, 30, 0], 28, 4, 128, 16, 0),
+])
+def test_shared_prefix_in_several_tiles(kernels, B, prefix, own, Hq, Hk, D, page, spare):
+    """Short prefixes, which tiles of sixteen rows read one by one."""
+    b = Batch([0] + [1] * B, [prefix] + own, Hq, Hk, D, page, seed=60 + B, spare_width=spare)
+    table, b.table, b.seq_lens, b.lens = b.table[0, :max(1, -(-prefix // page))].contiguous(), b.table[1:], b.seq_lens[1:], own
+    plen = torch.tensor([prefix], dtype=torch.int32, device="cuda")
+    ref, tol = prefix_reference(b, table, prefix)
+    wide = torch.full((b.T, Hq * D + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    args = (b.cache_k, b.cache_v, table, plen, b.table, b.seq_lens, *b.heads)
+    out = kernels.shared_prefix_attention(b.q, *args, out=wide[:, :Hq * D])
+    check(out, ref, tol)
+    assert (wide[:, Hq * D:] == 7.0).all() and torch.equal(out, kernels.shared_prefix_attention(b.q, *args))
