@@ -369,7 +369,7 @@ int b2_tp_wait(const void* wait_sig, const void* epoch, unsigned wait_per_epoch,
  *     which their weights, added up, exceed u times their sum.  Weights are held to 2^-44 of the largest.  temperature <= 0: the
  *     largest logit, lowest index.  NaN counts as no logit; -1 where a row has no logit above minus infinity.  Each parameter is
  *     an array [rows] on the device (top_k int32, the others fp32) or, where that is NULL, the value behind the arrays.
- *     V <= 262144.
+ *     V <= 262144, rows <= 2^20.
  */
 typedef struct b2_paged_cache {
   void* k;

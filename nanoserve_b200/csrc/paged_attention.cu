@@ -18,8 +18,8 @@
 //
 // Bound by the start and the end of a launch, then by memory: a block of 64 keys of 128 takes an SM 1240 cycles from shared memory
 // (at HBM's pace 32 KB take 1455), a launch some 7000 before the first block (lengths, tables, the first loads) and the join 2 to
-// 4 us behind it.  28 / 4 heads of 128: 16 sequences of 500 to 32767 tokens in a window of 4096, 22 us for 89 MB, 4.1 TB/s; the own
-// keys of 64 sequences behind a prefix, 34 us for 143 MB, 4.2 TB/s.
+// 4 us behind it.  28 / 4 heads of 128: 16 sequences of 500 to 32767 tokens in a window of 4096, 89 MB, 27 us (22 where the L2 still
+// holds a part of them); the own keys of 64 sequences behind a prefix, 34 us for 143 MB, 4.2 TB/s.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -752,7 +752,8 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
   // it does (777 tokens, three sequences of 28 / 4 heads of 128: 13.2 us the three launches, 18.9 through that one; 500 tokens, 16
   // sequences of 300 and of 2000: 15.8 and 29.4 against 18.4 and 26.4).  Where both tables hold more blocks than there are SMs, the two
   // kernels divide these in that ratio, up to eight blocks to a CTA of the prefix's; else idle CTAs make room by themselves.
-  const long long tiles = prefix_tiles(c.B, rep), blocks = tiles * c.Hk * (((long long)prefix_width * c.page + kKeys - 1) / kKeys);
+  const long long tiles = prefix_tiles(c.B, rep);
+  const long long blocks = tiles * c.Hk * std::max(1LL, ((long long)prefix_width * c.page + kKeys - 1) / kKeys);
   const long long own_blocks = (long long)c.B * c.Hk * (((long long)c.width * c.page + kKeys - 1) / kKeys);
   const bool little = blocks <= 2LL * sm_count;
   if (tiles == 1 || (tiles > 1 && little && c.B * rep <= 128 && own_blocks <= 4LL * sm_count)) {

@@ -512,3 +512,14 @@ def test_shared_prefix_in_several_tiles(kernels, B, prefix, own, Hq, Hk, D, page
     out = kernels.shared_prefix_attention(b.q, *args, out=wide[:, :Hq * D])
     check(out, ref, tol)
     assert (wide[:, Hq * D:] == 7.0).all() and torch.equal(out, kernels.shared_prefix_attention(b.q, *args))
+
+
+@pytest.mark.parametrize("B", [2, 9, 70])
+def test_shared_prefix_without_a_page(kernels, B):
+    """A prefix table of no page, whatever the length says: the own keys alone."""
+    b = Batch([1] * B, [30 + i for i in range(B)], 28, 4, 128, 16, seed=80 + B)
+    table = torch.empty(0, dtype=torch.int32, device="cuda")
+    ref, tol = paged_reference(b)
+    for length in (0, 50, -3):
+        plen = torch.tensor([length], dtype=torch.int32, device="cuda")
+        check(kernels.shared_prefix_attention(b.q, b.cache_k, b.cache_v, table, plen, b.table, b.seq_lens, *b.heads), ref, tol)
