@@ -25,7 +25,7 @@
 // row of way 3 takes 19 us.  64 rows: 71 us.
 #include <algorithm>
 
-#include "paged.cuh"
+#include "paged_attention.cuh"
 #include "ptx.cuh"
 #include "w4_internal.h"
 
@@ -40,6 +40,7 @@ constexpr int kList = kThreads;  // logits that one CTA looks at alone, one to a
 constexpr float kReach = 40.f;   // distances beyond it, in T, have a weight under 2^-57: none
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kSliceBytes = 150 * 1024;
+constexpr size_t kMaxSmem = 227 * 1024;
 constexpr double kOne = 17592186044416.0;  // 2^44: a weight of 1
 constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52: a double added to it is rounded to a whole number, in its low bits
 
@@ -763,9 +764,10 @@ template <typename L, int C>
 int launch_on(const Sampling& p, cudaStream_t s) {
   const int chunk = chunk_of<L>(p.V, C);
   const size_t smem = sizeof(Shared) + (size_t)kThreads * chunk * sizeof(typename Keys<L>::Stored);
-  if (smem > 227 * 1024) return kErrTooLarge;
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<L, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
+  if (smem > kMaxSmem) return kErrTooLarge;
+  // (the limit belongs to the kernel, not to the call: set to one call's size it would refuse another thread's launch)
+  static SharedMemoryOnce once;
+  if (const int rc = once.allow(sample_kernel<L, C>, kMaxSmem)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.rows * C));
   cfg.blockDim = dim3(kThreads);
