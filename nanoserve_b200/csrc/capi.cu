@@ -377,6 +377,8 @@ int b2_device_status(void) {
     if (e != cudaSuccess) return (int)e;
   }
   b2::noalloc_status_word(dev, &word2);  // the fixed array of b2_w4_gemv_noalloc, if that entry point has run
+  if (const int rc = b2::few_rows_timed_out(dev, false, &word)) return rc;  // the paged attention's words, where it has run
+  if (const int rc = b2::many_rows_timed_out(dev, false, &word)) return rc;
   return (word | word2) == 0 ? 0 : b2::kErrDevice;
 }
 
@@ -388,6 +390,9 @@ int b2_clear_status(void) {
   // a time-out may have left arrival counters half counted: clear them with the status word
   if (st) e = cudaMemset(st->ws.status, 0, (kCounters + 64) * sizeof(int));
   b2::noalloc_clear(dev);
+  int unused = 0;
+  if (e == cudaSuccess) e = (cudaError_t)b2::few_rows_timed_out(dev, true, &unused);
+  if (e == cudaSuccess) e = (cudaError_t)b2::many_rows_timed_out(dev, true, &unused);
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
   return (int)e;
 }

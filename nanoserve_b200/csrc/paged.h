@@ -46,4 +46,9 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
 size_t shared_prefix_workspace(int B, int Hq, int Hk, int D, int sm_count);
 int sample_launch(const Sampling& p, cudaStream_t s);
 
+// Whether a wait of the kernels for few rows, or for many, ran out on device `dev`: added to *word, or cleared.  The caller has
+// synchronised.
+int few_rows_timed_out(int dev, bool clear, int* word);
+int many_rows_timed_out(int dev, bool clear, int* word);
+
 }  // namespace b2

@@ -38,6 +38,9 @@ constexpr int kRows = 16;       // rows of a tile
 constexpr int kWarps = 4;       // each takes sixteen keys of a block
 constexpr int kThreads = 32 * (kWarps + 1);
 
+__device__ int g_timed_out;  // a wait of this file's kernels ran out
+Devices g_ran;
+
 template <int D>
 struct Geo {
   static constexpr int kTile = kKeys * D * 2;                 // K (or V) of a block
@@ -474,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       w.next(p, all);
     }
   }
-  if (tid == 0 && *abort_flag && p.status) atomicCAS(p.status, 0, kStatusGemvTimeout);
+  if (tid == 0 && *abort_flag) g_timed_out = 1;
   if (p.late_wait) pdl_wait_prior_grid();
 }
 
@@ -561,7 +564,7 @@ int launch_few_of(const FewRows& p, cudaStream_t s) {
   CUtensorMap mk, mv;
   if (!paged_tensor_maps(p.c, kKeys, &mk, &mv)) return kErrBadShape;
   static SharedMemoryOnce once;
-  if (const int rc = once.allow(few_rows_kernel<D>, Geo<D>::kSmem)) return rc;
+  if (const int rc = once.allow(few_rows_kernel<D>, Geo<D>::kSmem, &g_ran)) return rc;
   return launch_pdl(few_rows_kernel<D>, dim3(p.n_cta), kThreads, Geo<D>::kSmem, s, mk, mv, p);
 }
 
@@ -586,7 +589,6 @@ FewRows few_rows(const void* q, long long q_stride, const PagedCache& c, const i
   p.scale_log2 = scale_log2;
   p.part = static_cast<float*>(parts);
   p.stat = reinterpret_cast<float2*>(static_cast<char*>(parts) + align256((size_t)slots * kRows * c.D * 4));
-  p.status = device_status_word_if_ready();
   return p;
 }
 
@@ -664,7 +666,6 @@ ManyRows many_rows(const void* q, long long q_stride, const PagedCache& c, const
     p.stat = reinterpret_cast<float2*>(static_cast<char*>(parts) +
                                        align256((size_t)m.slots * c.Hk * m.splits * 128 * c.D * 4));
   }
-  p.status = device_status_word_if_ready();
   return p;
 }
 
@@ -675,6 +676,8 @@ bool few(int max_tokens, int rep) { return max_tokens == 1 || (long long)max_tok
 constexpr long long kMostKeys = 1LL << 30;
 
 }  // namespace
+
+int few_rows_timed_out(int dev, bool clear, int* word) { return timed_out_word(g_timed_out, g_ran, dev, clear, word); }
 
 size_t paged_attention_workspace(int T, int B, int max_tokens, int Hq, int Hk, int D, int sm_count) {
   max_tokens = std::min(max_tokens, T);

@@ -36,7 +36,6 @@ struct FewRows {
   float scale_log2;  // scale / ln 2
   float* part;       // [slot][16][D], not divided by the sum
   float2* stat;      // [slot][16] maximum (in powers of two) and sum
-  int* status;
 };
 
 // Tiles of 128 rows (token, query head) of a sequence and KV head.
@@ -55,25 +54,39 @@ struct ManyRows {
   float scale_log2;
   float* part;       // [KV head][slot][split][128][D], not divided by the sum; null: one split, to out
   float2* stat;      // beside it: maximum (in powers of two) and sum
-  int* status;
 };
 int many_rows_launch(const ManyRows& p, cudaStream_t s);
 int join_many_launch(const ManyRows& p, cudaStream_t s);
 
-// Dynamic shared memory beyond 48 KB is allowed a kernel once per device.
+// Devices on which kernels of a source file have been launched: a bit each.
+using Devices = std::atomic<unsigned long long>;
+
+// Dynamic shared memory beyond 48 KB is allowed a kernel once per device, which is noted in `ran`.
 struct SharedMemoryOnce {
-  std::atomic<unsigned long long> done{0};
+  Devices done{0};
   template <typename K>
-  int allow(K* kernel, size_t bytes) {
+  int allow(K* kernel, size_t bytes, Devices* ran = nullptr) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     const unsigned long long bit = 1ull << (dev & 63);
     if (e != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return (int)e;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    if (e == cudaSuccess && ran) ran->fetch_or(bit, std::memory_order_release);
     return (int)e;
   }
 };
+
+// A word `timed_out` of a source file's device image, which its kernels set where a wait ran out.  It is there from the first launch
+// on, captured or not, whether or not the library's state of the device is.  Added to *word; with `clear`, set to 0.
+template <typename Word>
+int timed_out_word(const Word& timed_out, const Devices& ran, int dev, bool clear, int* word) {
+  if (dev < 0 || dev >= 64 || !(ran.load(std::memory_order_acquire) >> dev & 1)) return 0;  // (never loads a kernel's image)
+  int here = 0;
+  const cudaError_t e = clear ? cudaMemcpyToSymbol(timed_out, &here, sizeof here) : cudaMemcpyFromSymbol(&here, timed_out, sizeof here);
+  *word |= here;
+  return (int)e;
+}
 
 template <typename... Args>
 int launch_pdl(void (*kernel)(Args...), dim3 grid, int block, size_t smem, cudaStream_t s, Args... args) {

@@ -24,7 +24,7 @@
 // that rows of half the length leave room in registers, 388 us where one took 353; every second, third or fourth pair a
 // polynomial 413, 358 and 357; the next block's scores in halves, beside the weights, 375 where 353 (products of 64 columns read
 // their operands twice); weights handed over as 96 and 32 keys 339 where 338.
-// Every wait is bounded; a time-out is recorded in the device's status word.
+// Every wait is bounded; a time-out is recorded in a word of this file's device image, which b2_device_status reads.
 #include <algorithm>
 
 #include "paged_attention.cuh"
@@ -41,6 +41,9 @@ constexpr int kThreads = 384;  // three warpgroups: registers are handed over in
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;  // 2 * 216 + 72 = 3 * 168, what the launch gives
 constexpr int kEvery = 8;      // every eighth pair of exponentials is a polynomial
 constexpr int kPresent = 16;   // blocks whose presence bits are kept
+
+__device__ int g_timed_out;  // a wait of this file's kernel ran out
+Devices g_ran;
 
 template <int D, bool TWO>
 struct Geo {
@@ -674,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
-  if (tid == 0 && *abort_flag && p.status) atomicCAS(p.status, 0, kStatusGemmTimeout);
+  if (tid == 0 && *abort_flag) g_timed_out = 1;
 }
 
 // Splits of the keys joined: sixteen rows of a tile of 128 to a CTA, four to a warp.
@@ -704,12 +707,14 @@ int launch(const ManyRows& p, cudaStream_t s) {
   if (!paged_tensor_maps(p.c, kKeys, &mk, &mv)) return kErrBadShape;
   using geo = Geo<D, TWO>;
   static SharedMemoryOnce once;
-  if (const int rc = once.allow(many_rows_kernel<D, TWO>, geo::kSmem)) return rc;
+  if (const int rc = once.allow(many_rows_kernel<D, TWO>, geo::kSmem, &g_ran)) return rc;
   const int tiles = TWO ? p.slots / 2 : p.slots;
   return launch_pdl(many_rows_kernel<D, TWO>, dim3((unsigned)(tiles * p.c.Hk * p.splits)), kThreads, geo::kSmem, s, mk, mv, p);
 }
 
 }  // namespace
+
+int many_rows_timed_out(int dev, bool clear, int* word) { return timed_out_word(g_timed_out, g_ran, dev, clear, word); }
 
 int many_rows_launch(const ManyRows& p, cudaStream_t s) {
   if (p.c.D == 64) return p.two ? launch<64, true>(p, s) : launch<64, false>(p, s);
