@@ -268,8 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (fresh) {
         const uint32_t slot = items & 1;
         const int rows = tile_rows(p, w.v, w.h), tok = token_of(p, lane);
-        mbar_wait(bar_q + 16 + 8 * slot, ((items >> 1) & 1) ^ 1, abort_flag);
-        __syncwarp();
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_q + 16 + 8 * slot, ((items >> 1) & 1) ^ 1, abort_flag))) break;
         if (lane == 0) mbar_arrive_expect_tx(bar_q + 8 * slot, rows * 2 * D);
         __syncwarp();
         if (lane < rows)
@@ -278,8 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    bar_q + 8 * slot);
         ++items;
       }
-      mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
-      __syncwarp();
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag))) break;  // (no loads behind a wait that ran out)
       const unsigned there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << boxes) - 1);
       if (lane == 0) {
         present[s] = there;
@@ -478,6 +476,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (tid == 0 && *abort_flag) g_timed_out = 1;
+  if (*abort_flag)
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);  // copies in flight land before the shared memory is released
   if (p.late_wait) pdl_wait_prior_grid();
 }
 

@@ -267,8 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int page[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) page[i] = __shfl_sync(0xffffffffu, held, from + i);
-        mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag);
-        __syncwarp();
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag))) break;  // (no loads behind a wait that ran out)
         if (lane == 0) {
           const uint32_t full = bar_full + 8 * s, to = ring + s * geo::kTile;
           if (!is_v) present[block % kPresent] = there;
@@ -676,8 +675,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
   if (tid == 0 && *abort_flag) g_timed_out = 1;
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);  // copies and products in flight end before their memory is released
+    __syncthreads();
+  }
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
 // Splits of the keys joined: sixteen rows of a tile of 128 to a CTA, four to a warp.

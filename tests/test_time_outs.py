@@ -27,6 +27,24 @@ def test_time_outs_of_the_paged_attention_are_recorded(name):
         assert f"b2::{reader}(dev, {clear}, " in body
 
 
+@pytest.mark.parametrize("name", [n for n in WAITING if n.startswith("paged_")])
+def test_copies_of_the_paged_attention_land_behind_a_time_out(name):
+    """Shared and tensor memory are not released under copies and products on their way: the loading warp issues none behind a
+    wait that ran out (it could be thousands, into buffers whose barriers still count the last ones), and the CTA stays a while."""
+    s = SOURCES[name]
+    loader = s[s.index("// ------------------------------------------------------------ loads"):]
+    end = "// -------------------------------------------------------------- products" if name == "paged_attention.cu" else \
+        "// ------------------------------------------------------------ products"
+    loader = loader[:loader.index(end)]
+    waits = re.findall(r"^ *(\S.*mbar_wait\(.*)$", loader, re.M)
+    assert len(waits) == (2 if name == "paged_attention.cu" else 1)
+    for w in waits:
+        assert re.match(r"if \(!__all_sync\(0xffffffffu, mbar_wait\(.*\)\)\) break;", w), w
+    after = s[s.index("g_timed_out = 1;"):]
+    assert re.match(r"g_timed_out = 1;\n  if \(\*abort_flag\)(?: \{)?\n    for \(int i = 0; i < 64; \+\+i\) __nanosleep\(2000\);", after)
+    assert "tmem_dealloc" not in s[:s.index("g_timed_out = 1;")]
+
+
 FIRST = """
 import torch
 from nanoserve_b200.ops import Kernels
