@@ -336,8 +336,9 @@ int b2_tp_wait(const void* wait_sig, const void* epoch, unsigned wait_per_epoch,
  *
  * b2_paged_cache: pages of `page_size` tokens (a power of two, 16 to 1024) in two arrays that share one layout: the row of head h
  * at token s of page p is the head_dim values from p * page_stride + h * head_stride + s * token_stride on (elements, multiples of
- * 8; k and v 16-byte aligned), so pages may be [head, token, dim] or [token, head, dim], or parts of larger tensors.  Token j of
- * sequence b is in page block_table[b * table_stride + j / page_size], at j % page_size.  An entry outside 0 .. n_pages - 1, or
+ * 8; k and v 16-byte aligned), so pages may be [head, token, dim] or [token, head, dim], or parts of larger tensors.  (The stride
+ * between pages, heads, sequences or a call's rows is not looked at where there is one of them.)  Token j of sequence b is in
+ * page block_table[b * table_stride + j / page_size], at j % page_size.  An entry outside 0 .. n_pages - 1, or
  * beyond table_width, stands for a page that is not there: its keys take no part, and nothing is stored for it.
  * seq_lens [n_seqs] (int32): the tokens of each sequence, the call's new ones included.
  *

@@ -166,10 +166,9 @@ int to_paged(const b2_paged_cache* c, b2::PagedCache* out) {
   if (c->n_pages < 1 || c->n_kv_heads < 1 || c->n_seqs < 1 || c->table_width < 1 || c->head_dim < 16 || c->head_dim > 256 ||
       c->head_dim % 16 || c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
     return b2::kErrBadShape;
-  // (a stride of 0 or below would lay rows over one another; where there is one page, its stride says nothing)
-  if (c->page_stride % 8 || c->head_stride % 8 || c->token_stride % 8 ||
-      c->page_stride < (c->n_pages > 1 ? c->head_dim : 0) || c->head_stride < c->head_dim ||
-      c->token_stride < c->head_dim || c->table_stride < (c->n_seqs > 1 ? c->table_width : 0))
+  // (a stride of 0 or below would lay rows over one another; where there is one page, or one head, its stride says nothing)
+  if (!b2::rows_fit(c->page_stride, c->head_dim, c->n_pages) || !b2::rows_fit(c->head_stride, c->head_dim, c->n_kv_heads) ||
+      !b2::rows_fit(c->token_stride, c->head_dim, c->page_size) || c->table_stride < (c->n_seqs > 1 ? c->table_width : 0))
     return b2::kErrBadShape;
   if ((long long)c->table_width * c->page_size > (1LL << 30)) return b2::kErrTooLarge;  // positions are 32-bit
   auto off = [](const void* p, uintptr_t to) { return !p || (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; };

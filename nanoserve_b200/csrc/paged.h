@@ -32,6 +32,9 @@ struct Sampling {
   long long* tokens;
 };
 
+// Whether rows of `width` values may lie `stride` elements apart; where there is one row, its stride says nothing.
+inline bool rows_fit(long long stride, long long width, int rows) { return rows == 1 || (stride >= width && stride % 8 == 0); }
+
 // sm_count below 1: minus the error that the device gave, returned once the arguments are found right.
 int paged_append_launch(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq, void* q_out,
                         long long q_stride, const PagedCache& c, const int* cu_tokens, int T, int Hq, int sm_count,

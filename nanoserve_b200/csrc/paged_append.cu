@@ -142,7 +142,7 @@ int paged_append_launch(const void* qkv, long long qkv_stride, const void* bias,
                         cudaStream_t s) {
   const long long heads = (long long)Hq + 2 * c.Hk;
   if (T < 1 || Hq < 1 || (!cu_tokens && T != c.B)) return kErrBadShape;
-  if (qkv_stride < heads * c.D || qkv_stride % 8 || q_stride < (long long)Hq * c.D || q_stride % 8) return kErrBadShape;
+  if (!rows_fit(qkv_stride, heads * c.D, T) || !rows_fit(q_stride, (long long)Hq * c.D, T)) return kErrBadShape;
   if (!qkv || !inv_freq || !q_out || misaligned(qkv, 16) || misaligned(bias, 16) || misaligned(q_out, 16) ||
       misaligned(inv_freq, 4) || misaligned(cu_tokens, 4))
     return kErrBadPointer;

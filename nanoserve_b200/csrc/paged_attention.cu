@@ -601,7 +601,7 @@ int join(const JoinArgs& a, int rows, cudaStream_t s) {
 int check_rows(const void* q, long long q_stride, const PagedCache& c, int T, int Hq, float scale, const void* out,
                long long out_stride) {
   if (!(scale > 0.f) || scale > FLT_MAX / 2 || T < 1 || Hq < 1 || Hq % c.Hk || (c.D != 64 && c.D != 128)) return kErrBadShape;
-  if (q_stride < (long long)Hq * c.D || q_stride % 8 || out_stride < (long long)Hq * c.D || out_stride % 8) return kErrBadShape;
+  if (!rows_fit(q_stride, (long long)Hq * c.D, T) || !rows_fit(out_stride, (long long)Hq * c.D, T)) return kErrBadShape;
   if (!q || !out || misaligned(q, 16) || misaligned(out, 16)) return kErrBadPointer;
   // rows and blocks are counted in 31 bits
   if ((long long)T * Hq > 0x3fffffffLL || ((long long)c.width * c.page / kKeys + 2) * c.B * Hq > 0x7fffffffLL) return kErrTooLarge;
