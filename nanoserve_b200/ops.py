@@ -113,6 +113,12 @@ class PagedCache(ctypes.Structure):
                 ("table_stride", _i64), ("table_width", _i32), ("n_seqs", _i32), ("seq_lens", _vp)]
 
 
+def _int32(x):
+    """x, or where an int of C does not hold it the nearest number that one does (ctypes would take it modulo 2^32): bounds and
+    counts beyond 2^31 mean what 2^31 - 1 does, sizes are refused."""
+    return min(max(x, -2 ** 31), 2 ** 31 - 1)
+
+
 def staged_x_bytes(K: int) -> int:
     """Bytes of one token's activations in the converted form EPI_SWIGLU_STAGED writes and PRO_STAGED reads."""
     return 4 * K + (K // 128) * 32
@@ -428,8 +434,9 @@ class Kernels:
         sp, sh, st, sd = cache_k.stride()
         self._need(what, heads == n_kv_heads, dim == head_dim, sd == 1 and seq_lens.is_contiguous(),
                    block_table.shape[0] == n_seqs, block_table.stride(1) == 1 or block_table.shape[1] == 1)
-        return PagedCache(cache_k.data_ptr(), cache_v.data_ptr(), sp, sh, st, n_pages, page, heads, dim, block_table.data_ptr(),
-                          block_table.stride(0), block_table.shape[1], n_seqs, seq_lens.data_ptr())
+        return PagedCache(cache_k.data_ptr(), cache_v.data_ptr(), sp, sh, st, _int32(n_pages), _int32(page), heads, dim,
+                          block_table.data_ptr(), block_table.stride(0), _int32(block_table.shape[1]), _int32(n_seqs),
+                          seq_lens.data_ptr())
 
     def _rows(self, what, t, width, cu_tokens, n_seqs, rows=None):
         """Checks rows [T, width] (unit stride within a row) and cu_tokens; returns cu_tokens' address."""
@@ -487,8 +494,7 @@ class Kernels:
         c = self._paged(what, cache_k, cache_v, block_table, seq_lens, n_kv_heads, head_dim)
         cu = self._rows(what, q, n_heads * head_dim, cu_tokens, c.n_seqs)
         T = q.shape[0]
-        if max_tokens is None:
-            max_tokens = 1 if cu is None else T
+        max_tokens = _int32(max_tokens if max_tokens is not None else 1 if cu is None else T)
         if out is None:
             out = torch.empty((T, n_heads * head_dim), dtype=q.dtype, device=q.device)
         else:
@@ -496,8 +502,8 @@ class Kernels:
         if T:
             n = self.lib.b2_paged_attention_workspace_bytes(T, c.n_seqs, max_tokens, n_heads, n_kv_heads, head_dim)
             ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-            rc = self.lib.b2_paged_attention(q.data_ptr(), q.stride(0), ctypes.byref(c), cu, T, max_tokens, n_heads, window,
-                                             sinks, head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
+            rc = self.lib.b2_paged_attention(q.data_ptr(), q.stride(0), ctypes.byref(c), cu, T, max_tokens, n_heads, _int32(window),
+                                             _int32(sinks), head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
                                              out.stride(0), ws.data_ptr(), n, self._stream())
             self._check(rc, "b2_paged_attention")
         return out
@@ -527,7 +533,7 @@ class Kernels:
         n = self.lib.b2_shared_prefix_workspace_bytes(c.n_seqs, n_heads, n_kv_heads, head_dim)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         rc = self.lib.b2_shared_prefix_attention(q.data_ptr(), q.stride(0), ctypes.byref(c), prefix_table.data_ptr(),
-                                                 prefix_table.numel(), prefix_len.data_ptr(), n_heads,
+                                                 _int32(prefix_table.numel()), prefix_len.data_ptr(), n_heads,
                                                  head_dim ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0),
                                                  ws.data_ptr(), n, self._stream())
         self._check(rc, "b2_shared_prefix_attention")
@@ -559,12 +565,12 @@ class Kernels:
                 values.append(off)
             else:
                 arrays.append(None)
-                values.append(t)
+                values.append(_int32(t) if dtype == torch.int32 else t)
         if out is None:
             out = torch.empty(B, dtype=torch.int64, device=logits.device)
         self._need("sample", row(out, torch.int64))
         if B:
-            rc = self.lib.b2_sample(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), B, V, u.data_ptr(),
+            rc = self.lib.b2_sample(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), _int32(B), _int32(V), u.data_ptr(),
                                     *arrays, *values, out.data_ptr(), self._stream())
             self._check(rc, "b2_sample")
         return out

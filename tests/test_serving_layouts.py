@@ -63,3 +63,29 @@ def test_contiguous_rows_with_a_stride_of_one(kernels, native):
     want = run(qkv, caches, lambda t: t)
     got = run(turned(qkv), odd, turned)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_settings_beyond_an_int_of_c(kernels, native):
+    """A window, first tokens, a bound of rows or a top-k of 2^32 and more leave all that there is."""
+    k = kernels
+    if not native:
+        k = ops.Kernels()
+        k._append = k._attend = k._prefix = k._sample = None
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).to(torch.bfloat16)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    caches, table, lens, heads = (r(9, 2, 16, 64), r(9, 2, 16, 64)), ints(*range(9))[None], ints(140), (4, 2, 64)
+    args, far = (r(5, 256), *caches, table, lens, *heads), 2 ** 32 + 1
+    attend = lambda **kw: k.paged_attention(*args, cu_tokens=ints(0, 5), out=torch.zeros_like(args[0]), **kw)
+    want = attend(max_tokens=5)
+    assert torch.equal(attend(max_tokens=5, window=far), want)
+    assert torch.equal(attend(max_tokens=5, window=3, sinks=far), attend(max_tokens=5, window=3, sinks=140))
+    assert torch.equal(attend(max_tokens=far), attend(max_tokens=2 ** 31 - 1)) and (attend(max_tokens=far) != 0).any(1).all()
+    logits, u = r(1, 999), torch.full((1,), 0.9, device="cuda")
+    pick = lambda n: int(k.sample(logits, u, temperature=30.0, top_k=n))
+    assert pick(0) != pick(1) and pick(far) == pick(0) == pick(-far) == pick(-2 ** 40)
+    for bad in (dict(window=-far), dict(max_tokens=-far), dict(window=3, sinks=-far)):
+        with pytest.raises(RuntimeError, match="b2_paged_attention failed with code -1"):
+            attend(**bad)
