@@ -734,7 +734,10 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
   if (const int bad = check_rows(q, q_stride, c, c.B, Hq, scale, out, out_stride)) return bad;
   const int rep = Hq / c.Hk;
   if (prefix_width < 0) return kErrBadShape;
-  if ((long long)prefix_width * c.page > (1LL << 30)) return kErrTooLarge;
+  // (its tiles' blocks are counted in 31 bits too; several tiles are few rows' work only where there are few)
+  if ((long long)prefix_width * c.page > (1LL << 30) ||
+      (prefix_tiles(c.B, rep) == 1 && ((long long)prefix_width * c.page / kKeys + 2) * c.Hk > 0x7fffffffLL))
+    return kErrTooLarge;
   if (!prefix_len || (prefix_width > 0 && !prefix_table) || misaligned(prefix_table, 4) || misaligned(prefix_len, 4))
     return kErrBadPointer;
   if (sm_count < 1) return -sm_count;

@@ -89,3 +89,17 @@ def test_settings_beyond_an_int_of_c(kernels, native):
     for bad in (dict(window=-far), dict(max_tokens=-far), dict(window=3, sinks=-far)):
         with pytest.raises(RuntimeError, match="b2_paged_attention failed with code -1"):
             attend(**bad)
+
+
+def test_a_prefix_whose_blocks_31_bits_do_not_count(lib_path):
+    """One tile of rows reads 2^24 blocks of 64 keys for each of 256 heads: 2^32, which would count as none."""
+    lib = ops.load_library(lib_path)
+
+    def call(heads, width):
+        c = ops.PagedCache(k=A, v=A, page_stride=heads * 1024 * 64, head_stride=1024 * 64, token_stride=64, n_pages=4, page_size=1024,
+                           n_kv_heads=heads, head_dim=64, block_table=A, table_stride=8, table_width=8, n_seqs=2, seq_lens=A)
+        return lib.b2_shared_prefix_attention(A, heads * 64, ctypes.byref(c), A, width, A + 2, heads, 0.1, A, heads * 64, A, 1 << 40,
+                                              None)
+
+    assert call(256, 1 << 20) == call(128, 1 << 20) == -6
+    assert call(256, 1 << 18) == call(64, 1 << 20) == BAD_POINTER  # (the length's address, which is looked at next)
