@@ -103,7 +103,9 @@ int launch_pdl(void (*kernel)(Args...), dim3 grid, int block, size_t smem, cudaS
   return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Parts of a row joined by a warp, in the order of their keys: a lane holds D / 32 columns of the row.
+// Parts of a row joined by a warp, in the order of their keys: a lane holds D / 32 columns of the row.  They are added up in units of
+// the power of two that the heaviest weighs (its reference and its sum's exponent): a part is then no more than twice the average of
+// its values, whatever its sum in its own units (the kernel for many rows lets those grow).
 struct Part {
   const float2* stat;  // maximum (in powers of two) and sum
   const float* sums;   // D to a row
@@ -113,6 +115,9 @@ template <int D>
 struct Row {
   static constexpr int E = D / 32;
   float l = 0.f, o[E] = {};
+  static __device__ __forceinline__ float weighs(float2 stat) {
+    return stat.y == 0.f ? -INFINITY : stat.x + (float)((int)(__float_as_uint(stat.y) >> 23) - 127);
+  }
   template <typename F>
   __device__ __forceinline__ void join(int n, int lane, F part) {
     float m = -INFINITY;
@@ -127,9 +132,9 @@ struct Row {
     }
     for (int i = 64 + lane; i < n; i += 32) {
       const Part x = part(i);
-      m = fmaxf(m, __ldcg(x.stat + x.at).x);
+      m = fmaxf(m, weighs(__ldcg(x.stat + x.at)));
     }
-    m = fmaxf(m, fmaxf(kept[0].x, kept[1].x));
+    m = fmaxf(m, fmaxf(weighs(kept[0]), weighs(kept[1])));
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
     for (int i0 = 0; i0 < n; i0 += 32) {
@@ -141,7 +146,7 @@ struct Row {
           st = __ldcg(x.stat + x.at);
         }
       }
-      const float f = st.y == 0.f ? 0.f : st.x == m ? 1.f : ex2(st.x - m);
+      const float f = st.y == 0.f ? 0.f : ex2(st.x - m);
       l += f * st.y;
       const int here = min(32, n - i0);
       for (int i1 = 0; i1 < here; i1 += 8) {  // eight on their way at a time

@@ -14,7 +14,8 @@
 // The reference m of a row's weights is its maximum over the first block that it sees something of.  After that no maximum is
 // taken: weights over 1 are as exact as others, in fp32 and in bf16 alike, and a block whose weights add up to over 2^10 raises m
 // by the sum's exponent, for the next one; O is then rescaled in tensor memory, between the products that use it.  Where half a
-// block adds up to over 2^24 (scores that jump), m is taken anew at once, and that half's weights too: O stays under 2^25 |v|.
+// block adds up to over 2^24 (scores that jump), m is taken anew at once, and that half's weights too.  O stays under 2^10 |v| for
+// every block and another 2^25 |v|: under 2^128 for |v| < 2^100 over 2^17 blocks, for |v| < 2^94 over the 2^23 that a table may hold.
 // What bounds it: 128 x 128 scores of heads of 128 take the tensor core 1024 cycles (both products), and the 16 exponentials per
 // cycle of an SM as long.  An eighth of the exponentials are therefore polynomials on the multiply-add pipes, pairs at a time, and
 // the second product starts when half of the weights are there.  The products are issued by one thread without a branch between
