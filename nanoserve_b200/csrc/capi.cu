@@ -470,7 +470,9 @@ int b2_sample(const void* logits, long long logits_stride, int fp32, int rows, i
   p.top_p_all = top_p_all;
   p.min_p_all = min_p_all;
   p.tokens = static_cast<long long*>(tokens);
-  return b2::sample_launch(p, static_cast<cudaStream_t>(stream));
+  int rc = 0;
+  const int sms = sm_count_of_device(&rc);
+  return b2::sample_launch(p, rc ? -rc : sms, static_cast<cudaStream_t>(stream));
 }
 
 const char* b2_version(void) { return "nanoserve-b200 0.1 sm_100a"; }

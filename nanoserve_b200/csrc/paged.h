@@ -47,7 +47,7 @@ int shared_prefix_launch(const void* q, long long q_stride, const PagedCache& c,
                          int prefix_width, const int* prefix_len, int Hq, float scale, void* out, long long out_stride,
                          void* workspace, size_t workspace_bytes, int sm_count, cudaStream_t s);
 size_t shared_prefix_workspace(int B, int Hq, int Hk, int D, int sm_count);
-int sample_launch(const Sampling& p, cudaStream_t s);
+int sample_launch(const Sampling& p, int sm_count, cudaStream_t s);
 
 // Whether a wait of the kernels for few rows, or for many, ran out on device `dev`: added to *word, or cleared.  The caller has
 // synchronised.

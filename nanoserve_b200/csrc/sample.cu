@@ -783,10 +783,10 @@ int launch_on(const Sampling& p, cudaStream_t s) {
 }
 
 template <typename L>
-int launch(const Sampling& p, cudaStream_t s) {
+int launch(const Sampling& p, int sm_count, cudaStream_t s) {
   const size_t row = (size_t)p.V * sizeof(typename Keys<L>::Stored);
   int C = 1;
-  while (C < 8 && ((p.rows * C < 148 && p.V / C > 4096) || row / C > kSliceBytes)) C *= 2;
+  while (C < 8 && ((p.rows * C < sm_count && p.V / C > 4096) || row / C > kSliceBytes)) C *= 2;
   switch (C) {
     case 1: return launch_on<L, 1>(p, s);
     case 2: return launch_on<L, 2>(p, s);
@@ -797,13 +797,14 @@ int launch(const Sampling& p, cudaStream_t s) {
 
 }  // namespace
 
-int sample_launch(const Sampling& p, cudaStream_t s) {
+int sample_launch(const Sampling& p, int sm_count, cudaStream_t s) {
   if (p.rows < 1 || p.V < 1 || p.stride < 0) return kErrBadShape;
   if (p.V > kMaxVocab || p.rows > (1 << 20)) return kErrTooLarge;
   if (!p.logits || !p.u || !p.tokens || misaligned(p.logits, p.fp32 ? 4 : 2) || misaligned(p.u, 4) || misaligned(p.tokens, 8) ||
       misaligned(p.temperature, 4) || misaligned(p.top_k, 4) || misaligned(p.top_p, 4) || misaligned(p.min_p, 4))
     return kErrBadPointer;
-  return p.fp32 ? launch<float>(p, s) : launch<__nv_bfloat16>(p, s);
+  if (sm_count < 1) return -sm_count;
+  return p.fp32 ? launch<float>(p, sm_count, s) : launch<__nv_bfloat16>(p, sm_count, s);
 }
 
 }  // namespace b2
