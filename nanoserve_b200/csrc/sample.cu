@@ -784,9 +784,13 @@ int launch_on(const Sampling& p, cudaStream_t s) {
 
 template <typename L>
 int launch(const Sampling& p, int sm_count, cudaStream_t s) {
+  // As many CTAs to a row as the SMs take at once (one CTA fills one), down to 4096 logits each, and no fewer than a slice's shared
+  // memory asks for.  Twice as many, in two waves, were slower wherever that is a choice, 1.15 to 2.4 times (us, this rule and those
+  // in brackets, top-p alone / top-k 50 and top-p): 64 bf16 rows of 152064 66.4 / 34.0 (86.4 / 44.2), 70 67.2 / 34.0 (100.8 / 59.4);
+  // 20 rows of 40000 29.1 / 16.0 (45.0 / 25.4); 100 fp32 rows of 12000 27.0 / 13.9 (43.0 / 27.9).
   const size_t row = (size_t)p.V * sizeof(typename Keys<L>::Stored);
   int C = 1;
-  while (C < 8 && ((p.rows * C < sm_count && p.V / C > 4096) || row / C > kSliceBytes)) C *= 2;
+  while (C < 8 && ((2 * p.rows * C <= sm_count && p.V / C > 4096) || row / C > kSliceBytes)) C *= 2;
   switch (C) {
     case 1: return launch_on<L, 1>(p, s);
     case 2: return launch_on<L, 2>(p, s);
