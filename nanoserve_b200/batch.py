@@ -66,7 +66,7 @@ class Batch:
         u = self.u.index_select(0, self.step_no)[0]
         self.k.sample(self.logits, u, out=self.last, **self.sampling)
         self.tokens.index_copy_(0, self.step_no, self.last[None])
-        self.step_no += 1
+        self.step_no.add_(1).clamp_(max=self.max_own - 1)  # (a captured step replayed beyond the room goes on writing the last row)
 
     @torch.no_grad()
     def prefill(self, prefix: torch.Tensor, prompts: Sequence[torch.Tensor]):
@@ -107,8 +107,9 @@ class Batch:
 
     @torch.no_grad()
     def step(self):
-        """The next token of every sequence (nothing of it on the host: it can be captured).  A row without a token (-1: its logits
-        were not numbers) goes on from token 0."""
+        """The next token of every sequence (nothing of it on the host: it can be captured; replays beyond the room write the last row
+        of `tokens`, and keys that find no page are left out).  A row without a token (-1: its logits were not numbers) goes on from
+        token 0."""
         if self.left < 1:
             raise ValueError("no prefill, or no room for another token")
         self.left -= 1
