@@ -21,6 +21,10 @@ class Batch:
         if runner.world != 1:
             raise ValueError("a batch runs on one GPU")
         cfg, dev = runner.cfg, runner.dev
+        if n_seqs < 1 or max_own < 1 or max_prefix < 0:
+            raise ValueError(f"{n_seqs} sequences of up to {max_own} tokens behind up to {max_prefix}")
+        if page not in (16, 32, 64, 128, 256, 512, 1024) or cfg.head_dim not in (64, 128):
+            raise ValueError(f"pages of {page} tokens, heads of {cfg.head_dim}: a power of two from 16 to 1024, and 64 or 128")
         self.r, self.k, self.B, self.page, self.max_own = runner, runner.k, n_seqs, page, max_own
         self.heads = (cfg.n_heads, cfg.n_kv_heads, cfg.head_dim)
         self.n_shared = max_prefix // page

@@ -69,3 +69,15 @@ def test_a_captured_step_replayed_beyond_the_room(kernels):
     assert b.tokens[:-1].T.tolist() == [w[:-1] for w in want]
     assert ((b.tokens >= 0) & (b.tokens < 1024)).all()
     runner.check_status()
+
+
+@pytest.mark.parametrize("kw", [dict(n_seqs=0), dict(n_seqs=-1), dict(max_own=0), dict(max_prefix=-1), dict(page=8), dict(page=48),
+                                dict(page=2048), dict(head_dim=96)])
+def test_sizes_that_a_batch_does_not_take(kw):
+    """Refused when it is made: without a row of random numbers the first pick would end in a device assertion."""
+    d = dict(n_seqs=2, max_prefix=64, max_own=3, page=16)
+    runner = on_host(**{n: v for n, v in kw.items() if n == "head_dim"})
+    d.update({n: v for n, v in kw.items() if n != "head_dim"})
+    with pytest.raises(ValueError):
+        Batch(runner, **d)
+    Batch(on_host(), 1, 0, 1, page=1024)
