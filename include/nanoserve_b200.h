@@ -350,16 +350,18 @@ int b2_tp_wait(const void* wait_sig, const void* epoch, unsigned wait_per_epoch,
  *
  *   b2_paged_kv_append: qkv [T, (Hq + 2 Hk) D] (rows qkv_stride apart): + bias (may be NULL), rotate-half RoPE on q and k at the
  *     row's position (the angle in 64 bits), one rounding to bf16; q to q_out [T, Hq D] (rows q_stride apart), k and v to the cache.
- *     qkv is not modified.  A row whose position is negative is left out.  head_dim % 16 == 0, at most 256.
+ *     qkv is not modified.  A row whose position is negative is left out.  Where two rows of a call fall on one slot (a page that
+ *     two sequences' tables hold) it gets values of either.  head_dim % 16 == 0, at most 256.
  *   b2_paged_attention: out [T, Hq D] = softmax(scale q K^T) V; the row at position i sees the keys j <= i of its sequence and, with
  *     window > 0, of those only j > i - window and the first `sinks`.  A row that sees no key is zero.  head_dim 64 or 128,
  *     Hq % Hk == 0, 0 < scale < 2^127.  max_tokens: no sequence has more rows than that (rows beyond it are left as they are).
  *   b2_shared_prefix_attention: one row per sequence, which sees the first *prefix_len (int32, on the device) tokens of the pages
  *     prefix_table [prefix_width], and all seq_lens[b] tokens (which may be none) of its own pages.  The prefix's keys and values
  *     are read once for all sequences.
- *   Both: what no row of a call sees (slots behind a sequence's end, keys in front of every row's window) may hold anything.  A value
- *   (of v) that is infinite or not a number reaches the rows that see its key and, with several rows per sequence, may reach others
- *   of the same sequence.  Weighted values are added up in fp32 before they are divided by the sum of the weights: |v| < 2^100, or
+ *   Both: weights are rounded to bf16 for their product with v, as tensor cores take them (up to 2^-8 of the average |v|, beside the
+ *   result's own rounding); scores, sums and the division are in fp32.  What no row of a call sees (slots behind a sequence's end,
+ *   keys in front of every row's window) may hold anything.  A value (of v) that is infinite or not a number reaches the rows that
+ *   see its key and, with several rows per sequence, may reach others of the same sequence.  Weighted values are added up in fp32 before they are divided by the sum of the weights: |v| < 2^100, or
  *   2^94 where a row sees over 2^24 keys.
  *   T * Hq < 2^30, and (n_seqs + blocks of 64 keys that the tables hold, the prefix's too) * Hq < 2^31.
  *   Both take device scratch of the caller's, 16-byte aligned, of at least the bytes that the two size calls give, contents

@@ -8,8 +8,9 @@
 //
 // Bound by memory.  A thread moves eight (i, i + D/2) pairs of one head, two rows at a time, for rows the grid's length apart: while
 // its loads are on their way, a thread makes an angle of the next rows and a warp finds where the rows behind those belong, so that
-// nothing waits for the chain of row, sequence, page and angle (8065 rows of 28 / 4 heads of 128: 41 us with a CTA to a row and
-// its loads behind the chain, 30 us so; 16 rows 3.3 and 2.5 us).  Of these 30 us the 123 MB are 19 at HBM's pace.
+// nothing waits for the chain of row, sequence, page and angle (6665 rows of 28 / 4 heads of 128: 41 us with a CTA to a row and
+// its loads behind the chain, 29 us so; 16 rows 3.3 and 2.6 us).  Of these 29 us the 123 MB are 19 at HBM's pace; the rest is that a
+// row's loads live within one turn of the loop: issued at its top, used behind the next rows' angles (DRAM at 34 %).
 #include <algorithm>
 
 #include "paged_attention.cuh"

@@ -624,7 +624,7 @@ namespace {
 // How the kernel for many rows cuts a call up: tiles of 128 rows, two to a CTA where sequences have more; CTAs that would leave
 // SMs idle share the keys of a tile, down to two blocks of 128 each.  Where single tiles just fill the SMs, or over half of them,
 // they are a CTA's each: it then works on two blocks of keys at a time, which two CTAs would have to join (three chunks of
-// 150 to 517 tokens, 16 / 2 heads of 64: 22 us against 30 when it was chosen, 18.7 since).
+// 280 to 468 tokens, 16 / 2 heads of 64: 22 us against 30 when it was chosen, 18.7 since).
 struct ManyPlan {
   int two, slots, splits;
 };

@@ -21,10 +21,11 @@
 // the second product starts when half of the weights are there.  The products are issued by one thread without a branch between
 // them: with a choice of the lane and a barrier of the warp around each group that warp alone took 2900 cycles per 256 rows x 128
 // keys, where the products take 2048.  8192 new tokens in a window of 4096, 28 / 4 heads of 128: 333 us, 1080 TFLOP/s (a bf16 GEMM
-// here: 1670), at the board's power limit; with nothing done between the products 242 us.  Tried there: two threads to a row, so
-// that rows of half the length leave room in registers, 388 us where one took 353; every second, third or fourth pair a
-// polynomial 413, 358 and 357; the next block's scores in halves, beside the weights, 375 where 353 (products of 64 columns read
-// their operands twice); weights handed over as 96 and 32 keys 339 where 338.
+// here: 1670), in a long row of calls 380 to 390, 930, at the clock that the board's power limit leaves.  The tensor pipe is busy for
+// 53 % of it: what is left is the softmax's chain and its wait for the next scores (with nothing done between the products 242 us).
+// Tried there: two threads to a row, so that rows of half the length leave room in registers, 388 us where one took 353; every
+// second, third or fourth pair a polynomial 413, 358 and 357; the next block's scores in halves, beside the weights, 375 where 353
+// (products of 64 columns read their operands twice); weights handed over as 96 and 32 keys 339 where 338.
 // Every wait is bounded; a time-out is recorded in a word of this file's device image, which b2_device_status reads.
 #include <algorithm>
 
