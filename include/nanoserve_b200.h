@@ -361,8 +361,8 @@ int b2_tp_wait(const void* wait_sig, const void* epoch, unsigned wait_per_epoch,
  *   Both: weights are rounded to bf16 for their product with v, as tensor cores take them (up to 2^-8 of the average |v|, beside the
  *   result's own rounding); scores, sums and the division are in fp32.  What no row of a call sees (slots behind a sequence's end,
  *   keys in front of every row's window) may hold anything.  A value (of v) that is infinite or not a number reaches the rows that
- *   see its key and, with several rows per sequence, may reach others of the same sequence.  Weighted values are added up in fp32 before they are divided by the sum of the weights: |v| < 2^100, or
- *   2^94 where a row sees over 2^24 keys.
+ *   see its key and, with several rows per sequence, may reach others of the same sequence.  Weighted values are added up in fp32
+ *   before they are divided by the sum of the weights: |v| < 2^100, or 2^94 where a row sees over 2^24 keys.
  *   T * Hq < 2^30, and (n_seqs + blocks of 64 keys that the tables hold, the prefix's too) * Hq < 2^31.
  *   Both take device scratch of the caller's, 16-byte aligned, of at least the bytes that the two size calls give, contents
  *   undefined before and after; calls that may overlap in time need scratch of their own.

@@ -570,8 +570,8 @@ class Kernels:
             out = torch.empty(B, dtype=torch.int64, device=logits.device)
         self._need("sample", row(out, torch.int64))
         if B:
-            rc = self.lib.b2_sample(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), _int32(B), _int32(V), u.data_ptr(),
-                                    *arrays, *values, out.data_ptr(), self._stream())
+            rc = self.lib.b2_sample(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), _int32(B), _int32(V),
+                                    u.data_ptr(), *arrays, *values, out.data_ptr(), self._stream())
             self._check(rc, "b2_sample")
         return out
 
